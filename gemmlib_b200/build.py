@@ -86,8 +86,8 @@ def build_ext(force: bool = False) -> str:
     """Build the PyTorch extension ``ms_blkq4linear_ext`` next to the library it links."""
     build_lib()
     out = ext_path()
-    src = os.path.join(CSRC, "ms_blkq4linear_ext.cpp")
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(LIB)):
+    sources = sorted(glob.glob(os.path.join(CSRC, "*_ext.cpp")))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(_newest(sources), os.path.getmtime(LIB)):
         return out
     import sysconfig
 
@@ -96,16 +96,26 @@ def build_ext(force: bool = False) -> str:
 
     inc = cpp_extension.include_paths("cuda")
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + os.path.join(ROOT, "include"), "-I" + sysconfig.get_paths()["include"]]
     cmd += ["-isystem" + p for p in inc]
-    cmd += [src, "-o", out, "-L" + PKG, "-l:libms_blkq4gemm.so", "-Wl,-rpath,$ORIGIN",
-            "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-            "-Wl,-rpath," + tlib]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("building ms_blkq4linear_ext failed:\n" + r.stdout + r.stderr)
+    objs = [os.path.join(OBJ, os.path.basename(src)[:-4] + ".o") for src in sources]
+    hdr_time = _newest(glob.glob(os.path.join(ROOT, "include", "*.h")) + [os.path.abspath(__file__)])
+
+    def run(c):
+        r = subprocess.run(c, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("building ms_blkq4linear_ext failed:\n" + r.stdout + r.stderr)
+
+    jobs = [cmd + ["-c", src, "-o", obj] for src, obj in zip(sources, objs)
+            if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), hdr_time)]
+    if jobs:
+        with ThreadPoolExecutor(max_workers=len(jobs)) as ex:
+            list(ex.map(run, jobs))
+    run(["g++", "-shared", *objs, "-o", out, "-L" + PKG, "-l:libms_blkq4gemm.so", "-Wl,-rpath,$ORIGIN",
+         "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+         "-Wl,-rpath," + tlib])
     return out
 
 

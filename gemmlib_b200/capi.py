@@ -47,6 +47,15 @@ SYMBOLS = (
     "blkq4_version",
 )
 
+INT8_SYMBOLS = (
+    "int8_rows_quant_sm100",
+    "int8_rows_rms_norm_sm100",
+    "int8_rows_silu_mul_sm100",
+    "int8_rows_dequant_sm100",
+    "int8_gemm_sm100",
+)
+INT8_FP16, INT8_BF16 = 0, 1
+
 
 class BlkQ4Error(RuntimeError):
     pass
@@ -131,6 +140,15 @@ def _load() -> ctypes.CDLL:
     lib.blkq4_gather_status.restype = i
     lib.blkq4_gather_destroy.argtypes = [vp]
     lib.blkq4_gather_destroy.restype = i
+    i64 = ctypes.c_int64
+    matrix, vector = [vp, sz, i64], [vp, sz]
+    lib.int8_rows_quant_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *vector, vp]
+    lib.int8_rows_rms_norm_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *vector, ctypes.c_float, *matrix, *matrix, *vector, vp]
+    lib.int8_rows_silu_mul_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *matrix, *vector, vp]
+    lib.int8_rows_dequant_sm100.argtypes = [i, i, i, vp, *matrix, *vector, *matrix, vp]
+    lib.int8_gemm_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, *matrix, *vector, *vector, *matrix, ctypes.c_uint, vp]
+    for name in INT8_SYMBOLS:
+        getattr(lib, name).restype = i
     return lib
 
 
@@ -388,3 +406,37 @@ class GatherContext:
                               "its device block is left allocated", ResourceWarning)
         except Exception:
             pass
+
+
+# ---- 8-bit path: a matrix is (tensor or (pointer, bytes), leading dimension), None for a null pointer ----
+def _matrix(m):
+    return (0, 0, 0) if m is None else (*_ptr_size(m[0]), m[1])
+
+
+def _int8_call(fn, *args):
+    with _ErrMsg() as e:
+        if fn(*args, e.p) != 0:
+            raise BlkQ4Error(e.text())
+
+
+def int8_rows_quant(dtype, rows, cols, x, values, scales, stream=0):
+    _int8_call(lib.int8_rows_quant_sm100, dtype, rows, cols, stream, *_matrix(x), *_matrix(values), *_ptr_size(scales))
+
+
+def int8_rows_rms_norm(dtype, rows, cols, x, residual, weight, eps, residual_out, values, scales, stream=0):
+    _int8_call(lib.int8_rows_rms_norm_sm100, dtype, rows, cols, stream, *_matrix(x), *_matrix(residual), *_ptr_size(weight), eps,
+               *_matrix(residual_out), *_matrix(values), *_ptr_size(scales))
+
+
+def int8_rows_silu_mul(dtype, rows, cols, gate, up, values, scales, stream=0):
+    _int8_call(lib.int8_rows_silu_mul_sm100, dtype, rows, cols, stream, *_matrix(gate), *_matrix(up), *_matrix(values),
+               *_ptr_size(scales))
+
+
+def int8_rows_dequant(dtype, rows, cols, values, scales, out, stream=0):
+    _int8_call(lib.int8_rows_dequant_sm100, dtype, rows, cols, stream, *_matrix(values), *_ptr_size(scales), *_matrix(out))
+
+
+def int8_gemm(dtype, m, n, k, x, x_scales, w, w_scales, bias, out, flags=0, stream=0):
+    _int8_call(lib.int8_gemm_sm100, dtype, m, n, k, stream, *_matrix(x), *_ptr_size(x_scales), *_matrix(w), *_ptr_size(w_scales),
+               *_ptr_size(bias), *_matrix(out), flags)

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "blkq4_common.cuh"
+#include "int8.cuh"
 #include "ms_blkq4gemm.h"
 
 namespace {
@@ -314,7 +315,9 @@ extern "C" int blkq4_last_kernel_status(void* stream_ptr) {
   const int gv = blkq4::read_gemv_error();
   if (gv != 0) return gv > 0 ? (0x10000 | gv) : gv;
   const int sk = blkq4::read_skinny_tc_error();
-  return sk > 0 ? (0x20000 | sk) : sk;
+  if (sk != 0) return sk > 0 ? (0x20000 | sk) : sk;
+  const int i8 = blkq4::int8::read_gemm_error();
+  return i8 > 0 ? (0x40000 | i8) : i8;
 }
 extern "C" int blkq4_reset(void* stream_ptr) {
   auto stream = reinterpret_cast<cudaStream_t>(stream_ptr);
@@ -322,6 +325,7 @@ extern "C" int blkq4_reset(void* stream_ptr) {
   rc |= blkq4::clear_gemm_tc_error(stream);
   rc |= blkq4::clear_gemv_error(stream);
   rc |= blkq4::clear_skinny_tc_error(stream);
+  rc |= blkq4::int8::clear_gemm_error(stream);
   rc |= blkq4::reset_static_scratch(stream);
   return rc == 0 ? 0 : -1;
 }

@@ -1,0 +1,364 @@
+// Product of int8 rows for sm_100a: out[m, n] = T(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]).
+//
+// Both operands are K-major rows of bytes as they lie in memory: TMA brings 128 k of a tile at a time into shared memory with
+// the 128-byte swizzle, tcgen05.mma (kind::i8) multiplies them from there and adds in int32 in tensor memory.  The sums are exact,
+// so neither the tiles nor the split of K show in the result; the two scales and the bias are applied in fp32 and the
+// result is rounded once.
+//
+// gemm_rows_kernel: 128 weight rows (TMEM lanes) x up to 256 activation rows per tile, so that few rows waste no weights'
+// bandwidth; the K range of a tile is split over a cluster of CTAs, which exchange their int32 parts through distributed shared
+// memory.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstddef>
+#include <cstdint>
+#include <string>
+
+#include "blkq4_common.cuh"
+#include "blkq4_tc.cuh"
+#include "blkq4_tma.cuh"
+#include "int8.cuh"
+#include "ms_blkq4gemm.h"
+
+namespace blkq4 {
+namespace int8 {
+
+__device__ int g_int8_error = 0;  // 0 ok; otherwise (role << 8) | stage of the wait that gave up
+
+namespace {
+
+constexpr int kStepK = 128;                 // k of a pipeline step: one 128-byte swizzle row
+constexpr int kTileN = 128;                 // weight rows of a tile
+constexpr uint32_t kWeightBytes = kTileN * kStepK;
+constexpr long long kWaitCycles = 4000000000ll;  // ~2 s: far beyond any legitimate wait
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  return mbar_wait_bounded(bar, parity, abort_flag, &g_int8_error, who, kWaitCycles);
+}
+// Instruction descriptor of kind::i8: int32 accumulator (bits 4-5 = 2), signed A and B (bits 7-9 and 10-12 = 1), both K-major,
+// N >> 3 in bits 17-22, M >> 4 in bits 24-28.
+__host__ __device__ inline uint32_t make_idesc_i8(int umma_m, int umma_n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(umma_n >> 3) << 17) | ((uint32_t)(umma_m >> 4) << 24);
+}
+// The four MMAs of a step: 32 k each, both operands two descriptor units (32 bytes) further on.
+__device__ __forceinline__ void umma_i8_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\t"
+      "add.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+      "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+      "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], a0, b0, %4, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], a1, b1, %4, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], a2, b2, %4, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], a3, b3, %4, q;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void st_shared_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+struct Params {
+  int M, N;
+  int BM;          // activation rows of a tile, a multiple of 16, <= 256
+  int m_tiles;
+  int k_steps;     // of a tile
+  int split;       // CTAs of a tile: the cluster size
+  int k_per_cta;   // steps of each, the last one what is left
+  int slice;       // activation rows whose sums one CTA of the cluster collects, a multiple of 8
+  int stages;
+  int early;       // weights may be copied before the kernels ahead in the stream have completed
+  uint32_t stage_bytes, tmem_cols;
+  int pairs;       // two neighbouring outputs of a row may be stored at once
+  void* out;
+  int64_t ldo;
+  const float* x_scales;
+  const float* w_scales;
+  const void* bias;
+};
+
+constexpr int kMaxStages = 16;
+constexpr int kEpiWarps = 4, kThreads = 32 * (2 + kEpiWarps);
+constexpr uint32_t kBarBytes = 512;  // full[], empty[], accumulator, abort flag, TMEM address
+
+// Grid: tiles * split CTAs, those of a tile a cluster.  The m tiles of a column tile follow one another.
+template <class T>
+__global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                             const __grid_constant__ CUtensorMap tm_w, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + (uint32_t)p.stages * p.stage_bytes;
+  uint8_t* bars_ptr = base_ptr + (size_t)p.stages * p.stage_bytes;
+  auto full = [&](int s) { return bars + 16u * (uint32_t)s; };
+  auto empty = [&](int s) { return bars + 16u * (uint32_t)s + 8u; };
+  const uint32_t acc_full = bars + 16u * kMaxStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 16 * kMaxStages + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + 16 * kMaxStages + 12);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(p.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int tile = (int)blockIdx.x / p.split, part = (int)blockIdx.x % p.split;
+  const int m0 = tile % p.m_tiles * p.BM, n0 = tile / p.m_tiles * kTileN;
+  const int ks0 = part * p.k_per_cta, count = min(p.k_per_cta, p.k_steps - ks0);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t tx = kWeightBytes + (uint32_t)p.BM * kStepK;
+      const int ahead = min(count, p.stages);
+      if (p.early) {
+        for (int i = 0; i < ahead; ++i) {
+          mbar_arrive_expect_tx(full(i), tx);
+          tma_load_2d(base + i * p.stage_bytes, &tm_w, (ks0 + i) * kStepK, n0, full(i));
+        }
+      } else {  // at least on their way into L2, where a write that is still to come would find them
+        for (int i = 0; i < ahead; ++i) prefetch_l2_2d(&tm_w, (ks0 + i) * kStepK, n0);
+      }
+      griddep_wait();
+      for (int i = 0; i < count; ++i) {
+        const int s = i % p.stages;
+        if (i >= p.stages && !wait(empty(s), ((i / p.stages) - 1) & 1, abort_flag, 0x100 | s)) break;
+        if (i >= ahead || !p.early) {
+          mbar_arrive_expect_tx(full(s), tx);
+          tma_load_2d(base + s * p.stage_bytes, &tm_w, (ks0 + i) * kStepK, n0, full(s));
+        }
+        tma_load_2d(base + s * p.stage_bytes + kWeightBytes, &tm_x, (ks0 + i) * kStepK, m0, full(s));
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_i8(kTileN, p.BM);
+      const uint64_t desc = tc::make_sw128_kmajor_desc(0);
+      const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc;
+      bool ok = true;
+      for (int i = 0; i < count; ++i) {
+        const int s = i % p.stages;
+        if (!wait(full(s), (i / p.stages) & 1, abort_flag, 0x200 | s)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t w_addr = base + s * p.stage_bytes;
+        umma_i8_x4(tmem, desc_lo | ((w_addr >> 4) & 0x3FFFu), desc_lo | (((w_addr + kWeightBytes) >> 4) & 0x3FFFu), desc_hi, idesc,
+                   i > 0);
+        tc::umma_commit(empty(s));
+      }
+      if (ok) tc::umma_commit(acc_full);
+    }
+  } else {
+    griddep_wait();  // scales of the activations and the output belong to stream order
+    wait(acc_full, 0, abort_flag, 0x300);
+  }
+  __syncwarp();
+  auto dead = [&] { return __shfl_sync(0xffffffffu, *abort_flag, 0) != 0; };  // one answer a warp
+
+  // ---- the parts of a split tile: CTA o of the cluster collects the sums of activation rows [o * slice, (o + 1) * slice)
+  // in its stages, [part][row][128], which every CTA of the cluster is done with after the first barrier.
+  const int rows = min(p.BM, p.M - m0);
+  const int quarter = warp & 3, n_l = quarter * 32 + lane;  // TMEM lanes of an epilogue warp: a quarter, by warp number mod 4
+  const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
+  if (p.split > 1) {
+    __syncthreads();
+    tc::cluster_sync_all();
+    if (warp >= 2 && !dead()) {
+      tc::tc_fence_after();
+      for (int o = 0; o < p.split; ++o) {
+        if (o == part) continue;
+        const int end = min(rows, (o + 1) * p.slice);
+        const uint32_t dst = tc::map_to_cta(base + (uint32_t)((part - (part > o)) * p.slice * kTileN + n_l) * 4u, (uint32_t)o);
+        for (int m = o * p.slice; m < end; m += 8) {
+          uint32_t r[8];
+          tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (m + j < end) st_shared_cluster_u32(dst + (uint32_t)((m + j - o * p.slice) * kTileN) * 4u, r[j]);
+        }
+      }
+    }
+    __syncwarp();
+    tc::cluster_sync_all();
+  }
+
+  if (warp >= 2 && !dead()) {
+    tc::tc_fence_after();
+    const int n = n0 + n_l;
+    const float w_scale = n < p.N ? p.w_scales[n] : 0.0f;
+    const float bias = p.bias && n < p.N ? to_float(reinterpret_cast<const T*>(p.bias)[n]) : 0.0f;
+    const int first = part * p.slice, end = min(rows, first + p.slice);
+    const uint32_t* parts = reinterpret_cast<const uint32_t*>(base_ptr) + n_l;
+    T* out = reinterpret_cast<T*>(p.out);
+    const int odd = lane & 1;
+    for (int m = first; m < end; m += 8) {
+      uint32_t r[8];
+      tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
+      tc::tmem_ld_wait();
+      for (int q = 0; q < p.split - 1; ++q) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (m + j < end) r[j] += parts[(size_t)(q * p.slice + m + j - first) * kTileN];
+      }
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x_scale = m + j < end ? p.x_scales[m0 + m + j] : 0.0f;
+        v[j] = fmaf((float)(int)r[j] * x_scale, w_scale, bias);
+      }
+      if (p.pairs) {
+        // lanes of an even and an odd n trade: the even one stores the even row's two values, the odd one the odd row's
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float give = odd ? v[j] : v[j + 1], keep = odd ? v[j + 1] : v[j];
+          const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+          const uint32_t both = odd ? pack2<T>(got, keep) : pack2<T>(keep, got);
+          if (m + j + odd < end && n < p.N)  // N is even: n and its partner are inside together
+            *reinterpret_cast<uint32_t*>(out + (int64_t)(m0 + m + j + odd) * p.ldo + (n & ~1)) = both;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (m + j < end && n < p.N) out[(int64_t)(m0 + m + j) * p.ldo + n] = from_float<T>(v[j]);
+      }
+    }
+  }
+  __syncwarp();
+
+  tc::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) __nanosleep(50000);  // let copies in flight land
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+  }
+}
+
+// K-major rows of bytes `ld` apart.
+bool encode_rows(CUtensorMap* map, const int8_t* ptr, int64_t ld, int K, int rows, int box_rows) {
+  TensorMapEncodeFn fn = tensor_map_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)kStepK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(ptr), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct RowsPlan {
+  int BM, m_tiles, n_tiles, split, k_per_cta, slice, stages;
+  uint32_t stage_bytes, smem;
+};
+RowsPlan plan_rows(int M, int N, int K, int sms) {
+  RowsPlan r{};
+  r.m_tiles = (M + 255) / 256;
+  r.BM = ((M + r.m_tiles - 1) / r.m_tiles + 15) / 16 * 16;
+  r.n_tiles = (N + kTileN - 1) / kTileN;
+  r.stage_bytes = kWeightBytes + (uint32_t)r.BM * kStepK;
+  const int k_steps = (K + kStepK - 1) / kStepK;
+  // two CTAs of an SM where their stages are small, else one
+  const uint32_t ring = r.BM <= 128 ? 108u * 1024 : 216u * 1024;
+  r.stages = std::min<int>(kMaxStages, (int)(ring / r.stage_bytes));
+  const int slots = sms * (r.BM <= 128 ? 2 : 1), tiles = r.m_tiles * r.n_tiles;
+  r.split = std::max(1, std::min({8, slots / tiles, k_steps / 2}));
+  r.k_per_cta = (k_steps + r.split - 1) / r.split;
+  r.split = (k_steps + r.k_per_cta - 1) / r.k_per_cta;
+  const int rows = std::min(M, r.BM);
+  r.slice = r.split > 1 ? ((rows + r.split - 1) / r.split + 7) / 8 * 8 : r.BM;
+  r.smem = (uint32_t)r.stages * r.stage_bytes + kBarBytes + 1024;
+  return r;
+}
+
+template <class T>
+std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
+  const int sms = sm_count();
+  const RowsPlan r = plan_rows(g.M, g.N, g.K, sms);
+  CUtensorMap tm_x, tm_w;
+  if (!encode_rows(&tm_x, g.x, g.ldx, g.K, g.M, r.BM) || !encode_rows(&tm_w, g.w, g.ldw, g.K, g.N, kTileN))
+    return "cuTensorMapEncodeTiled failed";
+  Params p{};
+  p.M = g.M; p.N = g.N;
+  p.BM = r.BM; p.m_tiles = r.m_tiles;
+  p.k_steps = (g.K + kStepK - 1) / kStepK;
+  p.split = r.split; p.k_per_cta = r.k_per_cta; p.slice = r.slice; p.stages = r.stages;
+  p.early = (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0;
+  p.stage_bytes = r.stage_bytes;
+  p.tmem_cols = 32;
+  while ((int)p.tmem_cols < r.BM) p.tmem_cols *= 2;
+  p.pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
+  p.out = g.out; p.ldo = g.ldo;
+  p.x_scales = g.x_scales; p.w_scales = g.w_scales; p.bias = g.bias;
+  static std::atomic<int> granted[64];
+  cudaError_t e = ensure_dynamic_smem(gemm_rows_kernel<T>, r.smem, granted);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(r.m_tiles * r.n_tiles * r.split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = r.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)r.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = r.split > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, gemm_rows_kernel<T>, tm_x, tm_w, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
+}
+
+}  // namespace
+
+std::string launch_gemm(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream) {
+  return dtype == kFp16 ? launch_rows_gemm<__half>(g, flags, stream) : launch_rows_gemm<__nv_bfloat16>(g, flags, stream);
+}
+
+int read_gemm_error() {
+  int v = 0;
+  return cudaMemcpyFromSymbol(&v, g_int8_error, sizeof(int)) == cudaSuccess ? v : -1;
+}
+int clear_gemm_error(cudaStream_t stream) {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_int8_error) != cudaSuccess) return -1;
+  return cudaMemsetAsync(p, 0, sizeof(int), stream) == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace int8
+}  // namespace blkq4

@@ -323,6 +323,80 @@ int blkq4_gather_supported_sm100(int block_size, bool column_wise_blocking, int 
 int blkq4_gather_destroy(void* ctx);
 
 /*
+ * The 8-bit path: rows of int8 with one fp32 scale each - activations by token, weights by output channel - what produces them,
+ * and their product.  No counterpart in the reference.
+ *
+ *   - A row stands for scale * values.  scale = max|t| / 127 and values[k] = round(t[k] * (127 / max|t|)), half to even, where t
+ *     is the row to be quantized in fp32.  A row of zeros has scale 0.  A row that holds an infinity or NaN (or whose sum with
+ *     the residual overflows the 16-bit type) has scale NaN and values 0, so that whatever reads it is NaN in that row only.
+ *   - dtype: INT8_FP16 or INT8_BF16, the type of the 16-bit operands of the call.
+ *   - ld*: elements from row to row (of an int8 matrix: bytes), at least the row's length.  *_size: bytes that may be
+ *     accessed, at least those from the first to the last element.  Rows that all begin on 16 bytes (int8 ones of the first
+ *     three calls: on 8) are read and written in vectors, others one element at a time with the same results.
+ *   - Columns up to 2^28.  The norm's sum of squares is held in fp32: |x| up to 1e17.
+ */
+#define INT8_FP16 0
+#define INT8_BF16 1
+
+/** values, scales = rows of x [rows, cols] (activations, or weights [out_features, in_features]). */
+int int8_rows_quant_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size,
+  void* error_message);
+
+/**
+ * RMS norm: t = h / sqrt(mean(h^2) + eps) * weight, with h = x + residual rounded to the 16-bit type, or x without a
+ * residual (null).  With one, h is written to residual_out, which may be x or residual itself (same ld) but may not overlap
+ * them otherwise.  The sum of squares, the factor and t are held in fp32.
+ */
+int int8_rows_rms_norm_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* residual, size_t residual_size, int64_t ldr,
+  void const* weight, size_t weight_size, float eps,
+  void* residual_out, size_t residual_out_size, int64_t ldo,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size,
+  void* error_message);
+
+/** t = gate / (1 + exp(-gate)) * up: the input of a feed-forward block's last projection. */
+int int8_rows_silu_mul_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* gate, size_t gate_size, int64_t ldg,
+  void const* up, size_t up_size, int64_t ldu,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size,
+  void* error_message);
+
+/** out = scale * values, rounded to the 16-bit type. */
+int int8_rows_dequant_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* values, size_t values_size, int64_t ldv,
+  void const* scales, size_t scales_size,
+  void* out, size_t out_size, int64_t ldo,
+  void* error_message);
+
+/**
+ * out[m, n] = x_scales[m] * w_scales[n] * sum over k of x[m, k] w[n, k] (+ bias[n]), for any m, n and k up to 131071.  The sums
+ * are exact (int32); scales and bias are applied in fp32 and the result is rounded to the 16-bit type once.  bias: [n] of that
+ * type, or null.  x and w: 16-byte aligned, ldx and ldw multiples of 16.
+ * BLKQ4_GEMM_EARLY_WEIGHT_FETCH: the caller vouches that w (not w_scales or bias) is not written by any work still pending on
+ * `stream`; its first tiles are then fetched while the preceding kernel still runs.
+ */
+int int8_gemm_sm100(
+  int dtype, int m, int n, int k, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* x_scales, size_t x_scales_size,
+  void const* w, size_t w_size, int64_t ldw,
+  void const* w_scales, size_t w_scales_size,
+  void const* bias, size_t bias_size,
+  void* out, size_t out_size, int64_t ldo,
+  unsigned flags,
+  void* error_message);
+
+/*
  * Additions with no counterpart in the reference.  The reference reports errors
  * through a std::string*, which only a C++ caller can supply.  These three let
  * a C, ctypes, cgo or JNI caller own such an object.
@@ -336,7 +410,7 @@ void blkq4_errmsg_destroy(void* errmsg);      /* delete                         
  * every in-kernel wait completed.  Waits on mbarriers are bounded; one that expires makes
  * the CTA drain and records (role << 8 | barrier) here instead of hanging the GPU (the
  * skinny kernel's word is reported with bit 16 set, that of the tensor-core kernel of up to 16 rows
- * with bit 17).  -1 if the stream itself is in error.
+ * with bit 17, that of the int8 product with bit 18).  -1 if the stream itself is in error.
  * No counterpart in the reference, whose kernels have no such waits.
  */
 int blkq4_last_kernel_status(void* stream);

@@ -1,0 +1,295 @@
+"""int8 rows on the GPU, against their definition in 64 bits.
+
+Bounds.  u = 127 t / max|t| is what the values round.  The kernel multiplies t with fp32(127 / max|t|), off by 2^-24 of itself, and
+rounds the product once: |u - value| <= 1/2 + 127 * 2^-24, for t known exactly.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+EPS24 = 2.0 ** -24
+TYPES = [torch.float16, torch.bfloat16]
+# one to many threads and chunks a row, rows that end inside a vector, and a row read twice (over 32768)
+WIDTHS = [1, 2, 7, 8, 9, 16, 100, 128, 255, 512, 513, 1000, 2048, 2056, 4096, 5001, 8192, 8200, 11008, 28672, 32768, 32769, 40000]
+
+
+def ids(v):
+    return str(v).replace("torch.", "")
+
+
+def normal(*shape, dtype, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def check_rows(rows, t, factor=None, t_error=0.0, factor_error=0.0):
+    """`t`: the rows in 64 bits, known up to the relative error t_error (a number or a tensor like t); `factor`: by row, times the
+    scale."""
+    values, scales = rows
+    assert values.dtype == torch.int8 and values.shape == t.shape and scales.dtype == torch.float32
+    assert scales.shape == t.shape[:-1]
+    top = t.abs().amax(-1, keepdim=True)
+    error = torch.as_tensor(t_error, device=t.device, dtype=torch.float64).expand_as(t)
+    top_error = error.amax()
+    u = torch.where(top > 0, 127 * t / torch.where(top > 0, top, 1.0), 0.0)
+    off = (u - values.double()).abs()
+    assert (off <= 0.5 + 127 * EPS24 + u.abs() * (error + top_error) * 1.01).all(), float((off - 0.5).max())
+    want = top[..., 0] / 127 * (1.0 if factor is None else factor)
+    # below 2^-126 floats are 2^-149 apart, so that a rounding is off by up to 2^-150 whatever the value
+    assert ((scales.double() - want).abs() <= want * (EPS24 * 1.01 + top_error * 1.01 + factor_error) + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_quantize(dtype, cols):
+    from gemmlib_b200.int8_linear import quantize_int8
+
+    x = normal(5, cols, dtype=dtype, seed=cols)
+    x[2] = 0
+    x[3] *= 1e-3
+    rows = quantize_int8(x)
+    check_rows(rows, x.double())
+    assert rows.scales[2] == 0 and not rows.values[2].any()
+    assert int(rows.values[0].abs().max()) == 127
+    if cols > 1:
+        assert rows.values.stride(0) % 16 == 0  # rows that the product takes as they are
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [1, 3, 4, 5, 127, 1000])
+@pytest.mark.parametrize("cols", [64, 4096])
+def test_quantize_many_rows(dtype, rows, cols):
+    from gemmlib_b200.int8_linear import quantize_int8
+
+    x = normal(rows, cols, dtype=dtype, seed=rows)
+    check_rows(quantize_int8(x), x.double())
+
+
+def test_rounding_is_half_to_even_and_symmetric():
+    from gemmlib_b200.int8_linear import quantize_int8
+
+    # max 127: the values are the inputs themselves, rounded
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 0.499, 126.5, -126.5, -127.0, 3.0]], dtype=torch.float16, device="cuda")
+    assert quantize_int8(x).values.tolist() == [[127, 0, 2, 2, 0, -2, -2, 0, 126, -126, -127, 3]]
+
+
+def test_extreme_magnitudes():
+    from gemmlib_b200.int8_linear import quantize_int8
+
+    for dtype, top in ((torch.float16, [65504.0, 2.0 ** -24, 2.0 ** -14]), (torch.bfloat16, [3.3e38, 1e-30, 2.0 ** -126])):
+        x = torch.tensor([[t, -t / 2, 0.0, t / 4] for t in top], dtype=torch.float64, device="cuda").to(dtype)
+        check_rows(quantize_int8(x), x.double())
+    # a scale below the smallest normal float keeps what bits it has: within half a step of 2^-149
+    x = torch.tensor([[2.0 ** -133, -(2.0 ** -133), 0.0]], dtype=torch.bfloat16, device="cuda")
+    r = quantize_int8(x)
+    assert r.values.tolist() == [[127, -127, 0]]
+    assert abs(float(r.scales[0].double()) - 2.0 ** -133 / 127) <= 2.0 ** -150
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("cols,at", [(1, 0), (40, 39), (4096, 4095), (5001, 5000), (40000, 39999)])
+def test_a_row_with_an_infinity_or_nan_is_nan_alone(dtype, bad, cols, at):
+    from gemmlib_b200.int8_linear import quantize_int8, rms_norm_int8, silu_mul_int8
+
+    x = normal(3, cols, dtype=dtype)
+    x[1, at] = bad
+    w = torch.ones(cols, dtype=dtype, device="cuda")
+    w[at] = 0  # 0 * inf is NaN
+    good = normal(3, cols, dtype=dtype, seed=1)
+    made = [quantize_int8(x), rms_norm_int8(x, w), rms_norm_int8(good, w, residual=x)[0], silu_mul_int8(good, x)]
+    for r in made:
+        assert torch.isnan(r.scales).tolist() == [False, True, False]
+        assert not r.values[1].any() and torch.isnan(r.dequantize(dtype)[1]).all()
+        assert torch.isfinite(r.dequantize(dtype)[[0, 2]]).all()
+
+
+def norm_reference(h, w, eps):
+    h, w = h.double(), w.double()
+    return h * w, 1 / torch.sqrt(h.square().mean(-1) + eps)
+
+
+# fp32 sums of up to 64 squares a thread and a tree of ten: (64 + 10 + 2) * 2^-24, halved by the root, and five more roundings
+NORM_ERROR = 43 * EPS24
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_rms_norm(dtype, residual, cols):
+    from gemmlib_b200.int8_linear import rms_norm_int8
+
+    x, w = normal(5, cols, dtype=dtype, seed=cols), normal(cols, dtype=dtype, seed=7)
+    x[3] *= 100
+    eps = 1e-5
+    if residual:
+        r = normal(5, cols, dtype=dtype, seed=cols + 1, scale=3.0)
+        rows, h = rms_norm_int8(x, w, eps, residual=r)
+        assert torch.equal(h, x + r)
+    else:
+        x[2] = 0
+        rows, h = rms_norm_int8(x, w, eps), x
+        assert rows.scales[2] == 0
+    t, factor = norm_reference(h, w, eps)
+    check_rows(rows, t, factor, factor_error=NORM_ERROR)
+
+
+@pytest.mark.parametrize("place", ["x", "residual", "other", "slice of x's matrix"])
+@pytest.mark.parametrize("cols", [256, 40000])
+def test_rms_norm_residual_out_in_place(place, cols):
+    from gemmlib_b200.int8_linear import rms_norm_int8
+
+    both = normal(6, 2 * cols, dtype=torch.float16)
+    x, r, w = both[:, :cols], normal(6, cols, dtype=torch.float16, seed=1), normal(cols, dtype=torch.float16, seed=2)
+    want, sum_ = rms_norm_int8(x, w, residual=r)
+    keep = both[:, cols:].clone()
+    out = {"x": x, "residual": r, "other": torch.empty_like(r), "slice of x's matrix": both[:, cols:]}[place]
+    rows, h = rms_norm_int8(x, w, residual=r, residual_out=out)
+    assert h.data_ptr() == out.data_ptr() and torch.equal(out, sum_)
+    assert torch.equal(rows.values, want.values) and torch.equal(rows.scales, want.scales)
+    if place == "x":
+        assert torch.equal(both[:, cols:], keep)
+
+
+def test_rms_norm_refusals():
+    from gemmlib_b200.int8_linear import rms_norm_int8
+
+    both = normal(4, 64, dtype=torch.float16)
+    x, w = both[:, :32], normal(32, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="not overlap them otherwise"):
+        rms_norm_int8(x, w, residual=x.clone(), residual_out=both[:, 16:48])
+    with pytest.raises(RuntimeError, match="not overlap them otherwise"):
+        rms_norm_int8(both.view(8, 32)[:4], w, residual=x.clone(), residual_out=both.view(8, 32)[1:5])
+    with pytest.raises(RuntimeError, match="overlaps the weight"):
+        rms_norm_int8(x[:1].clone(), both[3, :32], residual=x[:1].clone(), residual_out=both[3:, :32])
+    with pytest.raises(RuntimeError, match="contiguous rows of one pitch"):
+        rms_norm_int8(x, w, residual=x.clone(), residual_out=normal(32, 4, dtype=torch.float16).t())
+    with pytest.raises(RuntimeError, match="one row of the input's length and type"):
+        rms_norm_int8(x, w[:31])
+    with pytest.raises(RuntimeError, match="one row of the input's length and type"):
+        rms_norm_int8(x, w.bfloat16())
+    with pytest.raises(RuntimeError, match="the residual must have the input's shape"):
+        rms_norm_int8(x, w, residual=x[:3])
+    with pytest.raises(RuntimeError, match="must be on the device"):
+        rms_norm_int8(x, w.cpu())
+
+
+def silu_error(gate):
+    """Relative: exp of -g 2 + 1.173 |g| ulp, the quotient 2 ulp, the sum and two products half an ulp each; an ulp is 2^-23."""
+    return (1.173 * gate.double().abs() + 2 + 2 + 1.5) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_silu_mul(dtype, cols):
+    from gemmlib_b200.int8_linear import silu_mul_int8
+
+    both = normal(5, 2 * cols, dtype=dtype, seed=cols, scale=3.0)
+    both[2, :cols] = 0
+    gate, up = both[:, :cols], both[:, cols:]
+    g = gate.double()
+    check_rows(silu_mul_int8(gate, up), g / (1 + torch.exp(-g)) * up.double(), t_error=silu_error(gate))
+
+
+def test_silu_mul_far_from_zero():
+    from gemmlib_b200.int8_linear import silu_mul_int8
+
+    gate = torch.tensor([[-60000.0, -100.0, -89.0, -60.0, 60.0, 100.0, 60000.0, 1.0]], dtype=torch.float16, device="cuda")
+    up = torch.ones_like(gate)
+    r = silu_mul_int8(gate, up)
+    assert r.values.tolist() == [[0, 0, 0, 0, 0, 0, 127, 0]] and abs(float(r.scales[0]) * 127 - 60000) < 0.01
+    r = silu_mul_int8(gate[:, :4].contiguous(), up[:, :4])  # -60 exp(-60) is the largest
+    g = gate[:, :4].double()
+    check_rows(r, g * torch.sigmoid(g), t_error=silu_error(torch.full_like(g, 61.0)))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("cols", [1, 15, 16, 17, 100, 4096, 5001, 28672])
+def test_dequantize(dtype, cols):
+    from gemmlib_b200.int8_linear import quantize_int8
+
+    r = quantize_int8(normal(7, cols, dtype=torch.bfloat16, seed=cols))
+    out = r.dequantize(dtype)
+    assert out.dtype == dtype and out.is_contiguous()
+    assert torch.equal(out, (r.values.float() * r.scales[:, None]).to(dtype))
+
+
+LAYOUTS = {
+    "slice": lambda x: torch.cat([x, x], -1)[..., : x.shape[-1]],
+    "odd offset": lambda x: torch.cat([x[..., :1], x], -1)[..., 1:],
+    "transposed": lambda x: x.transpose(-1, -2).contiguous().transpose(-1, -2),
+    "every second row": lambda x: x.repeat_interleave(2, -2)[..., ::2, :],
+    "expanded": lambda x: x[..., :1, :].expand_as(x),
+    "three dimensions": lambda x: x.reshape(2, 3, -1),
+    "permuted": lambda x: x.reshape(2, 3, -1).transpose(0, 1),
+    "one row": lambda x: x[0],
+    "no rows": lambda x: x[:0],
+}
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("cols", [40, 4096])
+def test_layouts_give_the_same_rows(layout, cols):
+    """A view gives what a contiguous copy of it gives, bit for bit, and no input is written."""
+    from gemmlib_b200.int8_linear import quantize_int8, rms_norm_int8, silu_mul_int8
+
+    x, y = (LAYOUTS[layout](normal(6, cols, dtype=torch.float16, seed=s)) for s in (0, 1))
+    w = normal(cols, dtype=torch.float16, seed=2)
+    before = x.clone()
+    calls = [quantize_int8, lambda v: rms_norm_int8(v, w), lambda v: silu_mul_int8(v, y), lambda v: silu_mul_int8(y, v),
+             lambda v: rms_norm_int8(v, w, residual=y)[0], lambda v: rms_norm_int8(y, w, residual=v)[0]]
+    for call in calls:
+        got, want = call(x), call(x.contiguous())
+        assert torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+        assert got.values.shape == x.shape and got.scales.shape == x.shape[:-1]
+        assert torch.equal(got.dequantize(), want.dequantize())
+    assert torch.equal(x, before)
+
+
+def test_nothing_is_written_outside_the_rows():
+    """Through the C entry points, into buffers with guards between the rows and behind them."""
+    from gemmlib_b200 import capi
+
+    for cols, pitch in ((40, 48), (41, 43), (4096, 4112), (5001, 5003)):
+        x, w = normal(4, cols, dtype=torch.float16), normal(cols, dtype=torch.float16, seed=1)
+        values = torch.full((4 * pitch + 64,), 99, dtype=torch.int8, device="cuda")
+        sums = torch.full((4 * pitch + 64,), 7.0, dtype=torch.float16, device="cuda")
+        scales = torch.full((8,), 5.0, device="cuda")
+        capi.int8_rows_rms_norm(capi.INT8_FP16, 4, cols, (x, cols), (x, cols), w, 1e-5, (sums, pitch), (values, pitch), scales)
+        torch.cuda.synchronize()
+        inside = torch.zeros(4 * pitch + 64, dtype=torch.bool, device="cuda")
+        inside[: 4 * pitch].view(4, pitch)[:, :cols] = True
+        assert (values[~inside] == 99).all() and (sums[~inside] == 7).all() and (scales[4:] == 5).all()
+        assert torch.equal(sums[: 4 * pitch].view(4, pitch)[:, :cols], x + x)
+        out = torch.full((4 * pitch + 64,), 7.0, dtype=torch.float16, device="cuda")
+        capi.int8_rows_dequant(capi.INT8_FP16, 4, cols, (values, pitch), scales, (out, pitch))
+        torch.cuda.synchronize()
+        assert (out[~inside] == 7).all()
+
+
+def test_repeats_are_equal_and_streams_and_graphs_work():
+    from gemmlib_b200.int8_linear import quantize_int8, rms_norm_int8
+
+    x, w = normal(64, 4096, dtype=torch.bfloat16), normal(4096, dtype=torch.bfloat16, seed=1)
+    want, h = rms_norm_int8(x, w, residual=x)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            got, _ = rms_norm_int8(x, w, residual=x)
+    stream.synchronize()
+    assert torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, _ = rms_norm_int8(x, w, residual=x)
+        again = quantize_int8(got.dequantize(torch.bfloat16))
+    x.copy_(normal(64, 4096, dtype=torch.bfloat16, seed=3))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    want, _ = rms_norm_int8(x, w, residual=x)
+    assert torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+    assert torch.equal(again.values, quantize_int8(want.dequantize(torch.bfloat16)).values)

@@ -5,9 +5,10 @@
 // so neither the tiles nor the split of K show in the result; the two scales and the bias are applied in fp32 and the
 // result is rounded once.
 //
-// gemm_rows_kernel: 128 weight rows (TMEM lanes) x up to 256 activation rows per tile, so that few rows waste no weights'
+// Two kernels.  gemm_rows_kernel: 128 weight rows (TMEM lanes) x up to 256 activation rows per tile, so that few rows waste no weights'
 // bandwidth; the K range of a tile is split over a cluster of CTAs, which exchange their int32 parts through distributed shared
-// memory.
+// memory.  gemm_pair_kernel: 256 activation rows (TMEM lanes of two CTAs) x up to 256 weight rows per tile, persistent, for problems
+// that fill the GPU with such tiles.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -267,6 +268,308 @@ __global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_consta
   }
 }
 
+// ---- pairs of CTAs ----
+// A pair (cta_group::2) computes 256 x BN outputs: each CTA stages its 128 activation rows and its half of the BN weight rows,
+// so that an SM reads 64 bytes of shared memory a cycle for the MMAs instead of 96 with a tile of its own, and every operand row
+// crosses from L2 once a pair.  The MMAs of a tile run while the epilogue warps empty the other of two accumulators.
+//   FULL[s]       of the even CTA (the leader): the bytes of both CTAs' copies; its MMA thread waits
+//   EMPTY[s]      of each CTA, by a commit to both: the stage may be written again
+//   ACC_FULL[b]   of each CTA, by a commit to both        ACC_EMPTY[b]   of the leader: the epilogue warps of both CTAs
+constexpr int kPairM = 256, kPairMaxN = 256;
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairHalfBytes = 128u * kStepK;            // one operand's rows of a stage, at most
+constexpr uint32_t kPairStageBytes = 2 * kPairHalfBytes;
+constexpr uint32_t kPairChunkBytes = 32u * 64u;               // 32 rows x 32 outputs
+constexpr uint32_t kPairOutBytes = kEpiWarps * 2 * kPairChunkBytes;
+constexpr uint32_t kPairScaleBytes = 2u * 2u * kPairMaxN * 4u;  // scales and biases of two tiles' columns
+constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + kPairOutBytes + kPairScaleBytes + 512 + 1024;
+static_assert(kPairSmem <= 227 * 1024);
+
+struct PairParams {
+  int M, N;
+  int BN;  // weight rows of a tile, a multiple of 32, <= 256
+  int m_tiles, n_tiles, k_steps;
+  int group_m;  // m tiles that run side by side before the next column tiles
+  int early;
+  int bulk;     // outputs by TMA: rows of the output begin on 16 bytes
+  void* out;
+  int64_t ldo;
+  const float* x_scales;
+  const float* w_scales;
+  const void* bias;
+};
+
+__device__ __forceinline__ void umma_i8_x4_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\t"
+      "add.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+      "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+      "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a0, b0, %4, p;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a1, b1, %4, q;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a2, b2, %4, q;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %4, q;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives, once every earlier MMA of the pair has retired, on the barrier at this offset in both CTAs.
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Copy into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar_cluster)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// `wait` on a barrier that the other CTA arrives on.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  const long long t0 = clock64();
+  while (!try_wait_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *abort_flag = 1;
+      atomicCAS(&g_int8_error, 0, who);
+      return false;
+    }
+  }
+  return true;
+}
+
+// The tiles of a pair: every num_pairs-th.  Tiles run in bands of group_m m tiles, m fastest, so that those under way at a time
+// share the rows of both operands in L2.
+struct PairWalk {
+  int tile, step, count, m_tiles, n_tiles, group_m;
+  __device__ __forceinline__ PairWalk(const PairParams& p)
+      : tile((int)(blockIdx.x >> 1)), step((int)(gridDim.x >> 1)), count(p.m_tiles * p.n_tiles), m_tiles(p.m_tiles),
+        n_tiles(p.n_tiles), group_m(p.group_m) {}
+  __device__ __forceinline__ bool next(int& m_tile, int& n_tile) {
+    if (tile >= count) return false;
+    const int band = tile / (group_m * n_tiles), first = band * group_m, high = min(group_m, m_tiles - first);
+    const int in_band = tile - band * group_m * n_tiles;
+    m_tile = first + in_band % high;
+    n_tile = in_band / high;
+    tile += step;
+    return true;
+  }
+};
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                 const __grid_constant__ CUtensorMap tm_out, const PairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  constexpr uint32_t kOut = kPairStages * kPairStageBytes, kScales = kOut + kPairOutBytes, kBars = kScales + kPairScaleBytes;
+  auto full = [&](int s) { return base + kBars + 16u * (uint32_t)s; };
+  auto empty = [&](int s) { return base + kBars + 16u * (uint32_t)s + 8u; };
+  auto acc_full = [&](int b) { return base + kBars + 16u * (uint32_t)(kPairStages + b); };
+  auto acc_empty = [&](int b) { return base + kBars + 16u * (uint32_t)(kPairStages + b) + 8u; };
+  constexpr uint32_t kWords = kBars + 16u * (kPairStages + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + kWords);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kWords + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_ctarank();
+  const int half_n = p.BN >> 1;
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full(i), 1);
+      mbar_init(acc_empty(i), 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::cluster_sync_all();  // the other CTA's barriers exist before anything signals them
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t tx = 2u * (kPairHalfBytes + (uint32_t)half_n * kStepK);
+      PairWalk walk(p);
+      int m_tile, n_tile;
+      bool first = true;
+      uint32_t it = 0;
+      while (walk.next(m_tile, n_tile)) {
+        const int x_row = m_tile * kPairM + (int)rank * 128, w_row = n_tile * p.BN + (int)rank * half_n;
+        int ahead = 0;
+        if (first) {
+          ahead = min(p.k_steps, kPairStages);
+          for (int ks = 0; ks < ahead; ++ks) {
+            if (p.early) {
+              if (rank == 0) mbar_arrive_expect_tx(full(ks), tx);
+              tma_load_pair(base + ks * kPairStageBytes + kPairHalfBytes, &tm_w, ks * kStepK, w_row, tc::map_to_cta(full(ks), 0));
+            } else {  // on its way into L2, where a write that is still to come would find it
+              prefetch_l2_2d(&tm_w, ks * kStepK, w_row);
+            }
+          }
+          if (!p.early) ahead = 0;
+          griddep_wait();
+          first = false;
+        }
+        for (int ks = 0; ks < p.k_steps; ++ks, ++it) {
+          const int s = it % kPairStages;
+          if (it >= (uint32_t)kPairStages && !wait(empty(s), ((it / kPairStages) - 1) & 1, abort_flag, 0x1100 | s)) goto producer_done;
+          const uint32_t bar = tc::map_to_cta(full(s), 0), dst = base + s * kPairStageBytes;
+          if (ks >= ahead) {
+            if (rank == 0) mbar_arrive_expect_tx(full(s), tx);
+            tma_load_pair(dst + kPairHalfBytes, &tm_w, ks * kStepK, w_row, bar);
+          }
+          tma_load_pair(dst, &tm_x, ks * kStepK, x_row, bar);
+        }
+      }
+    producer_done:;
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = make_idesc_i8(kPairM, p.BN);
+      const uint64_t desc = tc::make_sw128_kmajor_desc(0);
+      const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc | ((base >> 4) & 0x3FFFu);
+      PairWalk walk(p);
+      int m_tile, n_tile;
+      uint32_t it = 0;
+      for (uint32_t t = 0; walk.next(m_tile, n_tile); ++t) {
+        const uint32_t b = t & 1u;
+        if (t >= 2 && !wait_cluster(acc_empty(b), ((t >> 1) - 1) & 1u, abort_flag, 0x1200 | b)) goto mma_done;
+        tc::tc_fence_after();
+        for (int ks = 0; ks < p.k_steps; ++ks, ++it) {
+          const int s = it % kPairStages;
+          if (!wait(full(s), (it / kPairStages) & 1, abort_flag, 0x1210 | s)) goto mma_done;
+          tc::tc_fence_after();
+          const uint32_t lo = desc_lo + s * (kPairStageBytes >> 4);
+          umma_i8_x4_pair(tmem + b * kPairMaxN, lo, lo + (kPairHalfBytes >> 4), desc_hi, idesc, ks > 0);
+          commit_both(empty(s));
+        }
+        commit_both(acc_full(b));
+      }
+    mma_done:;
+    }
+  } else {
+    // ---- epilogue: a warp empties the 32 rows of its quarter of the lanes, 32 outputs at a time, through two staging
+    // blocks of its own (64-byte rows, their 16-byte pieces swizzled by the row as TMA's 64-byte swizzle has them)
+    const int quarter = warp & 3, et = (int)threadIdx.x - 64;
+    const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint8_t* stage = base_ptr + kOut + (warp - 2) * 2 * kPairChunkBytes;
+    T* out = reinterpret_cast<T*>(p.out);
+    griddep_wait();
+    PairWalk walk(p);
+    int m_tile, n_tile;
+    uint32_t chunk = 0;
+    for (uint32_t t = 0; walk.next(m_tile, n_tile); ++t) {
+      const uint32_t b = t & 1u;
+      const int n0 = n_tile * p.BN, row0 = m_tile * kPairM + (int)rank * 128 + quarter * 32;
+      // the columns' scales and biases, for all four warps; the buffer of the tile before last is free, since every warp has
+      // passed the barrier of the last one
+      float* scales = reinterpret_cast<float*>(base_ptr + kScales) + b * 2 * kPairMaxN;
+      float* biases = scales + kPairMaxN;
+      for (int i = et; i < p.BN; i += 32 * kEpiWarps) {
+        const bool in = n0 + i < p.N;
+        scales[i] = in ? p.w_scales[n0 + i] : 0.0f;
+        biases[i] = in && p.bias ? to_float(reinterpret_cast<const T*>(p.bias)[n0 + i]) : 0.0f;
+      }
+      const float x_scale = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.0f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+      const bool ok = wait_cluster(acc_full(b), (t >> 1) & 1u, abort_flag, 0x1300 | b);
+      if (__any_sync(0xffffffffu, !ok)) continue;  // on to the barriers of the tiles that are left, so that no warp waits for another
+      tc::tc_fence_after();
+      for (int c0 = 0; c0 < p.BN; c0 += 32, ++chunk) {
+        uint32_t r[32];
+        tc::tmem_ld_32x32b_x32(tmem_row + b * kPairMaxN + (uint32_t)c0, r);
+        tc::tmem_ld_wait();
+        if (c0 + 32 >= p.BN) {  // the accumulator is in registers: the MMAs of the tile after next may have it
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_cluster(tc::map_to_cta(acc_empty(b), 0));
+        }
+        uint8_t* dst = stage + (chunk & 1u) * kPairChunkBytes;
+        // the store of the chunk before last has read this block
+        if (p.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t v[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 s4 = *reinterpret_cast<const float4*>(scales + c0 + q * 8 + h * 4);
+            const float4 b4 = *reinterpret_cast<const float4*>(biases + c0 + q * 8 + h * 4);
+            const uint32_t* a = r + q * 8 + h * 4;
+            v[h * 2] = pack2<T>(fmaf((float)(int)a[0] * x_scale, s4.x, b4.x), fmaf((float)(int)a[1] * x_scale, s4.y, b4.y));
+            v[h * 2 + 1] = pack2<T>(fmaf((float)(int)a[2] * x_scale, s4.z, b4.z), fmaf((float)(int)a[3] * x_scale, s4.w, b4.w));
+          }
+          *reinterpret_cast<uint4*>(dst + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        if (p.bulk) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < p.M && n0 + c0 < p.N)
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&tm_out), "r"(n0 + c0),
+                           "r"(row0), "r"(smem_u32(dst))
+                           : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          const int n = n0 + c0 + lane;
+          for (int row = 0; row < min(32, p.M - row0); ++row) {
+            const T v = *reinterpret_cast<const T*>(dst + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
+            if (n < p.N) out[(int64_t)(row0 + row) * p.ldo + n] = v;
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+
+  // neither CTA frees tensor memory or leaves while the other may still signal it
+  tc::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) __nanosleep(50000);  // let copies in flight land
+  __syncthreads();
+  tc::cluster_sync_all();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // K-major rows of bytes `ld` apart.
 bool encode_rows(CUtensorMap* map, const int8_t* ptr, int64_t ld, int K, int rows, int box_rows) {
   TensorMapEncodeFn fn = tensor_map_encode_fn();
@@ -344,10 +647,77 @@ std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t str
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
 }
 
+// ---- which kernel ----
+struct PairTiles {
+  int BN, m_tiles, n_tiles, rounds;
+};
+// The width of tiles that leaves the least work to the slowest of `pairs` pairs.
+PairTiles plan_pairs(int M, int N, int pairs) {
+  PairTiles best{};
+  long best_cost = 0;
+  for (int BN = 256; BN >= 128; BN -= 32) {
+    PairTiles t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0};
+    t.rounds = (int)(((long)t.m_tiles * t.n_tiles + pairs - 1) / pairs);
+    const long cost = (long)t.rounds * BN;
+    if (best.BN == 0 || cost < best_cost) best = t, best_cost = cost;
+  }
+  return best;
+}
+
+template <class T>
+std::string launch_pairs(const GemmArgs& g, const PairTiles& t, int pairs, unsigned flags, cudaStream_t stream) {
+  PairParams p{};
+  p.M = g.M; p.N = g.N;
+  p.BN = t.BN; p.m_tiles = t.m_tiles; p.n_tiles = t.n_tiles;
+  p.k_steps = (g.K + kStepK - 1) / kStepK;
+  p.group_m = 8;
+  p.early = (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0;
+  p.bulk = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo % 8 == 0;
+  p.out = g.out; p.ldo = g.ldo;
+  p.x_scales = g.x_scales; p.w_scales = g.w_scales; p.bias = g.bias;
+  CUtensorMap tm_x, tm_w, tm_out;
+  bool ok = encode_rows(&tm_x, g.x, g.ldx, g.K, g.M, 128) && encode_rows(&tm_w, g.w, g.ldw, g.K, g.N, t.BN / 2);
+  if (p.bulk) {
+    TensorMapEncodeFn fn = tensor_map_encode_fn();
+    cuuint64_t dims[2] = {(cuuint64_t)g.N, (cuuint64_t)g.M};
+    cuuint64_t strides[1] = {(cuuint64_t)g.ldo * 2};
+    cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
+    ok = ok && fn(&tm_out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, g.out, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  } else {
+    tm_out = tm_x;
+  }
+  if (!ok) return "cuTensorMapEncodeTiled failed";
+  static std::atomic<int> granted[64];
+  cudaError_t e = ensure_dynamic_smem(gemm_pair_kernel<T>, kPairSmem, granted);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2u * (unsigned)std::min(pairs, t.m_tiles * t.n_tiles));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, gemm_pair_kernel<T>, tm_x, tm_w, tm_out, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
+}
+
+template <class T>
+std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
+  const int pairs = std::max(1, sm_count() / 2);
+  const PairTiles t = plan_pairs(g.M, g.N, pairs);
+  if (g.M > 256 && t.m_tiles * t.n_tiles >= pairs / 2) return launch_pairs<T>(g, t, pairs, flags, stream);
+  return launch_rows_gemm<T>(g, flags, stream);
+}
+
 }  // namespace
 
 std::string launch_gemm(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream) {
-  return dtype == kFp16 ? launch_rows_gemm<__half>(g, flags, stream) : launch_rows_gemm<__nv_bfloat16>(g, flags, stream);
+  return dtype == kFp16 ? launch_typed<__half>(g, flags, stream) : launch_typed<__nv_bfloat16>(g, flags, stream);
 }
 
 int read_gemm_error() {

@@ -120,8 +120,12 @@ __device__ __forceinline__ void row_values(const RowsParams& p, int64_t row, int
   }
 }
 
-// round(t * inverse), half to even, of |t * inverse| < 2^22: the sum's low mantissa bits are the integer
-__device__ __forceinline__ uint32_t rounded(float t, float inverse) { return __float_as_uint(fmaf(t, inverse, 12582912.0f)); }
+// round(t * inverse), half to even, of |t * inverse| < 2^22: the sum's low mantissa bits are the integer.  The product is rounded
+// by itself: 16-bit inputs often stand exactly half-way between two integers (t = max / 2 is 63.5 steps), and a product of the
+// rounded inverse falls back on the tie where a fused one would always leave it to the side of the inverse's own error.
+__device__ __forceinline__ uint32_t rounded(float t, float inverse) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(t, inverse), 12582912.0f));
+}
 
 __device__ __forceinline__ void store_q(int8_t* row, bool vec, int chunk, int cols, const float (&t)[8], float inverse) {
   uint32_t b[8];

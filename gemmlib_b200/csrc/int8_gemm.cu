@@ -70,10 +70,6 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
 __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void st_shared_cluster_u32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
 struct Params {
   int M, N;
   int BM;          // activation rows of a tile, a multiple of 16, <= 256
@@ -94,12 +90,12 @@ struct Params {
 };
 
 constexpr int kMaxStages = 16;
-constexpr int kEpiWarps = 4, kThreads = 32 * (2 + kEpiWarps);
-constexpr uint32_t kBarBytes = 512;  // full[], empty[], accumulator, abort flag, TMEM address
+constexpr int kRowsEpiWarps = 8, kRowsThreads = 32 * (2 + kRowsEpiWarps);
+constexpr uint32_t kBarBytes = 512 + 1024;  // full[], empty[], accumulator, abort flag, TMEM address; the activations' scales
 
 // Grid: tiles * split CTAs, those of a tile a cluster.  The m tiles of a column tile follow one another.
 template <class T>
-__global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_constant__ CUtensorMap tm_x,
+__global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_constant__ CUtensorMap tm_x,
                                                              const __grid_constant__ CUtensorMap tm_w, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -111,10 +107,13 @@ __global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_consta
   const uint32_t acc_full = bars + 16u * kMaxStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 16 * kMaxStages + 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + 16 * kMaxStages + 12);
+  float* x_scales = reinterpret_cast<float*>(bars_ptr + 512);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(full(i), 1);
       mbar_init(empty(i), 1);
@@ -180,35 +179,48 @@ __global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_consta
       }
       if (ok) tc::umma_commit(acc_full);
     }
-  } else {
+  }
+
+  // ---- epilogue: a warp has the 32 weight rows n of its quarter of the TMEM lanes (by warp number mod 4), two warps share a
+  // quarter on groups of 8 activation rows m (TMEM columns) in turn
+  const int rows = min(p.BM, p.M - m0);
+  const int quarter = warp & 3, turn = (warp - 2) >> 2, n_l = quarter * 32 + lane, n = n0 + n_l;
+  const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
+  float w_scale = 0.0f, bias = 0.0f;
+  if (warp >= 2) {
     griddep_wait();  // scales of the activations and the output belong to stream order
+    // fetched while the MMAs run: behind them, their latency would be the tail of a short call
+    for (int i = (int)threadIdx.x - 64; i < rows; i += 32 * kRowsEpiWarps) x_scales[i] = p.x_scales[m0 + i];
+    if (n < p.N) {
+      w_scale = p.w_scales[n];
+      if (p.bias) bias = to_float(reinterpret_cast<const T*>(p.bias)[n]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsEpiWarps) : "memory");
     wait(acc_full, 0, abort_flag, 0x300);
   }
   __syncwarp();
   auto dead = [&] { return __shfl_sync(0xffffffffu, *abort_flag, 0) != 0; };  // one answer a warp
 
   // ---- the parts of a split tile: CTA o of the cluster collects the sums of activation rows [o * slice, (o + 1) * slice)
-  // in its stages, [part][row][128], which every CTA of the cluster is done with after the first barrier.
-  const int rows = min(p.BM, p.M - m0);
-  const int quarter = warp & 3, n_l = quarter * 32 + lane;  // TMEM lanes of an epilogue warp: a quarter, by warp number mod 4
-  const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
+  // in its stages, which every CTA of the cluster is done with after the first barrier: [part][4 rows][128 n][row], so that a
+  // lane moves 16 bytes and a warp 512 in a run.
+  const uint32_t part_words = (uint32_t)p.slice * kTileN;
   if (p.split > 1) {
     __syncthreads();
     tc::cluster_sync_all();
     if (warp >= 2 && !dead()) {
       tc::tc_fence_after();
-      for (int o = 0; o < p.split; ++o) {
+      int o = 0;  // owner of row m
+      for (int m = turn * 8; m < rows; m += 16) {
+        while (m >= (o + 1) * p.slice) ++o;
         if (o == part) continue;
-        const int end = min(rows, (o + 1) * p.slice);
-        const uint32_t dst = tc::map_to_cta(base + (uint32_t)((part - (part > o)) * p.slice * kTileN + n_l) * 4u, (uint32_t)o);
-        for (int m = o * p.slice; m < end; m += 8) {
-          uint32_t r[8];
-          tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (m + j < end) st_shared_cluster_u32(dst + (uint32_t)((m + j - o * p.slice) * kTileN) * 4u, r[j]);
-        }
+        uint32_t r[8];
+        tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
+        tc::tmem_ld_wait();
+        const uint32_t at = (uint32_t)(part - (part > o)) * part_words + (uint32_t)((m - o * p.slice) * kTileN + n_l * 4);
+        const uint32_t dst = tc::map_to_cta(base + at * 4u, (uint32_t)o);
+        tc::st_shared_cluster_v4(dst, r[0], r[1], r[2], r[3]);
+        if (m + 4 < rows) tc::st_shared_cluster_v4(dst + 4u * kTileN * 4u, r[4], r[5], r[6], r[7]);
       }
     }
     __syncwarp();
@@ -217,28 +229,26 @@ __global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_consta
 
   if (warp >= 2 && !dead()) {
     tc::tc_fence_after();
-    const int n = n0 + n_l;
-    const float w_scale = n < p.N ? p.w_scales[n] : 0.0f;
-    const float bias = p.bias && n < p.N ? to_float(reinterpret_cast<const T*>(p.bias)[n]) : 0.0f;
     const int first = part * p.slice, end = min(rows, first + p.slice);
-    const uint32_t* parts = reinterpret_cast<const uint32_t*>(base_ptr) + n_l;
+    const uint32_t* parts = reinterpret_cast<const uint32_t*>(base_ptr) + n_l * 4;
     T* out = reinterpret_cast<T*>(p.out);
     const int odd = lane & 1;
-    for (int m = first; m < end; m += 8) {
+    for (int m = first + turn * 8; m < end; m += 16) {
       uint32_t r[8];
       tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
       tc::tmem_ld_wait();
       for (int q = 0; q < p.split - 1; ++q) {
+        const uint32_t* at = parts + q * part_words + (m - first) * kTileN;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (m + j < end) r[j] += parts[(size_t)(q * p.slice + m + j - first) * kTileN];
+        for (int h = 0; h < 2; ++h) {
+          if (m + 4 * h >= end) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(at + 4 * h * kTileN);
+          r[4 * h] += v.x, r[4 * h + 1] += v.y, r[4 * h + 2] += v.z, r[4 * h + 3] += v.w;
+        }
       }
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x_scale = m + j < end ? p.x_scales[m0 + m + j] : 0.0f;
-        v[j] = fmaf((float)(int)r[j] * x_scale, w_scale, bias);
-      }
+      for (int j = 0; j < 8; ++j) v[j] = fmaf((float)(int)r[j] * x_scales[m + j], w_scale, bias);
       if (p.pairs) {
         // lanes of an even and an odd n trade: the even one stores the even row's two values, the odd one the odd row's
 #pragma unroll
@@ -275,6 +285,7 @@ __global__ void __launch_bounds__(kThreads) gemm_rows_kernel(const __grid_consta
 //   FULL[s]       of the even CTA (the leader): the bytes of both CTAs' copies; its MMA thread waits
 //   EMPTY[s]      of each CTA, by a commit to both: the stage may be written again
 //   ACC_FULL[b]   of each CTA, by a commit to both        ACC_EMPTY[b]   of the leader: the epilogue warps of both CTAs
+constexpr int kEpiWarps = 4, kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairM = 256, kPairMaxN = 256;
 constexpr int kPairStages = 6;
 constexpr uint32_t kPairHalfBytes = 128u * kStepK;            // one operand's rows of a stage, at most
@@ -594,15 +605,15 @@ RowsPlan plan_rows(int M, int N, int K, int sms) {
   r.n_tiles = (N + kTileN - 1) / kTileN;
   r.stage_bytes = kWeightBytes + (uint32_t)r.BM * kStepK;
   const int k_steps = (K + kStepK - 1) / kStepK;
-  // two CTAs of an SM where their stages are small, else one
-  const uint32_t ring = r.BM <= 128 ? 108u * 1024 : 216u * 1024;
-  r.stages = std::min<int>(kMaxStages, (int)(ring / r.stage_bytes));
   const int slots = sms * (r.BM <= 128 ? 2 : 1), tiles = r.m_tiles * r.n_tiles;
   r.split = std::max(1, std::min({8, slots / tiles, k_steps / 2}));
   r.k_per_cta = (k_steps + r.split - 1) / r.split;
   r.split = (k_steps + r.k_per_cta - 1) / r.k_per_cta;
   const int rows = std::min(M, r.BM);
   r.slice = r.split > 1 ? ((rows + r.split - 1) / r.split + 7) / 8 * 8 : r.BM;
+  // one CTA on an SM has all its shared memory for stages
+  const uint32_t ring = r.BM <= 128 && tiles * r.split > sms ? 108u * 1024 : 216u * 1024;
+  r.stages = std::min<int>(kMaxStages, (int)(ring / r.stage_bytes));
   r.smem = (uint32_t)r.stages * r.stage_bytes + kBarBytes + 1024;
   return r;
 }
@@ -631,7 +642,7 @@ std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t str
   if (e != cudaSuccess) return cudaGetErrorString(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(r.m_tiles * r.n_tiles * r.split));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kRowsThreads);
   cfg.dynamicSmemBytes = r.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

@@ -45,6 +45,9 @@ struct GemmArgs {
   void* out;
   int64_t ldo;  // elements
 };
+// The kernel of a few activation rows, and the problems it is for.
+bool gemv_takes(int M, int N, int K);
+std::string launch_gemv(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream);
 std::string launch_gemm(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream);
 int read_gemm_error();
 int clear_gemm_error(cudaStream_t stream);

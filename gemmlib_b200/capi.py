@@ -53,6 +53,7 @@ INT8_SYMBOLS = (
     "int8_rows_silu_mul_sm100",
     "int8_rows_dequant_sm100",
     "int8_gemm_sm100",
+    "int8_gemm_plan_sm100",
 )
 INT8_FP16, INT8_BF16 = 0, 1
 
@@ -147,6 +148,7 @@ def _load() -> ctypes.CDLL:
     lib.int8_rows_silu_mul_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *matrix, *vector, vp]
     lib.int8_rows_dequant_sm100.argtypes = [i, i, i, vp, *matrix, *vector, *matrix, vp]
     lib.int8_gemm_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, *matrix, *vector, *vector, *matrix, ctypes.c_uint, vp]
+    lib.int8_gemm_plan_sm100.argtypes = [i, i, i, ctypes.POINTER(i)]
     for name in INT8_SYMBOLS:
         getattr(lib, name).restype = i
     return lib
@@ -440,3 +442,12 @@ def int8_rows_dequant(dtype, rows, cols, values, scales, out, stream=0):
 def int8_gemm(dtype, m, n, k, x, x_scales, w, w_scales, bias, out, flags=0, stream=0):
     _int8_call(lib.int8_gemm_sm100, dtype, m, n, k, stream, *_matrix(x), *_ptr_size(x_scales), *_matrix(w), *_ptr_size(w_scales),
                *_ptr_size(bias), *_matrix(out), flags)
+
+
+def int8_gemm_plan(m: int, n: int, k: int) -> dict:
+    """The work plan of ``int8_gemm`` for a contiguous output (host only; see int8_gemm_plan_sm100)."""
+    out = (ctypes.c_int * 8)()
+    if lib.int8_gemm_plan_sm100(m, n, k, out) != 0:
+        raise BlkQ4Error(f"no plan for {m}x{n}x{k}")
+    names = ("kernel", "tile_m", "tile_n", "tiles", "split", "steps", "stages", "smem")
+    return {**dict(zip(names, out)), "kernel": ("stream", "one-cta", "pair")[out[0]]}

@@ -38,6 +38,30 @@ constexpr long long kWaitCycles = 4000000000ll;  // ~2 s: far beyond any legitim
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
   return mbar_wait_bounded(bar, parity, abort_flag, &g_int8_error, who, kWaitCycles);
 }
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// `wait` on a barrier that other CTAs of the cluster arrive on.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  const long long t0 = clock64();
+  while (!try_wait_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *abort_flag = 1;
+      atomicCAS(&g_int8_error, 0, who);
+      return false;
+    }
+  }
+  return true;
+}
 // Instruction descriptor of kind::i8: int32 accumulator (bits 4-5 = 2), signed A and B (bits 7-9 and 10-12 = 1), both K-major,
 // N >> 3 in bits 17-22, M >> 4 in bits 24-28.
 __host__ __device__ inline uint32_t make_idesc_i8(int umma_m, int umma_n) {
@@ -67,6 +91,12 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                : "r"(taddr)
                : "memory");
 }
+// 16 bytes to another CTA of the cluster, which complete on a barrier there.
+__device__ __forceinline__ void st_async_v4(uint32_t dst, uint32_t bar, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(dst), "r"(bar),
+               "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
 __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
@@ -79,6 +109,7 @@ struct Params {
   int k_per_cta;   // steps of each, the last one what is left
   int slice;       // activation rows whose sums one CTA of the cluster collects, a multiple of 8
   int stages;
+  uint32_t exchange_bytes;  // behind the stages: what a CTA collects
   int early;       // weights may be copied before the kernels ahead in the stream have completed
   uint32_t stage_bytes, tmem_cols;
   int pairs;       // two neighbouring outputs of a row may be stored at once
@@ -91,7 +122,7 @@ struct Params {
 
 constexpr int kMaxStages = 16;
 constexpr int kRowsEpiWarps = 8, kXWarp = 2 + kRowsEpiWarps, kRowsThreads = 32 * (kXWarp + 1);
-constexpr uint32_t kBarBytes = 512 + 1024;  // full[], empty[], accumulator, abort flag, TMEM address; the activations' scales
+constexpr uint32_t kBarBytes = 512 + 1024;  // full[], empty[], accumulator, exchange, abort flag, TMEM address; the activations' scales
 
 // Grid: tiles * split CTAs, those of a tile a cluster.  The m tiles of a column tile follow one another.
 template <class T>
@@ -100,14 +131,21 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bars = base + (uint32_t)p.stages * p.stage_bytes;
-  uint8_t* bars_ptr = base_ptr + (size_t)p.stages * p.stage_bytes;
+  const uint32_t exchange_at = (uint32_t)p.stages * p.stage_bytes, bars_at = exchange_at + p.exchange_bytes;
+  const uint32_t bars = base + bars_at;
+  uint8_t* bars_ptr = base_ptr + bars_at;
   auto full = [&](int s) { return bars + 16u * (uint32_t)s; };
   auto empty = [&](int s) { return bars + 16u * (uint32_t)s + 8u; };
-  const uint32_t acc_full = bars + 16u * kMaxStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 16 * kMaxStages + 8);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + 16 * kMaxStages + 12);
+  const uint32_t acc_full = bars + 16u * kMaxStages, exchanged = acc_full + 8u;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 16 * kMaxStages + 16);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + 16 * kMaxStages + 20);
   float* x_scales = reinterpret_cast<float*>(bars_ptr + 512);
+
+  const int tile = (int)blockIdx.x / p.split, part = (int)blockIdx.x % p.split;
+  const int m0 = tile % p.m_tiles * p.BM, n0 = tile / p.m_tiles * kTileN;
+  const int ks0 = part * p.k_per_cta, count = min(p.k_per_cta, p.k_steps - ks0);
+  const int rows = min(p.BM, p.M - m0);
+  const int first_row = min(rows, part * p.slice), end_row = min(rows, first_row + p.slice);  // whose sums end up here
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_launch_dependents();
@@ -119,8 +157,10 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
       mbar_init(empty(i), 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(exchanged, 1);
     *abort_flag = 0;
     mbar_init_fence();
+    if (p.split > 1) mbar_arrive_expect_tx(exchanged, (uint32_t)((p.split - 1) * ((end_row - first_row + 3) / 4) * kTileN * 16));
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(p.tmem_cols)
@@ -129,15 +169,12 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   }
   tc::tc_fence_before();
   __syncthreads();
+  if (p.split > 1) tc::cluster_sync_all();  // the others' barriers exist before anything is sent to them
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int tile = (int)blockIdx.x / p.split, part = (int)blockIdx.x % p.split;
-  const int m0 = tile % p.m_tiles * p.BM, n0 = tile / p.m_tiles * kTileN;
-  const int ks0 = part * p.k_per_cta, count = min(p.k_per_cta, p.k_steps - ks0);
-
   // Two producers, each with its operand: one thread took 0.26 us for the two copies of a step, which set the pace of all
-  // small problems (64 x 4096 x 4096: 8.2 us, now 6.9).
+  // small problems (M = 64, 4096 x 4096, tiles of 32 rows, K whole: 11.7 -> 7.7 us).
   if (warp == 0 || warp == kXWarp) {
     if (elect_one()) {
       const bool is_w = warp == 0;
@@ -196,7 +233,6 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
 
   // ---- epilogue: a warp has the 32 weight rows n of its quarter of the TMEM lanes (by warp number mod 4), two warps share a
   // quarter on groups of 8 activation rows m (TMEM columns) in turn
-  const int rows = min(p.BM, p.M - m0);
   const int quarter = warp & 3, turn = (warp - 2) >> 2, n_l = quarter * 32 + lane, n = n0 + n_l;
   const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
   float w_scale = 0.0f, bias = 0.0f;
@@ -215,36 +251,33 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   __syncwarp();
   auto dead = [&] { return __shfl_sync(0xffffffffu, *abort_flag, 0) != 0; };  // one answer a warp
 
-  // ---- the parts of a split tile: CTA o of the cluster collects the sums of activation rows [o * slice, (o + 1) * slice)
-  // in its stages, which every CTA of the cluster is done with after the first barrier: [part][4 rows][128 n][row], so that a
-  // lane moves 16 bytes and a warp 512 in a run.
+  // ---- the parts of a split tile: CTA o of the cluster collects the sums of activation rows [o * slice, (o + 1) * slice),
+  // [part][4 rows][128 n][row], so that a lane moves 16 bytes and a warp 512 in a run.  The bytes complete on the owner's
+  // barrier, so that it waits for them alone: two barriers of the whole cluster took 0.8 us each (M = 64, 4096 x 4096 in four
+  // parts FIGURE).  No CTA can leave before all that is sent to it has arrived.
   const uint32_t part_words = (uint32_t)p.slice * kTileN;
-  if (p.split > 1) {
-    __syncthreads();
-    tc::cluster_sync_all();
-    if (epilogue && !dead()) {
-      tc::tc_fence_after();
-      int o = 0;  // owner of row m
-      for (int m = turn * 8; m < rows; m += 16) {
-        while (m >= (o + 1) * p.slice) ++o;
-        if (o == part) continue;
-        uint32_t r[8];
-        tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
-        tc::tmem_ld_wait();
-        const uint32_t at = (uint32_t)(part - (part > o)) * part_words + (uint32_t)((m - o * p.slice) * kTileN + n_l * 4);
-        const uint32_t dst = tc::map_to_cta(base + at * 4u, (uint32_t)o);
-        tc::st_shared_cluster_v4(dst, r[0], r[1], r[2], r[3]);
-        if (m + 4 < rows) tc::st_shared_cluster_v4(dst + 4u * kTileN * 4u, r[4], r[5], r[6], r[7]);
-      }
+  if (p.split > 1 && epilogue && !dead()) {
+    tc::tc_fence_after();
+    int o = 0;  // owner of row m
+    for (int m = turn * 8; m < rows; m += 16) {
+      while (m >= (o + 1) * p.slice) ++o;
+      if (o == part) continue;
+      uint32_t r[8];
+      tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
+      tc::tmem_ld_wait();
+      const uint32_t at = (uint32_t)(part - (part > o)) * part_words + (uint32_t)((m - o * p.slice) * kTileN + n_l * 4);
+      const uint32_t dst = tc::map_to_cta(base + exchange_at + at * 4u, (uint32_t)o), bar = tc::map_to_cta(exchanged, (uint32_t)o);
+      st_async_v4(dst, bar, r[0], r[1], r[2], r[3]);
+      if (m + 4 < rows) st_async_v4(dst + 4u * kTileN * 4u, bar, r[4], r[5], r[6], r[7]);
     }
-    __syncwarp();
-    tc::cluster_sync_all();
+    if (end_row > first_row) wait_cluster(exchanged, 0, abort_flag, 0x310);
   }
+  __syncwarp();
 
   if (epilogue && !dead()) {
     tc::tc_fence_after();
-    const int first = part * p.slice, end = min(rows, first + p.slice);
-    const uint32_t* parts = reinterpret_cast<const uint32_t*>(base_ptr) + n_l * 4;
+    const int first = first_row, end = end_row;
+    const uint32_t* parts = reinterpret_cast<const uint32_t*>(base_ptr + exchange_at) + n_l * 4;
     T* out = reinterpret_cast<T*>(p.out);
     const int odd = lane & 1;
     for (int m = first + turn * 8; m < end; m += 16) {
@@ -284,8 +317,11 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
 
   tc::tc_fence_before();
   __syncthreads();
-  if (*abort_flag && threadIdx.x == 0) __nanosleep(50000);  // let copies in flight land
-  __syncthreads();
+  if (*abort_flag) {  // let copies in flight land, and the rest of the cluster give up or finish
+    if (threadIdx.x == 0) __nanosleep(50000);
+    __syncthreads();
+    if (p.split > 1) tc::cluster_sync_all();
+  }
   if (warp == 1) {
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
@@ -358,31 +394,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
 __device__ __forceinline__ void arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// `wait` on a barrier that the other CTA arrives on.
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
-  const long long t0 = clock64();
-  while (!try_wait_cluster(bar, parity)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      *abort_flag = 1;
-      atomicCAS(&g_int8_error, 0, who);
-      return false;
-    }
-  }
-  return true;
-}
-
 // The tiles of a pair: every num_pairs-th.  Tiles run in bands of group_m m tiles, m fastest, so that those under way at a time
 // share the rows of both operands in L2.
 struct PairWalk {
@@ -419,7 +430,6 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
-  const int half_n = p.BN >> 1;
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tm_w);
@@ -575,10 +585,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         } else {
           __syncwarp();
           const int n = n0 + c0 + lane;
-          for (int row = 0; row < min(32, p.M - row0); ++row) {
-            const T v = *reinterpret_cast<const T*>(dst + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
-            if (n < p.N) out[(int64_t)(row0 + row) * p.ldo + n] = v;
-          }
+          T v[32];
+#pragma unroll
+          for (int row = 0; row < 32; ++row)
+            v[row] = *reinterpret_cast<const T*>(dst + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
+          T* at = out + (int64_t)row0 * p.ldo + n;
+#pragma unroll
+          for (int row = 0; row < 32; ++row, at += p.ldo)
+            if (n < p.N && row0 + row < p.M) *at = v[row];
           __syncwarp();
         }
       }
@@ -599,6 +613,124 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
   }
 }
 
+// ---- plans ----
+struct RowsPlan {
+  int BM, m_tiles, n_tiles, split, k_per_cta, slice, stages;
+  uint32_t stage_bytes, exchange_bytes, smem;
+  float us;
+};
+constexpr uint32_t kSmemAlone = 222u * 1024, kSmemOfTwo = 110u * 1024;  // stages and exchange of a CTA alone on its SM, of one of two
+
+// CTAs that run at a time in clusters of `split`, `per_sm` on an SM: a cluster lies within one GPC, so that clusters of three and
+// more leave SMs over.
+int resident_ctas(int split, int per_sm, int sms) {
+  static std::atomic<int> known[64][9][2];
+  int dev = 0;
+  if (split == 1 || cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
+    cudaGetLastError();
+    return sms * per_sm;
+  }
+  std::atomic<int>& slot = known[dev][split][per_sm - 1];
+  int ctas = slot.load(std::memory_order_relaxed);
+  if (ctas > 0) return ctas;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = (per_sm == 2 ? kSmemOfTwo : kSmemAlone) + kBarBytes + 1024;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(sms / split * split));
+  int clusters = 0;
+  static std::atomic<int> granted[64];
+  if (ensure_dynamic_smem(gemm_rows_kernel<__half>, kSmemAlone + kBarBytes + 1024, granted) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, gemm_rows_kernel<__half>, &cfg) != cudaSuccess || clusters <= 0) {
+    cudaGetLastError();
+    clusters = sms * per_sm / split;
+  }
+  slot.store(clusters * split, std::memory_order_relaxed);
+  return clusters * split;
+}
+
+// The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
+// bytes that the busiest SM copies at 145 GB/s, or the call's bytes at 7.9 TB/s, the longer of the two and half of the other; 0.23 for
+// an exchange and its bytes at 16 GB/s an SM; 0.012 a row of the epilogue; 0.48 a further round of CTAs.  Fitted to 1100 timings (M 8 to
+// 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts): 16 % rms off, and its choices 3 % slower
+// than the best of all that were timed.
+RowsPlan plan_rows(int M, int N, int K, int sms) {
+  const int n_tiles = (N + kTileN - 1) / kTileN, k_steps = (K + kStepK - 1) / kStepK;
+  const float call = 0.126f * 1e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N);
+  RowsPlan best{};
+  int last = 0;
+  for (int cap : {256, 192, 128, 96, 64, 48, 32}) {
+    const int m_tiles = (M + cap - 1) / cap;
+    if (m_tiles == last) continue;
+    last = m_tiles;
+    const int BM = ((M + m_tiles - 1) / m_tiles + 15) / 16 * 16, rows = std::min(M, BM);
+    const int64_t tiles = (int64_t)m_tiles * n_tiles;
+    const uint32_t stage_bytes = kWeightBytes + (uint32_t)BM * kStepK;
+    for (int want : {1, 2, 3, 4, 6, 8}) {
+      if (want > 1 && (want > k_steps / 2 || tiles * want > 2 * sms)) break;
+      const int k_per_cta = (k_steps + want - 1) / want, split = (k_steps + k_per_cta - 1) / k_per_cta;
+      if (split != want) continue;
+      const int64_t ctas = tiles * split;
+      const int per_sm = BM <= 128 && ctas > sms ? 2 : 1;
+      const int64_t room = resident_ctas(split, per_sm, sms), rounds = (ctas + room - 1) / room;
+      const float busiest = (float)(rounds == 1 ? (ctas + sms - 1) / sms : rounds * per_sm);
+      const float copy = 6.9e-6f * busiest * (float)k_per_cta * (float)stage_bytes;
+      float us = 2.3f + 0.48f * (float)(rounds - 1) + std::max(copy, call) + 0.5f * std::min(copy, call) +
+                 0.0118f * busiest * (float)rows / (float)split;
+      if (split > 1) us += 0.23f + 6.1e-5f * busiest * (float)(split - 1) / (float)split * (float)rows * 512.0f;
+      RowsPlan t{BM, m_tiles, n_tiles, split, k_per_cta, 0, 0, stage_bytes, 0, 0, us};
+      t.slice = split > 1 ? ((rows + split - 1) / split + 7) / 8 * 8 : BM;
+      t.exchange_bytes = (uint32_t)(split - 1) * (uint32_t)t.slice * kTileN * 4;
+      t.stages = std::min<int>(kMaxStages, (int)(((per_sm == 2 ? kSmemOfTwo : kSmemAlone) - t.exchange_bytes) / stage_bytes));
+      t.smem = (uint32_t)t.stages * stage_bytes + t.exchange_bytes + kBarBytes + 1024;
+      if (t.stages >= 3 && (best.BM == 0 || us < best.us)) best = t;
+    }
+  }
+  return best;
+}
+
+struct PairPlan {
+  int BN, m_tiles, n_tiles, pairs;
+  float us;
+};
+// The width of tiles that leaves the least work to the slowest pair.  The estimate, us: 3.6 for a launch and its latencies, 0.1 + 0.0009 BN a
+// step (the copies of a pair's two operands set the pace: 100 GB/s an SM), 3.9 more where outputs are stored one by one.
+// Measured / estimated: 512 x 4096 x 4096 BN = 128 11.9 / 10.5; 1024 x 4096 x 4096 BN = 256 17.2 / 14.2, 160 18.2 / 19.2; 2048 x 4096 x 11008
+// 256 59.1 / 56; 2048 x 8192 x 8192 256 87 / 88, 224 83 / 81.
+PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
+  const int pairs = std::max(1, sms / 2), k_steps = (K + kStepK - 1) / kStepK;
+  PairPlan best{};
+  for (int BN = 256; BN >= 128; BN -= 32) {
+    PairPlan t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0, 0.0f};
+    const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
+    t.pairs = (int)std::min<int64_t>(pairs, tiles);
+    t.us = 3.6f + (float)(rounds * k_steps) * (0.1f + 0.0009f * (float)BN) + (bulk ? 0.0f : 3.9f);
+    if (best.BN == 0 || t.us < best.us) best = t;
+  }
+  return best;
+}
+
+struct Plan {
+  bool pair;
+  RowsPlan rows;
+  PairPlan pairs;
+};
+Plan plan_gemm(int M, int N, int K, bool bulk, int sms) {
+  Plan p{};
+  p.pairs = plan_pairs(M, N, K, bulk, sms);
+  p.pair = M > 512 && (int64_t)p.pairs.m_tiles * p.pairs.n_tiles >= sms / 2;
+  if (p.pair) return p;
+  p.rows = plan_rows(M, N, K, sms);
+  p.pair = p.pairs.us < p.rows.us;
+  return p;
+}
+
+// ---- launches ----
 // K-major rows of bytes `ld` apart.
 bool encode_rows(CUtensorMap* map, const int8_t* ptr, int64_t ld, int K, int rows, int box_rows) {
   TensorMapEncodeFn fn = tensor_map_encode_fn();
@@ -612,34 +744,8 @@ bool encode_rows(CUtensorMap* map, const int8_t* ptr, int64_t ld, int K, int row
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct RowsPlan {
-  int BM, m_tiles, n_tiles, split, k_per_cta, slice, stages;
-  uint32_t stage_bytes, smem;
-};
-RowsPlan plan_rows(int M, int N, int K, int sms) {
-  RowsPlan r{};
-  r.m_tiles = (M + 255) / 256;
-  r.BM = ((M + r.m_tiles - 1) / r.m_tiles + 15) / 16 * 16;
-  r.n_tiles = (N + kTileN - 1) / kTileN;
-  r.stage_bytes = kWeightBytes + (uint32_t)r.BM * kStepK;
-  const int k_steps = (K + kStepK - 1) / kStepK;
-  const int slots = sms * (r.BM <= 128 ? 2 : 1), tiles = r.m_tiles * r.n_tiles;
-  r.split = std::max(1, std::min({8, slots / tiles, k_steps / 2}));
-  r.k_per_cta = (k_steps + r.split - 1) / r.split;
-  r.split = (k_steps + r.k_per_cta - 1) / r.k_per_cta;
-  const int rows = std::min(M, r.BM);
-  r.slice = r.split > 1 ? ((rows + r.split - 1) / r.split + 7) / 8 * 8 : r.BM;
-  // one CTA on an SM has all its shared memory for stages
-  const uint32_t ring = r.BM <= 128 && tiles * r.split > sms ? 108u * 1024 : 216u * 1024;
-  r.stages = std::min<int>(kMaxStages, (int)(ring / r.stage_bytes));
-  r.smem = (uint32_t)r.stages * r.stage_bytes + kBarBytes + 1024;
-  return r;
-}
-
 template <class T>
-std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
-  const int sms = sm_count();
-  const RowsPlan r = plan_rows(g.M, g.N, g.K, sms);
+std::string launch_rows_gemm(const GemmArgs& g, const RowsPlan& r, unsigned flags, cudaStream_t stream) {
   CUtensorMap tm_x, tm_w;
   if (!encode_rows(&tm_x, g.x, g.ldx, g.K, g.M, r.BM) || !encode_rows(&tm_w, g.w, g.ldw, g.K, g.N, kTileN))
     return "cuTensorMapEncodeTiled failed";
@@ -648,6 +754,7 @@ std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t str
   p.BM = r.BM; p.m_tiles = r.m_tiles;
   p.k_steps = (g.K + kStepK - 1) / kStepK;
   p.split = r.split; p.k_per_cta = r.k_per_cta; p.slice = r.slice; p.stages = r.stages;
+  p.exchange_bytes = r.exchange_bytes;
   p.early = (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0;
   p.stage_bytes = r.stage_bytes;
   p.tmem_cols = 32;
@@ -676,32 +783,18 @@ std::string launch_rows_gemm(const GemmArgs& g, unsigned flags, cudaStream_t str
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
 }
 
-// ---- which kernel ----
-struct PairTiles {
-  int BN, m_tiles, n_tiles, rounds;
-};
-// The width of tiles that leaves the least work to the slowest of `pairs` pairs.
-PairTiles plan_pairs(int M, int N, int pairs) {
-  PairTiles best{};
-  long best_cost = 0;
-  for (int BN = 256; BN >= 128; BN -= 32) {
-    PairTiles t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0};
-    t.rounds = (int)(((long)t.m_tiles * t.n_tiles + pairs - 1) / pairs);
-    const long cost = (long)t.rounds * BN;
-    if (best.BN == 0 || cost < best_cost) best = t, best_cost = cost;
-  }
-  return best;
-}
+// Outputs by TMA: rows that begin on 16 bytes.
+bool stores_in_bulk(const GemmArgs& g) { return reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo % 8 == 0; }
 
 template <class T>
-std::string launch_pairs(const GemmArgs& g, const PairTiles& t, int pairs, unsigned flags, cudaStream_t stream) {
+std::string launch_pairs(const GemmArgs& g, const PairPlan& t, unsigned flags, cudaStream_t stream) {
   PairParams p{};
   p.M = g.M; p.N = g.N;
   p.BN = t.BN; p.m_tiles = t.m_tiles; p.n_tiles = t.n_tiles;
   p.k_steps = (g.K + kStepK - 1) / kStepK;
   p.group_m = 8;
   p.early = (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0;
-  p.bulk = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo % 8 == 0;
+  p.bulk = stores_in_bulk(g);
   p.out = g.out; p.ldo = g.ldo;
   p.x_scales = g.x_scales; p.w_scales = g.w_scales; p.bias = g.bias;
   CUtensorMap tm_x, tm_w, tm_out;
@@ -721,7 +814,7 @@ std::string launch_pairs(const GemmArgs& g, const PairTiles& t, int pairs, unsig
   cudaError_t e = ensure_dynamic_smem(gemm_pair_kernel<T>, kPairSmem, granted);
   if (e != cudaSuccess) return cudaGetErrorString(e);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2u * (unsigned)std::min(pairs, t.m_tiles * t.n_tiles));
+  cfg.gridDim = dim3(2u * (unsigned)t.pairs);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
@@ -737,10 +830,21 @@ std::string launch_pairs(const GemmArgs& g, const PairTiles& t, int pairs, unsig
 
 template <class T>
 std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
-  const int pairs = std::max(1, sm_count() / 2);
-  const PairTiles t = plan_pairs(g.M, g.N, pairs);
-  if (g.M > 256 && t.m_tiles * t.n_tiles >= pairs / 2) return launch_pairs<T>(g, t, pairs, flags, stream);
-  return launch_rows_gemm<T>(g, flags, stream);
+  const int sms = std::max(2, sm_count());
+  // the plan of the latest problem: a function of the sizes alone
+  struct Kept {
+    int M = 0, N = 0, K = 0, sms = 0;
+    bool bulk = false;
+    Plan plan;
+  };
+  static thread_local Kept kept[16];
+  const bool bulk = stores_in_bulk(g);
+  Kept& k = kept[((unsigned)g.M * 31u + (unsigned)g.N * 7u + (unsigned)g.K) / 8u % 16u];
+  if (k.M != g.M || k.N != g.N || k.K != g.K || k.bulk != bulk || k.sms != sms) {
+    k.plan = plan_gemm(g.M, g.N, g.K, bulk, sms);
+    k.M = g.M, k.N = g.N, k.K = g.K, k.bulk = bulk, k.sms = sms;
+  }
+  return k.plan.pair ? launch_pairs<T>(g, k.plan.pairs, flags, stream) : launch_rows_gemm<T>(g, k.plan.rows, flags, stream);
 }
 
 }  // namespace
@@ -762,3 +866,21 @@ int clear_gemm_error(cudaStream_t stream) {
 
 }  // namespace int8
 }  // namespace blkq4
+
+extern "C" int int8_gemm_plan_sm100(int m, int n, int k, int* out8) {
+  using namespace blkq4::int8;
+  if (!out8 || m <= 0 || n <= 0 || k <= 0 || m > (1 << 28) || n > (1 << 28) || k > kMaxK) return -1;
+  for (int i = 0; i < 8; ++i) out8[i] = 0;
+  if (gemv_takes(m, n, k)) return 0;
+  const int sms = blkq4::sm_count() > 0 ? blkq4::sm_count() : 148;
+  const Plan p = plan_gemm(m, n, k, n % 8 == 0, sms);
+  const int k_steps = (k + kStepK - 1) / kStepK;
+  if (p.pair) {
+    const int v[8] = {2, kPairM, p.pairs.BN, p.pairs.m_tiles * p.pairs.n_tiles, 1, k_steps, kPairStages, (int)kPairSmem};
+    std::copy(v, v + 8, out8);
+  } else {
+    const int v[8] = {1, p.rows.BM, kTileN, p.rows.m_tiles * p.rows.n_tiles, p.rows.split, p.rows.k_per_cta, p.rows.stages, (int)p.rows.smem};
+    std::copy(v, v + 8, out8);
+  }
+  return 0;
+}

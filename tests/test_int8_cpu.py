@@ -143,3 +143,43 @@ def test_extension_refuses_cpu_tensors_and_wrong_types():
         rms_norm_int8(x, x[0], residual_out=x)
     with pytest.raises(TypeError, match="a tensor is wanted"):
         quantize_int8(None)
+
+
+def test_plans_cover_k_and_fit_on_an_sm(lib_built):
+    """Sizes from one to the largest: every part of K has steps, the stages a round of them, and the shared memory its place
+    (227 KB a CTA, and two of 110 KB with their barriers on an SM)."""
+    import random
+
+    from gemmlib_b200 import capi
+
+    rng = random.Random(0)
+    size = lambda top: round(2 ** rng.uniform(0, top))
+    seen = set()
+    for _ in range(5000):
+        m, n, k = size(14), size(16), min(131071, size(17))
+        p = capi.int8_gemm_plan(m, n, k)
+        seen.add(p["kernel"])
+        steps = -(-k // 128)
+        if p["kernel"] == "stream":
+            assert m <= 4
+            continue
+        assert p["smem"] <= 227 * 1024 and p["stages"] >= 3
+        assert p["tiles"] == -(-m // p["tile_m"]) * -(-n // p["tile_n"])
+        assert (p["split"] - 1) * p["steps"] < steps <= p["split"] * p["steps"]
+        if p["kernel"] == "one-cta":
+            assert p["tile_m"] % 16 == 0 and 16 <= p["tile_m"] <= 256 and p["tile_n"] == 128
+            rows = min(m, p["tile_m"])
+            collected = (p["split"] - 1) * (-(-(-(-rows // p["split"])) // 8) * 8) * 512 if p["split"] > 1 else 0
+            assert p["smem"] >= p["stages"] * (128 + p["tile_m"]) * 128 + collected + 1536
+            assert p["split"] == 1 or p["tiles"] * p["split"] <= 2 * 148
+        else:
+            assert p["tile_m"] == 256 and p["tile_n"] % 32 == 0 and 128 <= p["tile_n"] <= 256
+    assert seen == {"stream", "one-cta", "pair"}
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 131072), (1 << 29, 1, 1)])
+def test_plans_that_there_are_none_of(lib_built, m, n, k):
+    from gemmlib_b200 import capi
+
+    with pytest.raises(capi.BlkQ4Error):
+        capi.int8_gemm_plan(m, n, k)

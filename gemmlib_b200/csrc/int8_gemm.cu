@@ -97,6 +97,13 @@ __device__ __forceinline__ void st_async_v4(uint32_t dst, uint32_t bar, uint32_t
                "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
+// Waits for this thread's loads from tensor memory; the registers they go to are named, so that no use of them moves ahead of it.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  tc::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
@@ -335,13 +342,13 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
 //   FULL[s]       of the even CTA (the leader): the bytes of both CTAs' copies; its MMA thread waits
 //   EMPTY[s]      of each CTA, by a commit to both: the stage may be written again
 //   ACC_FULL[b]   of each CTA, by a commit to both        ACC_EMPTY[b]   of the leader: the epilogue warps of both CTAs
-constexpr int kEpiWarps = 4, kPairXWarp = 2 + kEpiWarps, kThreads = 32 * (kPairXWarp + 1);
+constexpr int kEpiWarps = 8, kPairXWarp = 2 + kEpiWarps, kThreads = 32 * (kPairXWarp + 1);
 constexpr int kPairM = 256, kPairMaxN = 256;
 constexpr int kPairStages = 6;
 constexpr uint32_t kPairHalfBytes = 128u * kStepK;            // one operand's rows of a stage, at most
 constexpr uint32_t kPairStageBytes = 2 * kPairHalfBytes;
 constexpr uint32_t kPairChunkBytes = 32u * 64u;               // 32 rows x 32 outputs
-constexpr uint32_t kPairOutBytes = kEpiWarps * 2 * kPairChunkBytes;
+constexpr uint32_t kPairOutBytes = kEpiWarps * kPairChunkBytes;
 constexpr uint32_t kPairScaleBytes = 2u * 2u * kPairMaxN * 4u;  // scales and biases of two tiles' columns
 constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + kPairOutBytes + kPairScaleBytes + 512 + 1024;
 static_assert(kPairSmem <= 227 * 1024);
@@ -519,20 +526,22 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     mma_done:;
     }
   } else {
-    // ---- epilogue: a warp empties the 32 rows of its quarter of the lanes, 32 outputs at a time, through two staging
-    // blocks of its own (64-byte rows, their 16-byte pieces swizzled by the row as TMA's 64-byte swizzle has them)
+    // ---- epilogue: a warp has the 32 rows of its quarter of the lanes and every second chunk of 32 outputs, which it brings
+    // to a staging block of its own (64-byte rows, their 16-byte pieces swizzled by the row as TMA's 64-byte swizzle has
+    // them).  The next chunk is on its way from tensor memory while one is scaled and packed, and the block is waited for only then.
+    // Four warps without this took 5.2 us a tile of 256 x 256, more than the MMAs of 2048 k; FIGURE2
     const int quarter = warp & 3, et = (int)threadIdx.x - 64;
     const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
-    uint8_t* stage = base_ptr + kOut + (warp - 2) * 2 * kPairChunkBytes;
+    uint8_t* stage = base_ptr + kOut + (warp - 2) * kPairChunkBytes;
+    const uint32_t stage_u32 = smem_u32(stage);
     T* out = reinterpret_cast<T*>(p.out);
     griddep_wait();
     PairWalk walk(p);
     int m_tile, n_tile;
-    uint32_t chunk = 0;
     for (uint32_t t = 0; walk.next(m_tile, n_tile); ++t) {
       const uint32_t b = t & 1u;
       const int n0 = n_tile * p.BN, row0 = m_tile * kPairM + (int)rank * 128 + quarter * 32;
-      // the columns' scales and biases, for all four warps; the buffer of the tile before last is free, since every warp has
+      // the columns' scales and biases, for all warps; the buffer of the tile before last is free, since every warp has
       // passed the barrier of the last one
       float* scales = reinterpret_cast<float*>(base_ptr + kScales) + b * 2 * kPairMaxN;
       float* biases = scales + kPairMaxN;
@@ -546,54 +555,56 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
       const bool ok = wait_cluster(acc_full(b), (t >> 1) & 1u, abort_flag, 0x1300 | b);
       if (__any_sync(0xffffffffu, !ok)) continue;  // on to the barriers of the tiles that are left, so that no warp waits for another
       tc::tc_fence_after();
-      for (int c0 = 0; c0 < p.BN; c0 += 32, ++chunk) {
+      const uint32_t acc = tmem_row + b * kPairMaxN;
+      uint32_t next[32];
+      int c0 = 32 * ((warp - 2) >> 2);
+      tc::tmem_ld_32x32b_x32(acc + (uint32_t)c0, next);
+      for (; c0 < p.BN; c0 += 64) {
         uint32_t r[32];
-        tc::tmem_ld_32x32b_x32(tmem_row + b * kPairMaxN + (uint32_t)c0, r);
-        tc::tmem_ld_wait();
-        if (c0 + 32 >= p.BN) {  // the accumulator is in registers: the MMAs of the tile after next may have it
+        tmem_ld_wait_for(next);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = next[i];
+        if (c0 + 64 < p.BN) {
+          tc::tmem_ld_32x32b_x32(acc + (uint32_t)c0 + 64u, next);
+        } else {  // all of the accumulator that is this warp's is in registers: the MMAs of the tile after next may have it
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_cluster(tc::map_to_cta(acc_empty(b), 0));
         }
-        uint8_t* dst = stage + (chunk & 1u) * kPairChunkBytes;
-        // the store of the chunk before last has read this block
-        if (p.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        uint32_t v[16];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 s4 = *reinterpret_cast<const float4*>(scales + c0 + q * 4);
+          const float4 b4 = *reinterpret_cast<const float4*>(biases + c0 + q * 4);
+          const uint32_t* a = r + q * 4;
+          v[q * 2] = pack2<T>(fmaf((float)(int)a[0] * x_scale, s4.x, b4.x), fmaf((float)(int)a[1] * x_scale, s4.y, b4.y));
+          v[q * 2 + 1] = pack2<T>(fmaf((float)(int)a[2] * x_scale, s4.z, b4.z), fmaf((float)(int)a[3] * x_scale, s4.w, b4.w));
+        }
+        if (p.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has read the block
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t v[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 s4 = *reinterpret_cast<const float4*>(scales + c0 + q * 8 + h * 4);
-            const float4 b4 = *reinterpret_cast<const float4*>(biases + c0 + q * 8 + h * 4);
-            const uint32_t* a = r + q * 8 + h * 4;
-            v[h * 2] = pack2<T>(fmaf((float)(int)a[0] * x_scale, s4.x, b4.x), fmaf((float)(int)a[1] * x_scale, s4.y, b4.y));
-            v[h * 2 + 1] = pack2<T>(fmaf((float)(int)a[2] * x_scale, s4.z, b4.z), fmaf((float)(int)a[3] * x_scale, s4.w, b4.w));
-          }
-          *reinterpret_cast<uint4*>(dst + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
+              make_uint4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
         if (p.bulk) {
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
             if (row0 < p.M && n0 + c0 < p.N)
               asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&tm_out), "r"(n0 + c0),
-                           "r"(row0), "r"(smem_u32(dst))
+                           "r"(row0), "r"(stage_u32)
                            : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
           __syncwarp();
           const int n = n0 + c0 + lane;
-          T v[32];
-#pragma unroll
-          for (int row = 0; row < 32; ++row)
-            v[row] = *reinterpret_cast<const T*>(dst + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
           T* at = out + (int64_t)row0 * p.ldo + n;
-#pragma unroll
-          for (int row = 0; row < 32; ++row, at += p.ldo)
-            if (n < p.N && row0 + row < p.M) *at = v[row];
-          __syncwarp();
+#pragma unroll 16
+          for (int row = 0; row < 32; ++row, at += p.ldo) {
+            const T o = *reinterpret_cast<const T*>(stage + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
+            if (n < p.N && row0 + row < p.M) *at = o;
+          }
         }
       }
     }
@@ -654,6 +665,9 @@ int resident_ctas(int split, int per_sm, int sms) {
   return clusters * split;
 }
 
+// All bytes of a call at 7.9 TB/s.
+float call_us(int M, int N, int K) { return 0.126e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
+
 // The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
 // bytes that the busiest SM copies at 145 GB/s, or the call's bytes at 7.9 TB/s, the longer of the two and half of the other; 0.23 for
 // an exchange and its bytes at 16 GB/s an SM; 0.012 a row of the epilogue; 0.48 a further round of CTAs.  Fitted to 1100 timings (M 8 to
@@ -661,7 +675,7 @@ int resident_ctas(int split, int per_sm, int sms) {
 // than the best of all that were timed.
 RowsPlan plan_rows(int M, int N, int K, int sms) {
   const int n_tiles = (N + kTileN - 1) / kTileN, k_steps = (K + kStepK - 1) / kStepK;
-  const float call = 0.126f * 1e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N);
+  const float call = call_us(M, N, K);
   RowsPlan best{};
   int last = 0;
   for (int cap : {256, 192, 128, 96, 64, 48, 32}) {
@@ -704,12 +718,14 @@ struct PairPlan {
 // 256 59.1 / 56; 2048 x 8192 x 8192 256 87 / 88, 224 83 / 81.
 PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
   const int pairs = std::max(1, sms / 2), k_steps = (K + kStepK - 1) / kStepK;
+  const float call = call_us(M, N, K);
   PairPlan best{};
   for (int BN = 256; BN >= 128; BN -= 32) {
     PairPlan t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0, 0.0f};
     const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
     t.pairs = (int)std::min<int64_t>(pairs, tiles);
-    t.us = 3.6f + (float)(rounds * k_steps) * (0.1f + 0.0009f * (float)BN) + (bulk ? 0.0f : 3.9f);
+    const float copy = (float)(rounds * k_steps) * (0.1f + 0.0009f * (float)BN);
+    t.us = 3.6f + std::max(copy, call) + 0.5f * std::min(copy, call) + (bulk ? 0.0f : 3.9f);
     if (best.BN == 0 || t.us < best.us) best = t;
   }
   return best;

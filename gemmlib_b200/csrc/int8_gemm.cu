@@ -538,20 +538,30 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     griddep_wait();
     PairWalk walk(p);
     int m_tile, n_tile;
-    for (uint32_t t = 0; walk.next(m_tile, n_tile); ++t) {
+    bool more = walk.next(m_tile, n_tile);
+    // a tile's scales and biases, fetched while the tile before it is stored: one column a thread, its row's scale a lane
+    float w_scale = 0.0f, bias = 0.0f, x_scale = 0.0f;
+    auto fetch = [&] {
+      const int n = n_tile * p.BN + et, m = m_tile * kPairM + (int)rank * 128 + quarter * 32 + lane;
+      const bool in = et < p.BN && n < p.N;
+      w_scale = in ? p.w_scales[n] : 0.0f;
+      bias = in && p.bias ? to_float(reinterpret_cast<const T*>(p.bias)[n]) : 0.0f;
+      x_scale = m < p.M ? p.x_scales[m] : 0.0f;
+    };
+    static_assert(32 * kEpiWarps >= kPairMaxN);
+    if (more) fetch();
+    for (uint32_t t = 0; more; ++t) {
       const uint32_t b = t & 1u;
       const int n0 = n_tile * p.BN, row0 = m_tile * kPairM + (int)rank * 128 + quarter * 32;
-      // the columns' scales and biases, for all warps; the buffer of the tile before last is free, since every warp has
-      // passed the barrier of the last one
+      const float row_scale = x_scale;
+      // for all warps; the buffer of the tile before last is free, since every warp has passed the barrier of the last one
       float* scales = reinterpret_cast<float*>(base_ptr + kScales) + b * 2 * kPairMaxN;
       float* biases = scales + kPairMaxN;
-      for (int i = et; i < p.BN; i += 32 * kEpiWarps) {
-        const bool in = n0 + i < p.N;
-        scales[i] = in ? p.w_scales[n0 + i] : 0.0f;
-        biases[i] = in && p.bias ? to_float(reinterpret_cast<const T*>(p.bias)[n0 + i]) : 0.0f;
-      }
-      const float x_scale = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.0f;
+      scales[et] = w_scale;
+      biases[et] = bias;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+      more = walk.next(m_tile, n_tile);
+      if (more) fetch();
       const bool ok = wait_cluster(acc_full(b), (t >> 1) & 1u, abort_flag, 0x1300 | b);
       if (__any_sync(0xffffffffu, !ok)) continue;  // on to the barriers of the tiles that are left, so that no warp waits for another
       tc::tc_fence_after();
@@ -577,8 +587,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
           const float4 s4 = *reinterpret_cast<const float4*>(scales + c0 + q * 4);
           const float4 b4 = *reinterpret_cast<const float4*>(biases + c0 + q * 4);
           const uint32_t* a = r + q * 4;
-          v[q * 2] = pack2<T>(fmaf((float)(int)a[0] * x_scale, s4.x, b4.x), fmaf((float)(int)a[1] * x_scale, s4.y, b4.y));
-          v[q * 2 + 1] = pack2<T>(fmaf((float)(int)a[2] * x_scale, s4.z, b4.z), fmaf((float)(int)a[3] * x_scale, s4.w, b4.w));
+          v[q * 2] = pack2<T>(fmaf((float)(int)a[0] * row_scale, s4.x, b4.x), fmaf((float)(int)a[1] * row_scale, s4.y, b4.y));
+          v[q * 2 + 1] = pack2<T>(fmaf((float)(int)a[2] * row_scale, s4.z, b4.z), fmaf((float)(int)a[3] * row_scale, s4.w, b4.w));
         }
         if (p.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has read the block
         __syncwarp();

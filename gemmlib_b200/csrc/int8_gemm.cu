@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <string>
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   // ---- the parts of a split tile: CTA o of the cluster collects the sums of activation rows [o * slice, (o + 1) * slice),
   // [part][4 rows][128 n][row], so that a lane moves 16 bytes and a warp 512 in a run.  The bytes complete on the owner's
   // barrier, so that it waits for them alone: two barriers of the whole cluster took 0.8 us each (M = 64, 4096 x 4096 in four
-  // parts FIGURE).  No CTA can leave before all that is sent to it has arrived.
+  // parts 7.7 -> 6.8 us).  No CTA can leave before all that is sent to it has arrived.
   const uint32_t part_words = (uint32_t)p.slice * kTileN;
   if (p.split > 1 && epilogue && !dead()) {
     tc::tc_fence_after();
@@ -529,7 +530,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     // ---- epilogue: a warp has the 32 rows of its quarter of the lanes and every second chunk of 32 outputs, which it brings
     // to a staging block of its own (64-byte rows, their 16-byte pieces swizzled by the row as TMA's 64-byte swizzle has
     // them).  The next chunk is on its way from tensor memory while one is scaled and packed, and the block is waited for only then.
-    // Four warps without this took 5.2 us a tile of 256 x 256, more than the MMAs of 2048 k; FIGURE2
+    // Four warps without this took 5.2 us a tile of 256 x 256, more than the MMAs of 2048 k; with eight, and a tile's scales fetched under the stores of
+    // the one before, 4096 x 128 x 28672 (25 tiles a pair) takes 82 us.
     const int quarter = warp & 3, et = (int)threadIdx.x - 64;
     const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
     uint8_t* stage = base_ptr + kOut + (warp - 2) * kPairChunkBytes;
@@ -675,12 +677,12 @@ int resident_ctas(int split, int per_sm, int sms) {
   return clusters * split;
 }
 
-// All bytes of a call at 7.9 TB/s.
-float call_us(int M, int N, int K) { return 0.126e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
+// All bytes of a call at 7.3 TB/s.
+float call_us(int M, int N, int K) { return 0.136e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
 
 // The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
-// bytes that the busiest SM copies at 145 GB/s, or the call's bytes at 7.9 TB/s, the longer of the two and half of the other; 0.23 for
-// an exchange and its bytes at 16 GB/s an SM; 0.012 a row of the epilogue; 0.48 a further round of CTAs.  Fitted to 1100 timings (M 8 to
+// bytes that the busiest SM copies at 130 GB/s, and the call's bytes at 7.3 TB/s, as the sides of a right angle; 0.26 for an exchange
+// and its bytes at 16 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further round of CTAs.  Fitted to 1100 timings (M 8 to
 // 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts): 16 % rms off, and its choices 3 % slower
 // than the best of all that were timed.
 RowsPlan plan_rows(int M, int N, int K, int sms) {
@@ -703,10 +705,10 @@ RowsPlan plan_rows(int M, int N, int K, int sms) {
       const int per_sm = BM <= 128 && ctas > sms ? 2 : 1;
       const int64_t room = resident_ctas(split, per_sm, sms), rounds = (ctas + room - 1) / room;
       const float busiest = (float)(rounds == 1 ? (ctas + sms - 1) / sms : rounds * per_sm);
-      const float copy = 6.9e-6f * busiest * (float)k_per_cta * (float)stage_bytes;
-      float us = 2.3f + 0.48f * (float)(rounds - 1) + std::max(copy, call) + 0.5f * std::min(copy, call) +
-                 0.0118f * busiest * (float)rows / (float)split;
-      if (split > 1) us += 0.23f + 6.1e-5f * busiest * (float)(split - 1) / (float)split * (float)rows * 512.0f;
+      const float copy = 7.8e-6f * busiest * (float)k_per_cta * (float)stage_bytes;
+      float us = 2.3f + 0.45f * (float)(rounds - 1) + std::sqrt(copy * copy + call * call) +
+                 0.0108f * busiest * (float)rows / (float)split;
+      if (split > 1) us += 0.26f + 6.1e-5f * busiest * (float)(split - 1) / (float)split * (float)rows * 512.0f;
       RowsPlan t{BM, m_tiles, n_tiles, split, k_per_cta, 0, 0, stage_bytes, 0, 0, us};
       t.slice = split > 1 ? ((rows + split - 1) / split + 7) / 8 * 8 : BM;
       t.exchange_bytes = (uint32_t)(split - 1) * (uint32_t)t.slice * kTileN * 4;
@@ -722,10 +724,11 @@ struct PairPlan {
   int BN, m_tiles, n_tiles, pairs;
   float us;
 };
-// The width of tiles that leaves the least work to the slowest pair.  The estimate, us: 3.6 for a launch and its latencies, 0.1 + 0.0009 BN a
-// step (the copies of a pair's two operands set the pace: 100 GB/s an SM), 3.9 more where outputs are stored one by one.
-// Measured / estimated: 512 x 4096 x 4096 BN = 128 11.9 / 10.5; 1024 x 4096 x 4096 BN = 256 17.2 / 14.2, 160 18.2 / 19.2; 2048 x 4096 x 11008
-// 256 59.1 / 56; 2048 x 8192 x 8192 256 87 / 88, 224 83 / 81.
+// The width of tiles that leaves the least work to the slowest pair.  The estimate, us: 3.8 for a launch and its latencies; 0.1 + 0.0009 BN a
+// step (the copies of a pair's two operands set the pace: 100 GB/s an SM), at least 0.013 BN a tile for its epilogue, and the call's bytes,
+// as above; 2 more where outputs are stored one by one.  Measured / estimated: 512 x 4096 x 4096 BN = 128 11.8 / 11.3; 1000 x 4096 x 4096
+// 256 16.3 / 15.3; 192 x 4096 x 11008 160 14.4 / 14.3; 256 x 8192 x 28672 224 54 / 55; 2048 x 4096 x 11008 256 58.9 / 57.4; 4096 x 128 x 28672 256
+// 82 / 95.
 PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
   const int pairs = std::max(1, sms / 2), k_steps = (K + kStepK - 1) / kStepK;
   const float call = call_us(M, N, K);
@@ -734,8 +737,8 @@ PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
     PairPlan t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0, 0.0f};
     const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
     t.pairs = (int)std::min<int64_t>(pairs, tiles);
-    const float copy = (float)(rounds * k_steps) * (0.1f + 0.0009f * (float)BN);
-    t.us = 3.6f + std::max(copy, call) + 0.5f * std::min(copy, call) + (bulk ? 0.0f : 3.9f);
+    const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN), 0.013f * (float)BN);
+    t.us = 3.8f + std::sqrt(copy * copy + call * call) + (bulk ? 0.0f : 2.0f);
     if (best.BN == 0 || t.us < best.us) best = t;
   }
   return best;

@@ -15,6 +15,7 @@
 #include <cstdint>
 #include <string>
 
+#include "blkq4_common.cuh"
 #include "int8.cuh"
 
 namespace blkq4 {
@@ -144,15 +145,14 @@ __device__ __forceinline__ void store_q(int8_t* row, bool vec, int chunk, int co
   }
 }
 
-// THREADS threads a row, NV chunks of 8 elements a thread (0: any number, two passes).  32 threads: four rows a CTA.
-template <int OP, class T, bool VEC, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) rows_kernel(const RowsParams p) {
+// blockDim.x threads a row, NV chunks of 8 elements a thread (0: any number, two passes); WARP: a warp a row, four rows a CTA.
+template <int OP, class T, bool VEC, int NV, int MAXT, bool WARP>
+__global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int kRows = THREADS < 128 ? 128 / THREADS : 1;
-  const int tid = (int)threadIdx.x % THREADS;
-  const int64_t row = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / THREADS;
-  if (kRows > 1 && row >= p.rows) return;  // whole warps
+  const int threads = WARP ? 32 : (int)blockDim.x, tid = WARP ? (int)threadIdx.x % 32 : (int)threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : (int64_t)blockIdx.x;
+  if (WARP && row >= p.rows) return;  // whole warps
 
   float t[NV > 0 ? NV : 1][8];
   float sum = 0.0f;
@@ -164,11 +164,11 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) rows_kernel(con
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      row_values<OP, T, VEC>(p, row, i * THREADS + tid, false, t[i], sum);
+      row_values<OP, T, VEC>(p, row, i * threads + tid, false, t[i], sum);
       take_top(t[i]);
     }
   } else {
-    for (int c = tid; c * 8 < p.cols; c += THREADS) {
+    for (int c = tid; c * 8 < p.cols; c += threads) {
       row_values<OP, T, VEC>(p, row, c, false, t[0], sum);
       take_top(t[0]);
     }
@@ -180,21 +180,20 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) rows_kernel(con
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   }
-  if constexpr (THREADS > 32) {
-    constexpr int kWarps = THREADS / 32;
-    __shared__ uint32_t tops[kWarps];
-    __shared__ float sums[kWarps];
-    if (tid % 32 == 0) {
+  if constexpr (!WARP) {
+    __shared__ uint32_t tops[32];
+    __shared__ float sums[32];
+    const int lane = tid % 32, warps = threads / 32;
+    if (lane == 0) {
       tops[tid / 32] = top;
       sums[tid / 32] = sum;
     }
     __syncthreads();
-    const int l = tid % 32 % kWarps;
-    top = __reduce_max_sync(0xffffffffu, tops[l]);
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
     if constexpr (kSums) {
-      sum = sums[l];
+      sum = lane < warps ? sums[lane] : 0.0f;
 #pragma unroll
-      for (int s = kWarps / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     }
   }
 
@@ -219,40 +218,40 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) rows_kernel(con
   };
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) write(i * THREADS + tid, t[i]);
+    for (int i = 0; i < NV; ++i) write(i * threads + tid, t[i]);
   } else {
-    for (int c = tid; c * 8 < p.cols; c += THREADS) {
+    for (int c = tid; c * 8 < p.cols; c += threads) {
       row_values<OP, T, VEC>(p, row, c, true, t[0], sum);
       write(c, t[0]);
     }
   }
 }
 
-template <int OP, class T, bool VEC, int THREADS, int NV>
+template <int OP, class T, bool VEC, int NV, int MAXT, bool WARP>
 std::string launch_instance(const RowsParams& p, cudaStream_t stream) {
+  const int per = 8 * (NV > 0 ? NV : 1);
   cudaLaunchConfig_t cfg = {};
-  constexpr int kRows = THREADS < 128 ? 128 / THREADS : 1;
-  cfg.gridDim = dim3((unsigned)((p.rows + kRows - 1) / kRows));
-  cfg.blockDim = dim3(THREADS < 128 ? 128 : THREADS);
+  cfg.gridDim = dim3((unsigned)(WARP ? (p.rows + 3) / 4 : p.rows));
+  cfg.blockDim = dim3((unsigned)(WARP ? 128 : NV > 0 ? ((p.cols + per - 1) / per + 31) / 32 * 32 : MAXT));
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, rows_kernel<OP, T, VEC, THREADS, NV>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, rows_kernel<OP, T, VEC, NV, MAXT, WARP>, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
 }
 
 template <int OP, class T, bool VEC>
 std::string launch_by_width(const RowsParams& p, cudaStream_t stream) {
-  const int chunks = (p.cols + 7) / 8;
-  if (chunks <= 64) return launch_instance<OP, T, VEC, 32, 2>(p, stream);
-  if (chunks <= 256) return launch_instance<OP, T, VEC, 128, 2>(p, stream);
-  if (chunks <= 1024) return launch_instance<OP, T, VEC, 256, 4>(p, stream);
-  if (chunks <= 4096) return launch_instance<OP, T, VEC, 1024, 4>(p, stream);
-  return launch_instance<OP, T, VEC, 1024, 0>(p, stream);
+  if (p.cols <= 1024) return launch_instance<OP, T, VEC, 4, 128, true>(p, stream);
+  if (p.cols <= 8192 && p.rows <= 2 * sm_count()) return launch_instance<OP, T, VEC, 1, 1024, false>(p, stream);
+  if (p.cols <= 8192) return launch_instance<OP, T, VEC, 4, 256, false>(p, stream);
+  if (p.cols <= 16384) return launch_instance<OP, T, VEC, 4, 512, false>(p, stream);
+  if (p.cols <= 32768) return launch_instance<OP, T, VEC, 4, 1024, false>(p, stream);
+  return launch_instance<OP, T, VEC, 0, 1024, false>(p, stream);
 }
 
 inline bool aligned(const void* p, int64_t ld, int bytes) {

@@ -317,7 +317,9 @@ extern "C" int blkq4_last_kernel_status(void* stream_ptr) {
   const int sk = blkq4::read_skinny_tc_error();
   if (sk != 0) return sk > 0 ? (0x20000 | sk) : sk;
   const int i8 = blkq4::int8::read_gemm_error();
-  return i8 > 0 ? (0x40000 | i8) : i8;
+  if (i8 != 0) return i8 > 0 ? (0x40000 | i8) : i8;
+  const int rows = blkq4::int8::read_rows_error();
+  return rows > 0 ? (0x80000 | rows) : rows;
 }
 extern "C" int blkq4_reset(void* stream_ptr) {
   auto stream = reinterpret_cast<cudaStream_t>(stream_ptr);
@@ -326,6 +328,7 @@ extern "C" int blkq4_reset(void* stream_ptr) {
   rc |= blkq4::clear_gemv_error(stream);
   rc |= blkq4::clear_skinny_tc_error(stream);
   rc |= blkq4::int8::clear_gemm_error(stream);
+  rc |= blkq4::int8::clear_rows_error(stream);
   rc |= blkq4::reset_static_scratch(stream);
   return rc == 0 ? 0 : -1;
 }

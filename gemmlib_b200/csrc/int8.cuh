@@ -27,9 +27,14 @@ struct RowsParams {
   int64_t lda, ldb, ldr, ldq;  // elements from row to row
   int rows, cols;
   float eps;
+  // set by the launcher
   bool q_vec;  // every row of q begins on 8 bytes
+  int parts, part_chunks;  // CTAs a row, chunks of 8 elements of each
 };
 std::string launch_rows(RowsOp op, Dtype dtype, const RowsParams& p, cudaStream_t stream);
+// Status word of the kernels' bounded waits: 0, or the first that gave up.
+int read_rows_error();
+int clear_rows_error(cudaStream_t stream);
 std::string launch_dequant(Dtype dtype, int rows, int cols, const int8_t* q, int64_t ldq, const float* scales, void* out,
                            int64_t ldo, cudaStream_t stream);
 

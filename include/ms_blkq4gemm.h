@@ -416,7 +416,7 @@ void blkq4_errmsg_destroy(void* errmsg);      /* delete                         
  * every in-kernel wait completed.  Waits on mbarriers are bounded; one that expires makes
  * the CTA drain and records (role << 8 | barrier) here instead of hanging the GPU (the
  * skinny kernel's word is reported with bit 16 set, that of the tensor-core kernel of up to 16 rows
- * with bit 17, that of the int8 product with bit 18).  -1 if the stream itself is in error.
+ * with bit 17, that of the int8 product with bit 18, that of the kernels that write int8 rows with bit 19).  -1 if the stream itself is in error.
  * No counterpart in the reference, whose kernels have no such waits.
  */
 int blkq4_last_kernel_status(void* stream);

@@ -578,6 +578,7 @@ std::string launch_stream(const RowsParams& p, cudaStream_t stream) {
 template <int OP, class T, bool VEC>
 std::string launch_by_width(const RowsParams& p, cudaStream_t stream) {
   if (p.cols <= 1024) return launch_instance<OP, T, VEC, 4, 128, kWarp>(p, 1, stream);
+  if (OP == kQuant && p.cols <= 2048) return launch_instance<OP, T, VEC, 8, 128, kWarp>(p, 1, stream);
   if (p.cols <= 8192) {
     if constexpr (OP == kQuant || OP == kNorm) return launch_instance<OP, T, VEC, 4, 256, kCta>(p, 1, stream);
     else return launch_instance<OP, T, VEC, 2, 512, kCta>(p, 1, stream);
@@ -613,9 +614,19 @@ std::string launch_op(RowsOp op, const RowsParams& p, cudaStream_t stream) {
   }
 }
 
-// T(scale * q): 16 values a thread and step; `lanes` (a power of two) threads of a CTA share a row.
+// Four bytes of q as two words of T(scale * q).
+template <class T>
+__device__ __forceinline__ void dequant4(uint32_t q, float scale, uint32_t& lo, uint32_t& hi) {
+  const char4 b = *reinterpret_cast<const char4*>(&q);
+  lo = pack2<T>(scale * (float)b.x, scale * (float)b.y);
+  hi = pack2<T>(scale * (float)b.z, scale * (float)b.w);
+}
+
+// T(scale * q); `lanes` (a power of two) threads of a CTA share a row.  VEC: rows of q and of the output begin on 16 bytes, 16 values
+// a step.  Else 8 values a step, those of 16 aligned bytes of the output: it has twice the bytes, and reads of q (by aligned 8
+// bytes where its rows begin on them: q_vec) are the easier to shift.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) dequant_kernel(int rows, int cols, int lanes, const int8_t* q, int64_t ldq,
+__global__ void __launch_bounds__(256) dequant_kernel(int rows, int cols, int lanes, bool q_vec, const int8_t* q, int64_t ldq,
                                                       const float* scales, T* out, int64_t ldo) {
   griddep_launch_dependents();
   griddep_wait();
@@ -624,22 +635,38 @@ __global__ void __launch_bounds__(256) dequant_kernel(int rows, int cols, int la
   const float scale = scales[row];
   q += row * ldq;
   out += row * ldo;
-  for (int c = threadIdx.x % lanes; c * 16 < cols; c += lanes) {
-    if (VEC && c * 16 + 16 <= cols) {
-      const uint4 u = *reinterpret_cast<const uint4*>(q + c * 16);
-      const uint32_t r[4] = {u.x, u.y, u.z, u.w};
-      uint32_t o[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char4 b = *reinterpret_cast<const char4*>(&r[i]);
-        o[2 * i] = pack2<T>(scale * (float)b.x, scale * (float)b.y);
-        o[2 * i + 1] = pack2<T>(scale * (float)b.z, scale * (float)b.w);
+  if constexpr (VEC) {
+    for (int c = threadIdx.x % lanes; c * 16 < cols; c += lanes) {
+      if (c * 16 + 16 <= cols) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q + (int64_t)c * 16);
+        uint4 lo, hi;
+        dequant4<T>(u.x, scale, lo.x, lo.y);
+        dequant4<T>(u.y, scale, lo.z, lo.w);
+        dequant4<T>(u.z, scale, hi.x, hi.y);
+        dequant4<T>(u.w, scale, hi.z, hi.w);
+        uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)c * 16);
+        dst[0] = lo;
+        dst[1] = hi;
+      } else {
+        for (int k = c * 16; k < cols; ++k) out[k] = from_float<T>(scale * (float)q[k]);
       }
-      uint4* dst = reinterpret_cast<uint4*>(out + c * 16);
-      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
-    } else {
-      for (int k = c * 16; k < min(c * 16 + 16, cols); ++k) out[k] = from_float<T>(scale * (float)q[k]);
+    }
+  } else {
+    const int before = (int)(reinterpret_cast<uintptr_t>(out) & 15u) / 2;  // elements that the row's first 16 bytes lack
+    const uint32_t shift = (uint32_t)(8 - before) % 8u * 8u;               // bits of q to drop from the 16 bytes it is read by
+    for (int c = threadIdx.x % lanes; c * 8 - before < cols; c += lanes) {
+      const int k0 = c * 8 - before, k1 = min(k0 + 8, cols);
+      if (q_vec && k0 >= 0 && c * 8 + 8 <= cols) {
+        const uint64_t hi = *reinterpret_cast<const uint64_t*>(q + (int64_t)c * 8);
+        const uint64_t lo = before ? *reinterpret_cast<const uint64_t*>(q + (int64_t)(c - 1) * 8) : hi;
+        const uint64_t v = shift ? lo >> shift | hi << (64u - shift) : lo;
+        uint4 o;
+        dequant4<T>((uint32_t)v, scale, o.x, o.y);
+        dequant4<T>((uint32_t)(v >> 32), scale, o.z, o.w);
+        *reinterpret_cast<uint4*>(out + k0) = o;
+      } else {
+        for (int k = max(k0, 0); k < k1; ++k) out[k] = from_float<T>(scale * (float)q[k]);
+      }
     }
   }
 }
@@ -647,9 +674,10 @@ __global__ void __launch_bounds__(256) dequant_kernel(int rows, int cols, int la
 template <class T>
 std::string launch_dequant_typed(int rows, int cols, const int8_t* q, int64_t ldq, const float* scales, T* out, int64_t ldo,
                                  cudaStream_t stream) {
+  const bool q_vec = reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
   const bool vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0 && aligned(out, ldo, 16);
   int lanes = 1;
-  while (lanes < 256 && lanes * 16 < cols) lanes *= 2;
+  while (lanes < 256 && lanes * (vec ? 16 : 8) < cols) lanes *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((rows + 256 / lanes - 1) / (256 / lanes)));
   cfg.blockDim = dim3(256);
@@ -659,7 +687,7 @@ std::string launch_dequant_typed(int rows, int cols, const int8_t* q, int64_t ld
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, vec ? dequant_kernel<T, true> : dequant_kernel<T, false>, rows, cols, lanes, q, ldq,
+  cudaError_t e = cudaLaunchKernelEx(&cfg, vec ? dequant_kernel<T, true> : dequant_kernel<T, false>, rows, cols, lanes, q_vec, q, ldq,
                                      scales, out, ldo);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));

@@ -253,6 +253,24 @@ def test_dequantize(dtype, cols):
     assert torch.equal(out, (r.values.float() * r.scales[:, None]).to(dtype))
 
 
+@pytest.mark.parametrize("q_pitch,q_offset,pitch,offset", [(512, 0, 507, 0), (512, 0, 507, 5), (504, 8, 512, 3), (509, 3, 512, 0), (509, 1, 511, 7)])
+def test_dequantize_rows_that_begin_anywhere(q_pitch, q_offset, pitch, offset):
+    from gemmlib_b200 import capi
+
+    rows, cols = 37, 501
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randint(-128, 128, (rows * q_pitch + 16,), generator=g, device="cuda", dtype=torch.int8)[q_offset:]
+    scales = torch.rand(rows, generator=g, device="cuda")
+    out = torch.full((rows * pitch + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+    capi.int8_rows_dequant(capi.INT8_BF16, rows, cols, (q, q_pitch), scales, (out[offset:], pitch))
+    torch.cuda.synchronize()
+    want = (q.as_strided((rows, cols), (q_pitch, 1)).float() * scales[:, None]).bfloat16()
+    inside = out[offset:].as_strided((rows, cols), (pitch, 1))
+    assert torch.equal(inside, want)
+    inside.fill_(7.0)
+    assert (out == 7).all()
+
+
 LAYOUTS = {
     "slice": lambda x: torch.cat([x, x], -1)[..., : x.shape[-1]],
     "odd offset": lambda x: torch.cat([x[..., :1], x], -1)[..., 1:],

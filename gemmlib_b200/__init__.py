@@ -1,4 +1,4 @@
-"""B200-native blockwise-int4 weight-only GEMM/GEMV (W4A16).
+"""B200-native blockwise-int4 weight-only GEMM/GEMV (W4A16), and an 8-bit path beside it (W8A8: ``int8_linear``).
 
 The product is the C-ABI shared library ``libms_blkq4gemm.so`` (entry points
 declared in ``include/ms_blkq4gemm.h``) built from the CUDA sources in
@@ -13,7 +13,7 @@ before the library exists.
 """
 import importlib
 
-__all__ = ["capi", "build", "ms_blkq4linear", "ms_blkq4linear_ext", "sharded"]
+__all__ = ["capi", "build", "ms_blkq4linear", "ms_blkq4linear_ext", "sharded", "int8_linear", "stack"]
 
 
 def __getattr__(name):

@@ -9,7 +9,7 @@ an output buffer, captures the whole pass once per row count M on its own stream
 replays it.  Inside the graph the skinny kernels are launched with
 ``BLKQ4_GEMM_EARLY_WEIGHT_FETCH``: the weights of layer i+1 stream in while layer i
 drains.  Consecutive layers that read the same buffer (q, k and v; gate and up) are one launch where a kernel
-takes them together with every bit of their own calls' results.
+takes them together with every bit of their own calls' results; ``Int8Linear`` layers that do share the int8 rows of the buffer.
 
 It runs the linears only: what sits between them in a model (attention, activation
 functions, norms) is the caller's and can be captured into the same graph by passing
@@ -21,6 +21,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .int8_linear import Int8Linear, Int8Rows, RMSNormInt8, quantize_int8, silu_mul_int8
 from .ms_blkq4linear import MAX_GROUP, BlkQ4Linear, can_share_launch, group_workspace_bytes, run_as_one, shares_launch, workspaces_owned_by
 
 
@@ -29,12 +30,21 @@ class LinearStack:
 
     Buffer ``"x"`` is the stack's input ([M, in_features of the first reader]); every other
     name is created on first use as an output and can be read by later steps.
+
+    ``int8_inputs``: step -> what makes the int8 rows that this step's ``Int8Linear`` multiplies, from the buffers: a norm
+    (which may write the residual's buffer), a gated activation.  Int8 steps without an entry quantize the buffer they read; those that follow
+    one another and read the same buffer share its rows.
     """
 
-    def __init__(self, steps: Sequence[Tuple[BlkQ4Linear, str, str]],
-                 between: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], None]]] = None):
+    def __init__(self, steps: Sequence[Tuple[BlkQ4Linear | Int8Linear, str, str]],
+                 between: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], None]]] = None,
+                 int8_inputs: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], Int8Rows]]] = None):
         self.steps = list(steps)
         self.between = dict(between or {})
+        self.int8_inputs = dict(int8_inputs or {})
+        for i in self.int8_inputs:
+            if not 0 <= i < len(self.steps) or not isinstance(self.steps[i][0], Int8Linear):
+                raise ValueError(f"int8_inputs names step {i}, which has no Int8Linear")
         self._graphs: Dict[int, Tuple[torch.cuda.CUDAGraph, Dict[str, torch.Tensor]]] = {}
         self._split_k: Dict[int, dict] = {}  # row count -> split-K workspaces of its graph
         self.device = self.steps[0][0].q_weights.device
@@ -84,16 +94,26 @@ class LinearStack:
         return launches
 
     def _run_eager(self, bufs, launches):
+        held = None  # the buffer that was quantized last and its rows, as long as nothing may have written it
         for run in launches:
             members = [self.steps[i] for i in run]
+            lyr, src, dst = members[0]
             if len(members) > 1:
-                run_as_one([lyr for lyr, _, _ in members], bufs[members[0][1]], [bufs[dst] for _, _, dst in members])
+                run_as_one([lyr for lyr, _, _ in members], bufs[src], [bufs[dst] for _, _, dst in members])
+            elif isinstance(lyr, Int8Linear):
+                make = self.int8_inputs.get(run[0])
+                if make is not None:
+                    held = src, make(bufs)
+                elif held is None or held[0] != src:
+                    held = src, quantize_int8(bufs[src])
+                lyr(held[1], out=bufs[dst])
             else:
-                lyr, src, dst = members[0]
                 lyr(bufs[src], out=bufs[dst])
             hook = self.between.get(run[-1])
             if hook is not None:
                 hook(bufs)
+            if hook is not None or (held is not None and any(held[0] == d for _, _, d in members)):
+                held = None
 
     def _capture(self, M: int):
         bufs = self._workspace(M)
@@ -145,7 +165,8 @@ class LinearStack:
         return len(self.steps)
 
     def weight_bytes(self) -> int:
-        return sum(l.q_weights.numel() + 2 * l.q_scales.numel() + l.q_zp.numel() for l, _, _ in self.steps)
+        return sum(l.weight_bytes() if isinstance(l, Int8Linear) else
+                   l.q_weights.numel() + 2 * l.q_scales.numel() + l.q_zp.numel() for l, _, _ in self.steps)
 
 
 def llama_like_stack(hidden: int, ffn: int, blocks: int, block_size: int, col_wise: bool, scale_only: bool,
@@ -169,3 +190,35 @@ def llama_like_stack(hidden: int, ffn: int, blocks: int, block_size: int, col_wi
                   (make(hidden, ffn), "gate", f"h{b % 2}")]
         src = f"h{b % 2}"
     return LinearStack(steps)
+
+
+def llama_like_int8_stack(hidden: int, ffn: int, blocks: int, device, sigma: float = 0.02, seed: int = 0, weight_fn=None,
+                          eps: float = 1e-5) -> LinearStack:
+    """The same seven linears with int8 weights and activations, and the norms and the gate of the block: buffer ``"x"`` is the
+    residual stream, to which every norm adds the output of the projection before it; q, k and v share the first norm's rows, o
+    reads q's output (attention is the caller's), gate and up share the second norm's, down reads silu(gate) * up.  After the
+    last block ``"x"`` is the stack's result."""
+    steps: List[Tuple[Int8Linear, str, str]] = []
+    int8_inputs: Dict[int, Callable] = {}
+    g = torch.Generator().manual_seed(seed)
+
+    def make(n, k):
+        w = weight_fn(n, k) if weight_fn else (torch.randn(n, k, generator=g) * sigma).to(torch.float16)
+        return Int8Linear(w.to(device))
+
+    def norm():
+        return RMSNormInt8((1 + 0.1 * torch.randn(hidden, generator=g)).to(device, torch.float16), eps)
+
+    def add_and_norm(n, name):
+        return lambda bufs: n(bufs[name], residual=bufs["x"], residual_out=bufs["x"])[0]
+
+    for b in range(blocks):
+        i, n = len(steps), norm()
+        int8_inputs[i] = (lambda bufs, n=n: n(bufs["x"])) if b == 0 else add_and_norm(n, "down")
+        src = "x" if b == 0 else "down"
+        steps += [(make(hidden, hidden), src, "q"), (make(hidden, hidden), src, "k"), (make(hidden, hidden), src, "v"),
+                  (make(hidden, hidden), "q", "o"), (make(ffn, hidden), "o", "gate"), (make(ffn, hidden), "o", "up"),
+                  (make(hidden, ffn), "gate", "down")]
+        int8_inputs[i + 4] = add_and_norm(norm(), "o")
+        int8_inputs[i + 6] = lambda bufs: silu_mul_int8(bufs["gate"], bufs["up"])
+    return LinearStack(steps, between={len(steps) - 1: lambda bufs: bufs["x"].add_(bufs["down"])}, int8_inputs=int8_inputs)

@@ -206,13 +206,13 @@ __device__ __forceinline__ uint32_t rounded(float t, float inverse) {
   return __float_as_uint(__fadd_rn(__fmul_rn(t, inverse), 12582912.0f));
 }
 
-// What a row's largest |t| (its bits) and its sum of squares say.
+// What a row's largest |t| (its bits) says.  (Divisions are what costs most here: a thread has 16 or 32 elements to spread them over,
+// so the row's scale is for one thread of it to compute.)
 struct Scale {
   bool finite;
-  float scale, up, inverse;
+  float up, inverse;
 };
-template <bool SQUARES>
-__device__ __forceinline__ Scale scale_of(const RowsParams& p, uint32_t top, float squares) {
+__device__ __forceinline__ Scale scale_of(uint32_t top) {
   Scale s;
   // A row with an infinity or NaN has no scale that its other values could be told by: it is NaN as a whole.
   s.finite = top < 0x7f800000u;
@@ -220,10 +220,14 @@ __device__ __forceinline__ Scale scale_of(const RowsParams& p, uint32_t top, flo
   // 127 / amax is no float below 2^-121: such rows are scaled up by 2^64 first
   s.up = amax < 0x1p-64f ? 0x1p64f : 1.0f;
   s.inverse = amax > 0.0f ? __fdiv_rn(127.0f, amax * s.up) : 0.0f;
-  s.scale = __fdiv_rn(amax, 127.0f);
-  if (SQUARES && amax > 0.0f) s.scale *= __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, (float)p.cols) + p.eps));
-  if (!s.finite) s.scale = __uint_as_float(0x7fc00000u);
   return s;
+}
+template <bool SQUARES>
+__device__ __forceinline__ void write_scale(const RowsParams& p, int64_t row, uint32_t top, float squares) {
+  const float amax = __uint_as_float(top);
+  float scale = __fdiv_rn(amax, 127.0f);
+  if (SQUARES && top > 0) scale *= __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, (float)p.cols) + p.eps));
+  p.scales[row] = top < 0x7f800000u ? scale : __uint_as_float(0x7fc00000u);
 }
 template <int OP, class T>
 __device__ __forceinline__ void write8(const Scale& s, int8_t* q, bool vec, int chunk, int cols, const Chunk<OP, T>& c) {
@@ -333,8 +337,8 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
       if constexpr (kSquares) squares = warp_sum(__uint_as_float(of.y));
     }
   }
-  const Scale scale = scale_of<kSquares>(p, top, squares);
-  if (tid == 0 && part == 0) p.scales[row] = scale.scale;
+  if (tid == 0 && part == 0) write_scale<kSquares>(p, row, top, squares);
+  const Scale scale = scale_of(top);
   int8_t* q = p.q + row * p.ldq;
   if constexpr (DEAL != kLoop) {
 #pragma unroll
@@ -535,8 +539,8 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
     asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
     top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[buffer][lane] : 0u);
     if constexpr (kSquares) squares = warp_sum(lane < warps ? all[buffer][lane] : 0.0f);
-    const Scale scale = scale_of<kSquares>(p, top, squares);
-    if (tid == 0) p.scales[row] = scale.scale;
+    if (tid == 0) write_scale<kSquares>(p, row, top, squares);
+    const Scale scale = scale_of(top);
     if (!ok) continue;
     int8_t* q = p.q + row * p.ldq;
 #pragma unroll

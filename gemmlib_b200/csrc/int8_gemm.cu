@@ -681,8 +681,8 @@ int resident_ctas(int split, int per_sm, int sms) {
 float call_us(int M, int N, int K) { return 0.136e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
 
 // The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
-// bytes that the busiest SM copies at 130 GB/s, and the call's bytes at 7.3 TB/s, as the sides of a right angle; 0.26 for an exchange
-// and its bytes at 16 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further round of CTAs.  Fitted to 1100 timings (M 8 to
+// bytes that the busiest SM copies at 130 GB/s, and the call's bytes at 7.3 TB/s (5.2 where few SMs ask for them), as the sides of a
+// right angle; 0.26 for an exchange and its bytes at 16 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further round of CTAs.  Fitted to 1100 timings (M 8 to
 // 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts): 16 % rms off, and its choices 3 % slower
 // than the best of all that were timed.
 RowsPlan plan_rows(int M, int N, int K, int sms) {
@@ -706,7 +706,8 @@ RowsPlan plan_rows(int M, int N, int K, int sms) {
       const int64_t room = resident_ctas(split, per_sm, sms), rounds = (ctas + room - 1) / room;
       const float busiest = (float)(rounds == 1 ? (ctas + sms - 1) / sms : rounds * per_sm);
       const float copy = 7.8e-6f * busiest * (float)k_per_cta * (float)stage_bytes;
-      float us = 2.3f + 0.45f * (float)(rounds - 1) + std::sqrt(copy * copy + call * call) +
+      const float all = ctas < sms ? call * (1.4f - 0.4f * (float)ctas / (float)sms) : call;
+      float us = 2.3f + 0.45f * (float)(rounds - 1) + std::sqrt(copy * copy + all * all) +
                  0.0108f * busiest * (float)rows / (float)split;
       if (split > 1) us += 0.26f + 6.1e-5f * busiest * (float)(split - 1) / (float)split * (float)rows * 512.0f;
       RowsPlan t{BM, m_tiles, n_tiles, split, k_per_cta, 0, 0, stage_bytes, 0, 0, us};

@@ -87,7 +87,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 // Programmatic dependent launch: nothing that another kernel of the stream wrote is read, and nothing written, before
-// griddep_wait, which returns once the kernels ahead in the stream have completed.
+// griddep_wait, which returns once the kernels ahead in the stream have completed.  The next kernel is let in (griddep_launch_dependents)
+// only after that: what it does ahead of its own wait - copies of weights, where the caller vouches for them - then
+// comes behind everything that was ahead of this kernel, such as the quantization of those weights.
 __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 #endif

@@ -156,7 +156,6 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   const int first_row = min(rows, part * p.slice), end_row = min(rows, first_row + p.slice);  // whose sums end up here
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
@@ -204,6 +203,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
         }
       }
       griddep_wait();
+      griddep_launch_dependents();
       while (i < ahead) step();
       while (i < count) {
         dst -= (uint32_t)p.stages * p.stage_bytes, bar -= 16u * (uint32_t)p.stages, parity ^= 1u;
@@ -438,7 +438,6 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
@@ -494,6 +493,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             }
           }
           griddep_wait();
+          griddep_launch_dependents();
         }
         for (; ks < p.k_steps; ++ks) {
           if (!wait(empty(s), parity, abort_flag, 0x1100 | s)) goto producer_done;
@@ -644,6 +644,13 @@ struct RowsPlan {
 };
 constexpr uint32_t kSmemAlone = 222u * 1024, kSmemOfTwo = 110u * 1024;  // stages and exchange of a CTA alone on its SM, of one of two
 
+// The most that a plan asks for, once a device.
+template <class T>
+cudaError_t allow_smem() {
+  static std::atomic<int> granted[64];
+  return ensure_dynamic_smem(gemm_rows_kernel<T>, kSmemAlone + kBarBytes + 1024, granted);
+}
+
 // CTAs that run at a time in clusters of `split`, `per_sm` on an SM: a cluster lies within one GPC, so that clusters of three and
 // more leave SMs over.
 int resident_ctas(int split, int per_sm, int sms) {
@@ -667,8 +674,7 @@ int resident_ctas(int split, int per_sm, int sms) {
   cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(sms / split * split));
   int clusters = 0;
-  static std::atomic<int> granted[64];
-  if (ensure_dynamic_smem(gemm_rows_kernel<__half>, kSmemAlone + kBarBytes + 1024, granted) != cudaSuccess ||
+  if (allow_smem<__half>() != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&clusters, gemm_rows_kernel<__half>, &cfg) != cudaSuccess || clusters <= 0) {
     cudaGetLastError();
     clusters = sms * per_sm / split;
@@ -792,8 +798,7 @@ std::string launch_rows_gemm(const GemmArgs& g, const RowsPlan& r, unsigned flag
   p.pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
   p.out = g.out; p.ldo = g.ldo;
   p.x_scales = g.x_scales; p.w_scales = g.w_scales; p.bias = g.bias;
-  static std::atomic<int> granted[64];
-  cudaError_t e = ensure_dynamic_smem(gemm_rows_kernel<T>, r.smem, granted);
+  cudaError_t e = allow_smem<T>();
   if (e != cudaSuccess) return cudaGetErrorString(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(r.m_tiles * r.n_tiles * r.split));

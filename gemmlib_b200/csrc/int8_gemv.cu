@@ -49,7 +49,6 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int c) {
 // MR >= M activation rows, R weight rows a warp, U pieces of 512 k of each in flight, CTAS resident on an SM: what is launched.
 template <class T, int MR, int R, int U, int CTAS>
 __global__ void __launch_bounds__(32 * kWarps, CTAS) gemv_kernel(const GemvParams p) {
-  griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int groups = (p.N + R - 1) / R, step = (int)gridDim.x * kWarps;
   // neighbouring groups go to different CTAs, so that every SM has the same number of them (give or take one)
@@ -77,6 +76,7 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) gemv_kernel(const GemvParam
                      : "memory");
   }
   griddep_wait();
+  griddep_launch_dependents();
   if (!p.early && g < groups) load(g, 0);
 
   for (; g < groups; g += step) {

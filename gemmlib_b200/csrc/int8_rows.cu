@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -227,7 +228,8 @@ __device__ __forceinline__ void write_scale(const RowsParams& p, int64_t row, ui
   const float amax = __uint_as_float(top);
   float scale = __fdiv_rn(amax, 127.0f);
   if (SQUARES && top > 0) scale *= __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, (float)p.cols) + p.eps));
-  p.scales[row] = top < 0x7f800000u ? scale : __uint_as_float(0x7fc00000u);
+  // (squares of which the sum is no float: 1 / sqrt would be 0)
+  p.scales[row] = top < 0x7f800000u && (!SQUARES || squares < INFINITY) ? scale : __uint_as_float(0x7fc00000u);
 }
 template <int OP, class T>
 __device__ __forceinline__ void write8(const Scale& s, int8_t* q, bool vec, int chunk, int cols, const Chunk<OP, T>& c) {
@@ -289,13 +291,13 @@ enum Deal {
 // blockDim.x threads a CTA, NV chunks a thread.
 template <int OP, class T, bool VEC, int NV, int MAXT, Deal DEAL>
 __global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
-  griddep_launch_dependents();
   const int threads = DEAL == kWarp ? 32 : (int)blockDim.x, tid = DEAL == kWarp ? (int)threadIdx.x % 32 : (int)threadIdx.x;
   const int parts = DEAL == kCluster ? p.parts : 1, part = DEAL == kCluster ? (int)blockIdx.x % parts : 0;
   const int64_t row = DEAL == kWarp ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : (int64_t)(blockIdx.x / (unsigned)parts);
   const int first = part * p.part_chunks + tid;
   if (DEAL == kCluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   griddep_wait();
+  griddep_launch_dependents();
   if (DEAL == kWarp && row >= p.rows) return;  // whole warps
 
   constexpr bool kSquares = Sums<OP, T>::kSquares;
@@ -436,7 +438,6 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
   const int threads = (int)blockDim.x - 32, tid = (int)threadIdx.x, warps = threads / 32;
   const int pieces = (p.cols + threads * 8 - 1) / (threads * 8);
   const uint32_t stage_bytes = sp.piece_bytes * (kTwo ? 2u : 1u), ring_u32 = smem_u32(ring);
-  griddep_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < sp.stages; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
   }
   __syncthreads();
   griddep_wait();
+  griddep_launch_dependents();
 
   int s = 0;
   uint32_t parity = 0;
@@ -632,8 +634,8 @@ __device__ __forceinline__ void dequant4(uint32_t q, float scale, uint32_t& lo, 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) dequant_kernel(int rows, int cols, int lanes, bool q_vec, const int8_t* q, int64_t ldq,
                                                       const float* scales, T* out, int64_t ldo) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
   if (row >= rows) return;
   const float scale = scales[row];

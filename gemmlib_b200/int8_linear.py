@@ -101,7 +101,7 @@ class Int8Linear(nn.Module):
         pad = -self.in_features % 16
         # kept with whole rows of 16 bytes, so that copies of the buffer have them too
         self.register_buffer("q_weights", nn.functional.pad(rows.values, (0, pad)) if pad else rows.values)
-        self.register_buffer("q_scales", rows.scales)
+        self.register_buffer("q_scales", rows.scales.clone())  # (the operators' rows and scales share their memory)
         self.bias = bias_tensor
         self.early_weight_fetch = True
         self._settled = False  # the first forward is a plain launch
@@ -112,6 +112,14 @@ class Int8Linear(nn.Module):
         self = cls.__new__(cls)
         nn.Module.__init__(self)
         self._set(Int8Rows(*weight), bias_tensor, dtype)
+        return self
+
+    def _apply(self, fn, recurse=True):
+        scales = self.q_scales
+        super()._apply(fn, recurse)
+        if self.q_scales.dtype != torch.float32:  # .half() and the like are for the model's 16-bit tensors
+            self.q_scales = scales.to(self.q_scales.device)
+        self._settled = False
         return self
 
     def _load_from_state_dict(self, *args, **kwargs):

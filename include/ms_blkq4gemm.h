@@ -327,13 +327,14 @@ int blkq4_gather_destroy(void* ctx);
  * and their product.  No counterpart in the reference.
  *
  *   - A row stands for scale * values.  scale = max|t| / 127 and values[k] = round(t[k] * (127 / max|t|)), half to even, where t
- *     is the row to be quantized in fp32.  A row of zeros has scale 0.  A row that holds an infinity or NaN (or whose sum with
- *     the residual overflows the 16-bit type) has scale NaN and values 0, so that whatever reads it is NaN in that row only.
+ *     is the row to be quantized in fp32.  A row of zeros has scale 0.  A row with an infinity or NaN among its inputs or its t
+ *     (a sum with the residual that overflows the 16-bit type, a product that overflows fp32) has scale NaN, so that whatever
+ *     reads it is NaN in that row only; so has a row whose sum of squares overflows fp32 (the norm of |x| beyond 1e17).
  *   - dtype: INT8_FP16 or INT8_BF16, the type of the 16-bit operands of the call.
  *   - ld*: elements from row to row (of an int8 matrix: bytes), at least the row's length.  *_size: bytes that may be
  *     accessed, at least those from the first to the last element.  Rows that all begin on 16 bytes (int8 ones of the first
  *     three calls: on 8) are read and written in vectors, others one element at a time with the same results.
- *   - Columns up to 2^28.  The norm's sum of squares is held in fp32: |x| up to 1e17.
+ *   - Columns up to 2^28.
  */
 #define INT8_FP16 0
 #define INT8_BF16 1

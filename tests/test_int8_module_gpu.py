@@ -53,6 +53,69 @@ def test_an_output_of_another_type_than_the_weights():
     assert (out.float() - layer(rows).float()).abs().max() <= 2.0 ** -8 * 1.01 * layer(rows).float().abs().max() + 2.0 ** -24
 
 
+def test_a_model_converted_to_another_type_keeps_its_scales():
+    from gemmlib_b200.int8_linear import Int8Linear
+
+    layer, x = Int8Linear(normal(32, 64), normal(32, seed=2)), normal(3, 64, seed=1)
+    want = layer(x)
+    same(copy.deepcopy(layer).half()(x), want)
+    other = copy.deepcopy(layer).to(torch.bfloat16)
+    assert other.q_scales.dtype == torch.float32 and torch.equal(other.q_scales, layer.q_scales)
+    same(other(x), want)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_forward_right_behind_the_quantization(rows):
+    """The weights of a second forward are fetched early: not before the quantizer ahead of the first one is done."""
+    from gemmlib_b200.int8_linear import Int8Linear, Int8Rows
+
+    w, x = normal(8192, 4096, seed=1, scale=0.02), normal(rows, 4096, seed=2)
+    want = Int8Linear(w)(x)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        layer = Int8Linear(w)  # into memory that another layer's weights were in
+        first, second = layer(x), layer(x)
+        same(first, want), same(second, want)
+        layer.q_weights.zero_()
+        del layer
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+
+    from tests._util import ROOT
+
+    code = """
+import torch
+from gemmlib_b200.int8_linear import Int8Rows, int8_linear, quantize_int8, rms_norm_int8, silu_mul_int8
+g = torch.Generator(device="cuda").manual_seed(0)
+made = []
+for m, k, n in ((1, 512, 256), (16, 4096, 512), (300, 1024, 256), (600, 256, 4096)):
+    x = torch.randn(m, k, generator=g, device="cuda").half()
+    q = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    made.append((x, Int8Rows(q, torch.full((n,), 1e-3, device="cuda"))))
+wide = torch.randn(700, 40000, generator=g, device="cuda").half()
+def run():
+    out = []
+    for x, w in made:
+        rows, h = rms_norm_int8(x, x[0], residual=x)
+        out += [int8_linear(rows, w), h, silu_mul_int8(x, x).dequantize(), quantize_int8(x).dequantize()]
+    return out + [quantize_int8(wide).dequantize(), quantize_int8(wide[:, :20000]).dequantize()]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(captured, run()))
+print("ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout + r.stderr
+
+
 def test_gradients_are_refused():
     from gemmlib_b200.int8_linear import Int8Linear, RMSNormInt8, rms_norm_int8
 

@@ -190,6 +190,29 @@ def test_rms_norm_residual_out_in_place(place, cols):
         assert torch.equal(both[:, cols:], keep)
 
 
+def test_rms_norm_of_values_whose_squares_overflow():
+    from gemmlib_b200.int8_linear import rms_norm_int8
+
+    x = normal(4, 300, dtype=torch.bfloat16)
+    x[1] *= 1e20
+    x[2] *= 1e16
+    rows = rms_norm_int8(x, torch.ones(300, dtype=torch.bfloat16, device="cuda"))
+    assert torch.isnan(rows.scales).tolist() == [False, True, False, False]
+    top = float(x[2].double().abs().max() / x[2].double().square().mean().sqrt()) / 127
+    assert abs(float(rows.scales[2]) - top) <= top * (NORM_ERROR + EPS24)
+
+
+@pytest.mark.parametrize("cols", [512, 9000, 70000])
+def test_rms_norm_of_a_tensor_added_to_itself_in_place(cols):
+    from gemmlib_b200.int8_linear import rms_norm_int8
+
+    x, w = normal(700, cols, dtype=torch.float16), normal(cols, dtype=torch.float16, seed=1)
+    want, h = rms_norm_int8(x, w, residual=x)
+    got, same = rms_norm_int8(x, w, residual=x, residual_out=x)
+    assert same.data_ptr() == x.data_ptr() and torch.equal(x, h)
+    assert torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+
+
 def test_rms_norm_refusals():
     from gemmlib_b200.int8_linear import rms_norm_int8
 

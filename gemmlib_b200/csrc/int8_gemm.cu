@@ -652,35 +652,36 @@ cudaError_t allow_smem() {
 }
 
 // CTAs that run at a time in clusters of `split`, `per_sm` on an SM: a cluster lies within one GPC, so that clusters of three and
-// more leave SMs over.
+// more leave SMs over.  (The occupancy query answers one CTA an SM for every kernel that allocates tensor memory; two do run.)
 int resident_ctas(int split, int per_sm, int sms) {
-  static std::atomic<int> known[64][9][2];
+  static std::atomic<int> known[64][9];
   int dev = 0;
   if (split == 1 || cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
     cudaGetLastError();
     return sms * per_sm;
   }
-  std::atomic<int>& slot = known[dev][split][per_sm - 1];
+  std::atomic<int>& slot = known[dev][split];
   int ctas = slot.load(std::memory_order_relaxed);
-  if (ctas > 0) return ctas;
+  if (ctas > 0) return ctas * per_sm;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kRowsThreads);
-  cfg.dynamicSmemBytes = (per_sm == 2 ? kSmemOfTwo : kSmemAlone) + kBarBytes + 1024;
+  cfg.dynamicSmemBytes = kSmemAlone + kBarBytes + 1024;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3((unsigned)(sms / split * split));
+  cfg.gridDim = dim3((unsigned)(sms * split));
   int clusters = 0;
   if (allow_smem<__half>() != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&clusters, gemm_rows_kernel<__half>, &cfg) != cudaSuccess || clusters <= 0) {
     cudaGetLastError();
-    clusters = sms * per_sm / split;
+    clusters = sms / split;
   }
-  slot.store(clusters * split, std::memory_order_relaxed);
-  return clusters * split;
+  ctas = clusters * split;
+  slot.store(ctas, std::memory_order_relaxed);
+  return ctas * per_sm;
 }
 
 // All bytes of a call at 7.3 TB/s.
@@ -732,10 +733,10 @@ struct PairPlan {
   float us;
 };
 // The width of tiles that leaves the least work to the slowest pair.  The estimate, us: 3.8 for a launch and its latencies; 0.1 + 0.0009 BN a
-// step (the copies of a pair's two operands set the pace: 100 GB/s an SM), at least 0.013 BN a tile for its epilogue, and the call's bytes,
+// step (the copies of a pair's two operands set the pace: 100 GB/s an SM), at least 0.8 + 0.0095 BN a tile for its epilogue, and the call's bytes,
 // as above; 2 more where outputs are stored one by one.  Measured / estimated: 512 x 4096 x 4096 BN = 128 11.8 / 11.3; 1000 x 4096 x 4096
 // 256 16.3 / 15.3; 192 x 4096 x 11008 160 14.4 / 14.3; 256 x 8192 x 28672 224 54 / 55; 2048 x 4096 x 11008 256 58.9 / 57.4; 4096 x 128 x 28672 256
-// 82 / 95.
+// 82 / 93.
 PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
   const int pairs = std::max(1, sms / 2), k_steps = (K + kStepK - 1) / kStepK;
   const float call = call_us(M, N, K);
@@ -744,7 +745,7 @@ PairPlan plan_pairs(int M, int N, int K, bool bulk, int sms) {
     PairPlan t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0, 0.0f};
     const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
     t.pairs = (int)std::min<int64_t>(pairs, tiles);
-    const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN), 0.013f * (float)BN);
+    const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN), 0.8f + 0.0095f * (float)BN);
     t.us = 3.8f + std::sqrt(copy * copy + call * call) + (bulk ? 0.0f : 2.0f);
     if (best.BN == 0 || t.us < best.us) best = t;
   }

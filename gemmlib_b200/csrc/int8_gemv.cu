@@ -150,9 +150,15 @@ std::string launch_instance(const GemvParams& p, cudaStream_t stream) {
 
 template <class T>
 std::string launch_typed(const GemvParams& p, cudaStream_t stream) {
-  // One row: single weight rows, so that the last ones are shared evenly.  More: two at a time, since the products, not the loads,
-  // take the issue slots.  Measured on B200, back to back in a graph, us, one / two / four weight rows a warp: M = 1, 4096 x 4096
-  // 3.9 / 4.4 / 5.0, 8192 x 28672 36.7 / 38.5 / 44; M = 2, 4096 x 11008 11.7 / 9.7 / -; M = 4, 4096 x 4096 9.3 / 5.3 / 5.8.
+  // One activation row: single weight rows, so that the last ones are shared evenly.  More: two at a time, since the products, not the
+  // loads, take the issue slots.  Short rows: more of them at a time, as many pieces as a row has.  Measured on B200, back to back
+  // in a graph, us, one / two / four weight rows a warp with four pieces each: M = 1, 4096 x 4096 3.9 / 4.4 / 5.0, 8192 x 28672
+  // 36.7 / 38.5 / 44; M = 2, 4096 x 11008 11.7 / 9.7 / -; M = 4, 4096 x 4096 9.3 / 5.3 / 5.8.  M = 1, 512 x 20000: one row, four pieces
+  // 5.7; two, two 4.2; four, one 3.2; 1024 x 20000: 6.2, 5.3, 5.6.
+  if (p.M <= 2 && p.K <= 1024) {
+    if (p.M == 1) return p.K <= 512 ? launch_instance<T, 1, 4, 1, 4>(p, stream) : launch_instance<T, 1, 2, 2, 4>(p, stream);
+    return p.K <= 512 ? launch_instance<T, 2, 4, 1, 4>(p, stream) : launch_instance<T, 2, 2, 2, 4>(p, stream);
+  }
   if (p.M == 1) return launch_instance<T, 1, 1, 4, 4>(p, stream);
   if (p.M == 2) return launch_instance<T, 2, 2, 4, 2>(p, stream);
   return launch_instance<T, 4, 2, 4, 2>(p, stream);
@@ -160,10 +166,14 @@ std::string launch_typed(const GemvParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// The tensor-core kernel's calls have some 2 us more of set-up and hand-overs, this one's products take 30 us a GB and row.
-// Measured, this one / tensor cores, us: M = 2, 4096 x 11008 9.7 / 9.9; M = 4, 2048 x 2048 2.8 / 8.1, 4096 x 4096 5.3 / 6.8, 4096 x
-// 11008 11.3 / 10.0; M = 8, 1024 x 1024 4.7 / 3.8.
-bool gemv_takes(int M, int N, int K) { return M <= 2 || (M <= 4 && (int64_t)N * K <= (24 << 20)); }
+// The tensor-core kernel's calls have some 2 us more of set-up and hand-overs, this one's products take 30 us a GB and row, and a
+// warp has a whole row of weights to itself, however few and long they are.  Measured, this one / tensor cores, us: M = 2, 4096 x
+// 11008 9.7 / 9.9; M = 4, 2048 x 2048 2.8 / 8.1, 4096 x 4096 5.3 / 6.8, 4096 x 11008 11.3 / 10.0; M = 8, 1024 x 1024 4.7 / 3.8; M = 1,
+// 8192 x 1024 5.4 / 4.5, 28672 x 1024 17.3 / 9.4, 11008 x 4096 9.6 / 10.5.
+bool gemv_takes(int M, int N, int K) {
+  if (K >= 8192 && N <= 2048) return false;
+  return M <= 2 || (M <= 4 && (int64_t)N * K <= (24 << 20));
+}
 
 std::string launch_gemv(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream) {
   const GemvParams p{g.M, g.N, g.K, (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0, g.x, g.ldx, g.x_scales, g.w, g.ldw, g.w_scales,

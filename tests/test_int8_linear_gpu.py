@@ -36,7 +36,7 @@ def check_close(got, x, w, bias=None):
 
 
 SHAPES = [  # rows, in_features, out_features: tiles and steps that end inside, one to many rows, K split or not
-    (1, 1, 1), (1, 16, 8), (1, 128, 128), (1, 100, 130), (1, 4096, 4096), (2, 4096, 1000), (7, 5001, 129), (8, 8192, 256),
+    (1, 1, 1), (1, 16, 8), (1, 500, 3001), (2, 512, 777), (1, 1000, 2050), (2, 1024, 99), (2, 530, 1500), (3, 5001, 70), (1, 20000, 300), (4, 9000, 2000), (1, 128, 128), (1, 100, 130), (1, 4096, 4096), (2, 4096, 1000), (7, 5001, 129), (8, 8192, 256),
     (15, 129, 127), (16, 256, 64), (17, 1000, 1237), (31, 2048, 384), (33, 640, 2048), (64, 4096, 512), (65, 127, 100),
     (100, 11008, 96), (127, 384, 641), (128, 1024, 1024), (129, 1024, 136), (200, 2000, 520), (255, 130, 300), (256, 512, 256),
     (257, 512, 513), (300, 4096, 768), (333, 5001, 1237), (512, 256, 1024), (513, 1040, 264), (1000, 136, 2000), (1024, 1024, 1024),

@@ -397,7 +397,7 @@ int int8_gemm_sm100(
   unsigned flags,
   void* error_message);
 
-/* Host-only description of the work plan of int8_gemm_sm100 for a contiguous output (nothing is launched; 148 SMs are assumed
+/* Host-only description of the work plan of int8_gemm_sm100 for operand rows k bytes apart (to the next 16) and a contiguous output (nothing is launched; 148 SMs are assumed
  * without a device): out8[0] kernel (0 = weights streamed through registers, 1 = one CTA a tile or a part of one, 2 = pairs of
  * CTAs), and for kernels 1 and 2 [1] activation rows and [2] weight rows of a tile, [3] tiles, [4] parts of K, [5] steps of 128 k a part,
  * [6] stages, [7] bytes of shared memory. */

@@ -688,12 +688,12 @@ int resident_ctas(int split, int per_sm, int sms) {
 float call_us(int M, int N, int K) { return 0.136e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
 
 // The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
-// bytes that the busiest SM copies at 130 GB/s (90 where operand rows begin inside the 128 bytes of a line: `lines` is that they do
-// not), and the call's bytes at 7.3 TB/s (5.2 where few SMs ask for them), as the sides of a
+// bytes that the busiest SM copies at 130 GB/s (90 where operand rows do not all begin on 32 bytes, `sectors`: pitches of 5008 / 5024 / 5120
+// bytes, 4096 x 5001 x 8192: 136 / 115 / 109 us), and the call's bytes at 7.3 TB/s (5.2 where few SMs ask for them), as the sides of a
 // right angle; 0.26 for an exchange and its bytes at 23 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further round of CTAs.  Fitted to 1100 timings (M 8 to
 // 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts): 16 % rms off, and its choices 3 % slower
 // than the best of all that were timed.
-RowsPlan plan_rows(int M, int N, int K, bool lines, int sms) {
+RowsPlan plan_rows(int M, int N, int K, bool sectors, int sms) {
   const int n_tiles = (N + kTileN - 1) / kTileN, k_steps = (K + kStepK - 1) / kStepK;
   const float call = call_us(M, N, K);
   RowsPlan best{};
@@ -713,7 +713,7 @@ RowsPlan plan_rows(int M, int N, int K, bool lines, int sms) {
       const int per_sm = BM <= 128 && ctas > sms ? 2 : 1;
       const int64_t room = resident_ctas(split, per_sm, sms), rounds = (ctas + room - 1) / room;
       const float busiest = (float)(rounds == 1 ? (ctas + sms - 1) / sms : rounds * per_sm);
-      const float copy = (lines ? 7.8e-6f : 1.1e-5f) * busiest * (float)k_per_cta * (float)stage_bytes;
+      const float copy = (sectors ? 7.8e-6f : 1.1e-5f) * busiest * (float)k_per_cta * (float)stage_bytes;
       const float all = ctas < sms ? call * (1.4f - 0.4f * (float)ctas / (float)sms) : call;
       float us = 2.3f + 0.45f * (float)(rounds - 1) + std::sqrt(copy * copy + all * all) +
                  0.0108f * busiest * (float)rows / (float)split;
@@ -738,7 +738,7 @@ struct PairPlan {
 // as above; 2 more where outputs are stored one by one.  Measured / estimated: 512 x 4096 x 4096 BN = 128 11.8 / 11.3; 1000 x 4096 x 4096
 // 256 16.3 / 15.3; 192 x 4096 x 11008 160 14.4 / 14.3; 256 x 8192 x 28672 224 54 / 55; 2048 x 4096 x 11008 256 58.9 / 57.4; 4096 x 128 x 28672 256
 // 82 / 93.
-PairPlan plan_pairs(int M, int N, int K, bool bulk, bool lines, int sms) {
+PairPlan plan_pairs(int M, int N, int K, bool bulk, bool sectors, int sms) {
   const int pairs = std::max(1, sms / 2), k_steps = (K + kStepK - 1) / kStepK;
   const float call = call_us(M, N, K);
   PairPlan best{};
@@ -746,7 +746,7 @@ PairPlan plan_pairs(int M, int N, int K, bool bulk, bool lines, int sms) {
     PairPlan t{BN, (M + kPairM - 1) / kPairM, (N + BN - 1) / BN, 0, 0.0f};
     const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
     t.pairs = (int)std::min<int64_t>(pairs, tiles);
-    const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN) * (lines ? 1.0f : 1.4f), 0.8f + 0.0095f * (float)BN);
+    const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN) * (sectors ? 1.0f : 1.4f), 0.8f + 0.0095f * (float)BN);
     t.us = 3.8f + std::sqrt(copy * copy + call * call) + (bulk ? 0.0f : 2.0f);
     if (best.BN == 0 || t.us < best.us) best = t;
   }
@@ -758,12 +758,12 @@ struct Plan {
   RowsPlan rows;
   PairPlan pairs;
 };
-Plan plan_gemm(int M, int N, int K, bool bulk, bool lines, int sms) {
+Plan plan_gemm(int M, int N, int K, bool bulk, bool sectors, int sms) {
   Plan p{};
-  p.pairs = plan_pairs(M, N, K, bulk, lines, sms);
+  p.pairs = plan_pairs(M, N, K, bulk, sectors, sms);
   p.pair = M > 512 && (int64_t)p.pairs.m_tiles * p.pairs.n_tiles >= sms / 2;
   if (p.pair) return p;
-  p.rows = plan_rows(M, N, K, lines, sms);
+  p.rows = plan_rows(M, N, K, sectors, sms);
   p.pair = p.pairs.us < p.rows.us;
   return p;
 }
@@ -871,15 +871,15 @@ std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream)
   // the plan of the latest problem: a function of the sizes alone
   struct Kept {
     int M = 0, N = 0, K = 0, sms = 0;
-    bool bulk = false, lines = false;
+    bool bulk = false, sectors = false;
     Plan plan;
   };
   static thread_local Kept kept[16];
-  const bool bulk = stores_in_bulk(g), lines = g.ldx % 128 == 0 && g.ldw % 128 == 0;
+  const bool bulk = stores_in_bulk(g), sectors = g.ldx % 32 == 0 && g.ldw % 32 == 0;
   Kept& k = kept[((unsigned)g.M * 31u + (unsigned)g.N * 7u + (unsigned)g.K) / 8u % 16u];
-  if (k.M != g.M || k.N != g.N || k.K != g.K || k.bulk != bulk || k.lines != lines || k.sms != sms) {
-    k.plan = plan_gemm(g.M, g.N, g.K, bulk, lines, sms);
-    k.M = g.M, k.N = g.N, k.K = g.K, k.bulk = bulk, k.lines = lines, k.sms = sms;
+  if (k.M != g.M || k.N != g.N || k.K != g.K || k.bulk != bulk || k.sectors != sectors || k.sms != sms) {
+    k.plan = plan_gemm(g.M, g.N, g.K, bulk, sectors, sms);
+    k.M = g.M, k.N = g.N, k.K = g.K, k.bulk = bulk, k.sectors = sectors, k.sms = sms;
   }
   return k.plan.pair ? launch_pairs<T>(g, k.plan.pairs, flags, stream) : launch_rows_gemm<T>(g, k.plan.rows, flags, stream);
 }
@@ -910,7 +910,7 @@ extern "C" int int8_gemm_plan_sm100(int m, int n, int k, int* out8) {
   for (int i = 0; i < 8; ++i) out8[i] = 0;
   if (gemv_takes(m, n, k)) return 0;
   const int sms = blkq4::sm_count() > 0 ? blkq4::sm_count() : 148;
-  const Plan p = plan_gemm(m, n, k, n % 8 == 0, (k + 15) / 16 % 8 == 0, sms);
+  const Plan p = plan_gemm(m, n, k, n % 8 == 0, true, sms);
   const int k_steps = (k + kStepK - 1) / kStepK;
   if (p.pair) {
     const int v[8] = {2, kPairM, p.pairs.BN, p.pairs.m_tiles * p.pairs.n_tiles, 1, k_steps, kPairStages, (int)kPairSmem};

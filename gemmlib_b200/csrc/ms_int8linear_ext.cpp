@@ -73,13 +73,13 @@ void no_backward(const Tensor& x) {
               "The int8 operators have no backward pass: call them under torch.no_grad(), or detach the tensor");
 }
 
-// int8 rows in the shape of `x`, every row beginning on 16 bytes, and their scales.
+// int8 rows in the shape of `x`, every row beginning on 32 bytes (what the product copies fastest), and their scales.
 struct Int8Out {
   Tensor values, scales;
   int64_t ld;
 };
 Int8Out int8_like(const Tensor& x) {
-  const int64_t cols = x.size(-1), pitch = (cols + 15) / 16 * 16, rows = x.numel() / cols;
+  const int64_t cols = x.size(-1), pitch = (cols + 31) / 32 * 32, rows = x.numel() / cols;
   Int8Out o;
   o.ld = pitch;
   // One allocation for both, the scales behind the rows: at a token's sizes an allocation (0.7 us) is a good part of a call.

@@ -98,8 +98,8 @@ class Int8Linear(nn.Module):
             raise ValueError("weights must be [out_features, in_features]")
         self.out_features, self.in_features = rows.values.shape
         self.dtype = dtype
-        pad = -self.in_features % 16
-        # kept with whole rows of 16 bytes, so that copies of the buffer have them too
+        pad = -self.in_features % 32
+        # kept with whole rows of 32 bytes, so that copies of the buffer have them too
         self.register_buffer("q_weights", nn.functional.pad(rows.values, (0, pad)) if pad else rows.values)
         self.register_buffer("q_scales", rows.scales.clone())  # (the operators' rows and scales share their memory)
         self.bias = bias_tensor

@@ -12,8 +12,8 @@ EPS24 = 2.0 ** -24
 TYPES = [torch.float16, torch.bfloat16]
 
 
-def rows_of(n, k, seed, full=False):
-    """Random int8 rows on 16-byte pitches, with the whole range of int8 (-128 too), and scales."""
+def rows_of(n, k, seed):
+    """Random int8 rows, on pitches of any multiple of 16 bytes, with the whole range of int8 (-128 too), and scales."""
     from gemmlib_b200.int8_linear import Int8Rows
 
     g = torch.Generator(device="cuda").manual_seed(seed)

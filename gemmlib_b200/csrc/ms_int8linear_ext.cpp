@@ -278,13 +278,33 @@ torch::ScalarType dtype_of(PyObject* o, const char* call) {
 }
 void count_args(Py_ssize_t nargs, Py_ssize_t wanted, const char* signature) { TORCH_CHECK_TYPE(nargs == wanted, signature); }
 
-PyObject* wrap(const Int8Out& o, const Tensor* third = nullptr) {
-  PyObject* t = PyTuple_New(third ? 3 : 2);
-  if (!t) throw python_error();
-  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(o.values));
-  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(o.scales));
-  if (third) PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(*third));
-  return t;
+// Int8Rows, a named tuple of the Python module: made here, since its own constructor is a Python function.
+PyTypeObject* g_rows_type = nullptr;
+
+PyObject* wrap(const Int8Out& o) {
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) throw python_error();
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(o.values));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(o.scales));
+  if (!g_rows_type) return pair;
+  PyObject* args = PyTuple_Pack(1, pair);
+  Py_DECREF(pair);
+  if (!args) throw python_error();
+  PyObject* rows = PyTuple_Type.tp_new(g_rows_type, args, nullptr);
+  Py_DECREF(args);
+  if (!rows) throw python_error();
+  return rows;
+}
+
+PyObject* py_rows_type(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  count_args(nargs, 1, "int8_rows_type(cls)");
+  TORCH_CHECK_TYPE(PyType_Check(args[0]) && PyType_IsSubtype(reinterpret_cast<PyTypeObject*>(args[0]), &PyTuple_Type),
+                   "int8_rows_type: a subclass of tuple is wanted");
+  Py_INCREF(args[0]);
+  g_rows_type = reinterpret_cast<PyTypeObject*>(args[0]);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -306,7 +326,13 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     out = tensor(args[4], "rms_norm_int8");
   }
   const Int8Out o = rms_norm(tensor(args[0], "rms_norm_int8"), tensor(args[1], "rms_norm_int8"), eps, residual, &out);
-  return wrap(o, residual ? &out : nullptr);
+  PyObject* rows = wrap(o);
+  if (!residual) return rows;
+  PyObject* both = PyTuple_New(2);
+  if (!both) throw python_error();
+  PyTuple_SET_ITEM(both, 0, rows);
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(out));
+  return both;
   END_HANDLE_TH_ERRORS
 }
 
@@ -342,9 +368,10 @@ PyCFunction fast() {
 }
 
 PyMethodDef g_methods[] = {
-    {"int8_quantize", fast<py_quantize>(), METH_FASTCALL, "(values, scales) of the rows of x"},
-    {"rms_norm_int8", fast<py_rms_norm>(), METH_FASTCALL, "(values, scales) of the normed rows, and the sum where there is a residual"},
-    {"silu_mul_int8", fast<py_silu_mul>(), METH_FASTCALL, "(values, scales) of silu(gate) * up"},
+    {"int8_rows_type", fast<py_rows_type>(), METH_FASTCALL, "The tuple's subclass that int8 rows are returned as"},
+    {"int8_quantize", fast<py_quantize>(), METH_FASTCALL, "The rows of x in int8"},
+    {"rms_norm_int8", fast<py_rms_norm>(), METH_FASTCALL, "The normed rows, or them and the sum where there is a residual"},
+    {"silu_mul_int8", fast<py_silu_mul>(), METH_FASTCALL, "The rows of silu(gate) * up"},
     {"int8_dequantize", fast<py_dequantize>(), METH_FASTCALL, "scales * values"},
     {"int8_linear", fast<py_linear>(), METH_FASTCALL, "The product of int8 rows with an int8 weight"},
     {nullptr, nullptr, 0, nullptr}};

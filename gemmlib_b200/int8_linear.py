@@ -37,9 +37,12 @@ class Int8Rows(NamedTuple):
         return _dequantize(self.values, self.scales, dtype)
 
 
+ms_blkq4linear_ext.int8_rows_type(Int8Rows)  # what the extension's functions return
+
+
 def quantize_int8(x: torch.Tensor) -> Int8Rows:
     """Every row of ``x`` by its largest magnitude: scale = max|x| / 127, values = round(x * (127 / max|x|))."""
-    return Int8Rows(*_quantize(x))
+    return _quantize(x)
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None,
@@ -47,15 +50,12 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
     """``h / sqrt(mean(h^2) + eps) * weight`` of every row, quantized.  Without a residual h = x and the result is an
     ``Int8Rows``.  With one h = x + residual, rounded to their type, and the result is (``Int8Rows``, h); h goes to
     ``residual_out`` where that is given, which may be ``x`` or ``residual``."""
-    if residual is None:
-        return Int8Rows(*_rms_norm(x, weight, eps, None, residual_out))
-    values, scales, h = _rms_norm(x, weight, eps, residual, residual_out)
-    return Int8Rows(values, scales), h
+    return _rms_norm(x, weight, eps, residual, residual_out)
 
 
 def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor) -> Int8Rows:
     """``gate / (1 + exp(-gate)) * up``, quantized by row; gate and up may be halves of one tensor."""
-    return Int8Rows(*_silu_mul(gate, up))
+    return _silu_mul(gate, up)
 
 
 def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,

@@ -43,6 +43,7 @@ linear_group_supported = _mod.linear_group_supported
 linear_group_workspace_size = _mod.linear_group_workspace_size
 graph_workspace = _mod.graph_workspace
 graph_workspaces = _mod.graph_workspaces
+int8_rows_type = _mod.int8_rows_type
 int8_quantize = _mod.int8_quantize
 rms_norm_int8 = _mod.rms_norm_int8
 silu_mul_int8 = _mod.silu_mul_int8

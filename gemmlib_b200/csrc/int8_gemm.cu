@@ -360,7 +360,7 @@ struct PairParams {
   int m_tiles, n_tiles, k_steps;
   int group_m;  // m tiles that run side by side before the next column tiles
   int early;
-  int bulk;     // outputs by TMA: rows of the output begin on 16 bytes
+  int bulk;     // outputs by TMA: rows of the output begin and end on 16 bytes
   void* out;
   int64_t ldo;
   const float* x_scales;
@@ -687,12 +687,12 @@ int resident_ctas(int split, int per_sm, int sms) {
 // All bytes of a call at 7.3 TB/s.
 float call_us(int M, int N, int K) { return 0.136e-6f * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N); }
 
-// The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; the
-// bytes that the busiest SM copies at 130 GB/s (90 where operand rows do not all begin on 32 bytes, `sectors`: pitches of 5008 / 5024 / 5120
-// bytes, 4096 x 5001 x 8192: 136 / 115 / 109 us), and the call's bytes at 7.3 TB/s (5.2 where few SMs ask for them), as the sides of a
-// right angle; 0.26 for an exchange and its bytes at 23 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further round of CTAs.  Fitted to 1100 timings (M 8 to
-// 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts): 16 % rms off, and its choices 3 % slower
-// than the best of all that were timed.
+// The height of tiles and the split of K with the least estimated time.  The estimate, us: 2.3 for a launch and its latencies; as
+// the sides of a right angle, the bytes that the busiest SM copies at 130 GB/s (90 where operand rows do not all begin on 32 bytes,
+// `sectors`: pitches of 5008 / 5024 / 5120 bytes, 4096 x 5001 x 8192: 136 / 115 / 109 us) and the call's bytes at 7.3 TB/s (5.2
+// where few SMs ask for them); 0.26 for an exchange and its bytes at 23 GB/s an SM; 0.011 a row of the epilogue; 0.45 a further
+// round of CTAs.  Fitted to 1100 timings (M 8 to 512, 1024 x 1024 to 8192 x 28672, tiles of 16 to 256 rows, K in 1 to 8 parts):
+// 16 % rms off, and its choices 2 % slower than the best of all that were timed.
 RowsPlan plan_rows(int M, int N, int K, bool sectors, int sms) {
   const int n_tiles = (N + kTileN - 1) / kTileN, k_steps = (K + kStepK - 1) / kStepK;
   const float call = call_us(M, N, K);
@@ -820,8 +820,11 @@ std::string launch_rows_gemm(const GemmArgs& g, const RowsPlan& r, unsigned flag
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
 }
 
-// Outputs by TMA: rows that begin on 16 bytes.
-bool stores_in_bulk(const GemmArgs& g) { return reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo % 8 == 0; }
+// Outputs by TMA: rows that begin and end on 16 bytes (a store writes the whole of the 16 bytes in which the tensor's rows end, and
+// what lies behind them in a wider matrix is not this call's).
+bool stores_in_bulk(const GemmArgs& g) {
+  return reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo % 8 == 0 && g.N % 8 == 0;
+}
 
 template <class T>
 std::string launch_pairs(const GemmArgs& g, const PairPlan& t, unsigned flags, cudaStream_t stream) {

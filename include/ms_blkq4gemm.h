@@ -333,7 +333,7 @@ int blkq4_gather_destroy(void* ctx);
  *   - dtype: INT8_FP16 or INT8_BF16, the type of the 16-bit operands of the call.
  *   - ld*: elements from row to row (of an int8 matrix: bytes), at least the row's length.  *_size: bytes that may be
  *     accessed, at least those from the first to the last element.  Rows that all begin on 16 bytes (int8 ones of the first
- *     three calls: on 8) are read and written in vectors, others one element at a time with the same results.
+ *     three calls: on 8) are read and written in vectors, others in words or single elements, with the same results.
  *   - Columns up to 2^28.
  */
 #define INT8_FP16 0

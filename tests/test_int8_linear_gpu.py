@@ -100,6 +100,20 @@ def test_strided_operands_and_output(m, k, n):
         assert (out[:, :pad - 1] == 9).all() and (out[:, pad - 1 + n:] == 9).all()
 
 
+@pytest.mark.parametrize("m,k,n", [(2, 256, 4), (40, 512, 201), (600, 256, 4927), (600, 256, 4924), (600, 256, 4920), (4000, 64, 1001)])
+@pytest.mark.parametrize("wider", [1, 4, 7, 8, 16])
+def test_nothing_is_written_beside_an_output_in_a_wider_matrix(m, k, n, wider):
+    """Whatever its rows end on: 16, 8 or 2 bytes of the wider matrix's aligned rows."""
+    from gemmlib_b200.int8_linear import int8_linear
+
+    x, w = rows_of(m, k, 6), rows_of(n, k, 7)
+    want = int8_linear(x, w)
+    for pitch in {n + wider, -(-(n + wider) // 8) * 8}:
+        out = torch.full((m + 1, pitch), 9.0, dtype=torch.float16, device="cuda")
+        assert torch.equal(int8_linear(x, w, out=out[:m, :n]), want)
+        assert (out[:, n:] == 9).all() and (out[m] == 9).all()
+
+
 def test_no_rows_and_nan_rows():
     from gemmlib_b200.int8_linear import Int8Rows, int8_linear, quantize_int8
 

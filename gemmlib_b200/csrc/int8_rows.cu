@@ -202,8 +202,11 @@ __device__ __forceinline__ void add8(uint32_t (&a)[4], const uint32_t (&b)[4]) {
 
 // round(t * inverse), half to even, of |t * inverse| < 2^22: the sum's low mantissa bits are the integer.  The product is rounded
 // by itself: 16-bit inputs often stand exactly half-way between two integers (t = max / 2 is 63.5 steps), and a product of the
-// rounded inverse falls back on the tie where a fused one would always leave it to the side of the inverse's own error.
+// rounded inverse falls back on the tie where a fused one would always leave it to the side of the inverse's own error.  Gated
+// values are no short numbers: there one instruction does (2048 x 28672 57.5 -> 56.9 us).
+template <int OP>
 __device__ __forceinline__ uint32_t rounded(float t, float inverse) {
+  if (OP == kSiluMul) return __float_as_uint(fmaf(t, inverse, 12582912.0f));
   return __float_as_uint(__fadd_rn(__fmul_rn(t, inverse), 12582912.0f));
 }
 
@@ -241,7 +244,7 @@ __device__ __forceinline__ void write8(const Scale& s, int8_t* q, bool vec, int 
   }
   uint32_t b[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) b[e] = rounded(v[e], s.inverse);
+  for (int e = 0; e < 8; ++e) b[e] = rounded<OP>(v[e], s.inverse);
   int8_t* dst = q + (int64_t)chunk * 8;
   if (vec && chunk * 8 + 8 <= cols) {
     uint2 o;

@@ -108,6 +108,10 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
 __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
+// How two neighbouring outputs of a row may be stored at once: not; from every even n; in rows of even m from every even n, in the others
+// from every odd one (contiguous rows of an odd length).
+enum Stores { kSingle, kEven, kAlternate };
+
 struct Params {
   int M, N;
   int BM;          // activation rows of a tile, a multiple of 16, <= 256
@@ -120,7 +124,7 @@ struct Params {
   uint32_t exchange_bytes;  // behind the stages: what a CTA collects
   int early;       // weights may be copied before the kernels ahead in the stream have completed
   uint32_t stage_bytes, tmem_cols;
-  int pairs;       // two neighbouring outputs of a row may be stored at once
+  int stores;      // Stores
   void* out;
   int64_t ldo;
   const float* x_scales;
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = fmaf((float)(int)r[j] * x_scales[m + j], w_scale, bias);
-      if (p.pairs) {
+      if (p.stores == kEven) {
         // lanes of an even and an odd n trade: the even one stores the even row's two values, the odd one the odd row's
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -313,6 +317,19 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
           const uint32_t both = odd ? pack2<T>(got, keep) : pack2<T>(keep, got);
           if (m + j + odd < end && n < p.N)  // N is even: n and its partner are inside together
             *reinterpret_cast<uint32_t*>(out + (int64_t)(m0 + m + j + odd) * p.ldo + (n & ~1)) = both;
+        }
+      } else if (p.stores == kAlternate) {
+        // every second row begins inside a word: its words are the outputs of an odd n and the next one
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float give = odd ? v[j] : v[j + 1], keep = odd ? v[j + 1] : v[j];
+          const float got = __shfl_down_sync(0xffffffffu, give, 1);
+          T* at = out + (int64_t)(m0 + m + j + odd) * p.ldo + n;
+          if (m + j + odd < end && n < p.N) {
+            if (lane < 31 && n + 1 < p.N) *reinterpret_cast<uint32_t*>(at) = pack2<T>(keep, got);
+            else *at = from_float<T>(keep);
+          }
+          if (lane == 0 && m + j + 1 < end && n < p.N) at[p.ldo] = from_float<T>(v[j + 1]);
         }
       } else {
 #pragma unroll
@@ -612,10 +629,18 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
           __syncwarp();
           const int n = n0 + c0 + lane;
           T* at = out + (int64_t)row0 * p.ldo + n;
-#pragma unroll 16
-          for (int row = 0; row < 32; ++row, at += p.ldo) {
-            const T o = *reinterpret_cast<const T*>(stage + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
-            if (n < p.N && row0 + row < p.M) *at = o;
+          const uint8_t* from[4];  // the lane's output in rows of each swizzle
+#pragma unroll
+          for (int i = 0; i < 4; ++i) from[i] = stage + ((lane >> 3) ^ i) * 16 + (lane & 7) * 2;
+          if (row0 + 32 <= p.M && n0 + c0 + 32 <= p.N) {  // (with its tests in every row: 4000 x 640 x 19999 126 us, 103 without)
+#pragma unroll
+            for (int row = 0; row < 32; ++row, at += p.ldo) *at = *reinterpret_cast<const T*>(from[(row >> 1) & 3] + row * 64);
+          } else {
+#pragma unroll 8
+            for (int row = 0; row < 32; ++row, at += p.ldo) {
+              const T o = *reinterpret_cast<const T*>(from[(row >> 1) & 3] + row * 64);
+              if (n < p.N && row0 + row < p.M) *at = o;
+            }
           }
         }
       }
@@ -735,7 +760,7 @@ struct PairPlan {
 };
 // The width of tiles that leaves the least work to the slowest pair.  The estimate, us: 3.8 for a launch and its latencies; 0.1 + 0.0009 BN a
 // step (the copies of a pair's two operands set the pace: 100 GB/s an SM), at least 0.8 + 0.0095 BN a tile for its epilogue, and the call's bytes,
-// as above; 2 more where outputs are stored one by one.  Measured / estimated: 512 x 4096 x 4096 BN = 128 11.8 / 11.3; 1000 x 4096 x 4096
+// as above; 1 more where outputs are stored one by one.  Measured / estimated: 512 x 4096 x 4096 BN = 128 11.8 / 11.3; 1000 x 4096 x 4096
 // 256 16.3 / 15.3; 192 x 4096 x 11008 160 14.4 / 14.3; 256 x 8192 x 28672 224 54 / 55; 2048 x 4096 x 11008 256 58.9 / 57.4; 4096 x 128 x 28672 256
 // 82 / 93.
 PairPlan plan_pairs(int M, int N, int K, bool bulk, bool sectors, int sms) {
@@ -747,7 +772,7 @@ PairPlan plan_pairs(int M, int N, int K, bool bulk, bool sectors, int sms) {
     const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, rounds = (tiles + pairs - 1) / pairs;
     t.pairs = (int)std::min<int64_t>(pairs, tiles);
     const float copy = (float)rounds * std::max((float)k_steps * (0.1f + 0.0009f * (float)BN) * (sectors ? 1.0f : 1.4f), 0.8f + 0.0095f * (float)BN);
-    t.us = 3.8f + std::sqrt(copy * copy + call * call) + (bulk ? 0.0f : 2.0f);
+    t.us = 3.8f + std::sqrt(copy * copy + call * call) + (bulk ? 0.0f : 1.0f);
     if (best.BN == 0 || t.us < best.us) best = t;
   }
   return best;
@@ -797,7 +822,7 @@ std::string launch_rows_gemm(const GemmArgs& g, const RowsPlan& r, unsigned flag
   p.stage_bytes = r.stage_bytes;
   p.tmem_cols = 32;
   while ((int)p.tmem_cols < r.BM) p.tmem_cols *= 2;
-  p.pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
+  p.stores = reinterpret_cast<uintptr_t>(g.out) % 4 != 0 ? kSingle : g.ldo % 2 != 0 ? kAlternate : g.N % 2 == 0 ? kEven : kSingle;
   p.out = g.out; p.ldo = g.ldo;
   p.x_scales = g.x_scales; p.w_scales = g.w_scales; p.bias = g.bias;
   cudaError_t e = allow_smem<T>();

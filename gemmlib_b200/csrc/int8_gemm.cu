@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
     }
   } else if (warp == 1) {
     if (elect_one()) {
+      griddep_wait();  // or the limit of the waits below would count the kernel ahead
       const uint32_t idesc = make_idesc_i8(kTileN, p.BM);
       const uint64_t desc = tc::make_sw128_kmajor_desc(0);
       const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc;
@@ -521,6 +522,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
+      griddep_wait();  // or the limit of the waits below would count the kernel ahead
       const uint32_t idesc = make_idesc_i8(kPairM, p.BN);
       const uint64_t desc = tc::make_sw128_kmajor_desc(0);
       const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc | ((base >> 4) & 0x3FFFu);

@@ -122,6 +122,10 @@ class Int8Linear(nn.Module):
         self._settled = False
         return self
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._settled = False  # a copy's buffers are written on some stream too
+
     def _load_from_state_dict(self, *args, **kwargs):
         self._settled = False  # the buffers are about to be overwritten by a copy on some stream
         return super()._load_from_state_dict(*args, **kwargs)

@@ -42,6 +42,17 @@ def test_module_is_its_operators(k, dtype):
         same(layer.cpu().cuda()(x), want)
 
 
+def test_a_copy_waits_for_its_weights():
+    from gemmlib_b200.int8_linear import Int8Linear
+
+    layer, x = Int8Linear(normal(96, 512)), normal(2, 512, seed=2)
+    want = layer(x)
+    assert layer._settled
+    other = copy.deepcopy(layer)
+    assert not other._settled
+    same(other(x), want)
+
+
 def test_an_output_of_another_type_than_the_weights():
     from gemmlib_b200.int8_linear import Int8Linear, quantize_int8
 

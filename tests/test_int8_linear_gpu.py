@@ -114,6 +114,31 @@ def test_nothing_is_written_beside_an_output_in_a_wider_matrix(m, k, n, wider):
         assert (out[:, n:] == 9).all() and (out[m] == 9).all()
 
 
+@pytest.mark.parametrize("n", [32776, 32767])  # outputs by TMA, and one by one
+def test_offsets_beyond_32_bits(n):
+    from gemmlib_b200.int8_linear import Int8Rows, int8_linear
+
+    m, k = 70000, 48
+    wide = torch.randint(-128, 128, (m, 32768), dtype=torch.int8, device="cuda")
+    x = Int8Rows(wide[:, 32000:32000 + k], torch.rand(m, device="cuda") / 100)
+    w = rows_of(n, k, 2)
+    out = int8_linear(x, w)
+    assert m * 32768 > 2 ** 31 and out.numel() > 2 ** 31
+    for at in (0, m // 2, m - 300):
+        part = Int8Rows(x.values[at:at + 300], x.scales[at:at + 300])
+        check_close(out[at:at + 300], part, w)
+
+
+@pytest.mark.parametrize("m", [1, 4, 40])  # the weights beyond 2^31 bytes, by loads and by copies
+def test_weights_beyond_32_bits(m):
+    from gemmlib_b200.int8_linear import Int8Rows, int8_linear
+
+    n, k = 70000, 500
+    wide = torch.randint(-128, 128, (n, 32768), dtype=torch.int8, device="cuda")
+    x, w = rows_of(m, k, 1), Int8Rows(wide[:, 32000:32000 + k], torch.rand(n, device="cuda") / 100)
+    check_close(int8_linear(x, w, dtype=torch.bfloat16), x, w)
+
+
 def test_no_rows_and_nan_rows():
     from gemmlib_b200.int8_linear import Int8Rows, int8_linear, quantize_int8
 

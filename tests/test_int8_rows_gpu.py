@@ -326,6 +326,31 @@ def test_layouts_give_the_same_rows(layout, cols):
     assert torch.equal(x, before)
 
 
+@pytest.mark.parametrize("cols", [96, 2000, 9000])
+def test_offsets_beyond_32_bits(cols):
+    from gemmlib_b200.int8_linear import quantize_int8, rms_norm_int8, silu_mul_int8
+
+    rows, pitch, end = 70000, 32768, slice(70000 - 300, 70000)
+    wide = torch.empty(rows, pitch, dtype=torch.bfloat16, device="cuda").normal_()
+    a, b = wide[:, :cols], wide[:, pitch - cols:]
+    assert rows * pitch > 2 ** 31
+    w = normal(cols, dtype=torch.bfloat16, seed=1)
+    tail_a, tail_b = a[end].clone(), b[end].clone()
+
+    def check(got, want):
+        assert torch.equal(got.values[end], want.values) and torch.equal(got.scales[end], want.scales)
+
+    got = quantize_int8(a)
+    check(got, quantize_int8(tail_a))
+    assert torch.equal(got.dequantize(torch.bfloat16)[end], quantize_int8(tail_a).dequantize(torch.bfloat16))
+    check(silu_mul_int8(a, b), silu_mul_int8(tail_a, tail_b))
+    check(rms_norm_int8(b, w), rms_norm_int8(tail_b, w))
+    want, h = rms_norm_int8(tail_a, w, residual=tail_b)
+    got, total = rms_norm_int8(a, w, residual=b, residual_out=b)
+    check(got, want)
+    assert torch.equal(b[end], h) and total.data_ptr() == b.data_ptr()
+
+
 def test_nothing_is_written_outside_the_rows():
     """Through the C entry points, into buffers with guards between the rows and behind them."""
     from gemmlib_b200 import capi

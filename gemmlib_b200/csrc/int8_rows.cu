@@ -65,13 +65,30 @@ __device__ __forceinline__ void unpack8(const uint32_t (&r)[4], float (&v)[8]) {
   }
 }
 
+// What L2 does with inputs that have been read.  Large ones make room first, so that what is written stays: 11008 x 4096 quantized 21.3 ->
+// 18.7 us, 4095 x 8192 normed 25.7 -> 21.9.  Those that fit in L2 beside other things are kept, since they may be read again: 2048 x 4096 quantized
+// 4.4 us time after time, 5.0 if its rows have made room.  A gate and its factor, which are read for this alone, always make room (4096 x 5504 20.1 ->
+// 18.9 us); the inputs of a sum never do (4095 x 8192 36.4 us, 37.9 else).
+enum Fetch { kKept, kOnce, kInOrder };  // `kInOrder`: kept, and in the order of the program among loads of kOnce
+template <Fetch F>
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  if constexpr (F == kKept)
+    v = *reinterpret_cast<const uint4*>(p);
+  else if constexpr (F == kOnce)
+    asm volatile("ld.global.cs.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  else
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // VEC: every row begins on 16 bytes.  Zeros behind the end of the row.
-template <class T, bool VEC>
+template <class T, bool VEC, Fetch F = kKept>
 __device__ __forceinline__ void load8(const T* row, int chunk, int cols, uint32_t (&r)[4]) {
   const T* src = row + (int64_t)chunk * 8;
   const uint16_t* one = reinterpret_cast<const uint16_t*>(src);
   if (VEC && chunk * 8 + 8 <= cols) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
+    const uint4 u = load16<F>(src);
     r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
   } else if (!VEC && (reinterpret_cast<uintptr_t>(src) & 2u) == 0 && chunk * 8 + 8 <= cols) {
 #pragma unroll
@@ -263,24 +280,38 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One chunk from memory.  `again`: the second pass over a long row, whose sums are already in res_out (which may be x or the
-// residual itself).
+// A chunk's inputs.
+template <int OP, class T, bool VEC, bool ONCE>
+__device__ __forceinline__ void load_chunk(const RowsParams& p, int64_t row, int chunk, uint32_t (&a)[4], uint32_t (&b)[4],
+                                           uint32_t (&w)[4]) {
+  constexpr Fetch kInput = ONCE ? kOnce : kKept;
+  load8<T, VEC, kInput>(reinterpret_cast<const T*>(p.a) + row * p.lda, chunk, p.cols, a);
+  if constexpr (OP == kNormResidual || OP == kSiluMul)
+    load8<T, VEC, kInput>(reinterpret_cast<const T*>(p.b) + row * p.ldb, chunk, p.cols, b);
+  if constexpr (Sums<OP, T>::kSquares) load8<T, VEC, ONCE ? kInOrder : kKept>(reinterpret_cast<const T*>(p.w), chunk, p.cols, w);
+}
 template <int OP, class T, bool VEC>
+__device__ __forceinline__ void take_chunk(const RowsParams& p, int64_t row, int chunk, uint32_t (&a)[4], const uint32_t (&b)[4],
+                                           const uint32_t (&w)[4], Chunk<OP, T>& c, Sums<OP, T>& sums) {
+  if constexpr (OP == kNormResidual) {
+    add8<T>(a, b);
+    store8<T, VEC>(reinterpret_cast<T*>(p.res_out) + row * p.ldr, chunk, p.cols, a);
+  }
+  combine(c, sums, a, b, w);
+}
+// One chunk of a row that is read twice.  `again`: the second pass, for which the sums are already in res_out (which may be x or
+// the residual itself).
+template <int OP, class T, bool VEC, bool ONCE>
 __device__ __forceinline__ void chunk_of(const RowsParams& p, int64_t row, int chunk, bool again, Chunk<OP, T>& c, Sums<OP, T>& sums) {
   uint32_t a[4], b[4] = {}, w[4] = {};
   if (OP == kNormResidual && again) {
     load8<T, VEC>(reinterpret_cast<const T*>(p.res_out) + row * p.ldr, chunk, p.cols, a);
+    load8<T, VEC>(reinterpret_cast<const T*>(p.w), chunk, p.cols, w);
+    combine(c, sums, a, b, w);
   } else {
-    load8<T, VEC>(reinterpret_cast<const T*>(p.a) + row * p.lda, chunk, p.cols, a);
-    if constexpr (OP == kNormResidual || OP == kSiluMul)
-      load8<T, VEC>(reinterpret_cast<const T*>(p.b) + row * p.ldb, chunk, p.cols, b);
-    if constexpr (OP == kNormResidual) {
-      add8<T>(a, b);
-      store8<T, VEC>(reinterpret_cast<T*>(p.res_out) + row * p.ldr, chunk, p.cols, a);
-    }
+    load_chunk<OP, T, VEC, ONCE>(p, row, chunk, a, b, w);
+    take_chunk<OP, T, VEC>(p, row, chunk, a, b, w, c, sums);
   }
-  if constexpr (Sums<OP, T>::kSquares) load8<T, VEC>(reinterpret_cast<const T*>(p.w), chunk, p.cols, w);
-  combine(c, sums, a, b, w);
 }
 
 // How the chunks of a row are dealt out.
@@ -292,7 +323,7 @@ enum Deal {
 };
 
 // blockDim.x threads a CTA, NV chunks a thread.
-template <int OP, class T, bool VEC, int NV, int MAXT, Deal DEAL>
+template <int OP, class T, bool VEC, int NV, int MAXT, Deal DEAL, bool ONCE>
 __global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
   const int threads = DEAL == kWarp ? 32 : (int)blockDim.x, tid = DEAL == kWarp ? (int)threadIdx.x % 32 : (int)threadIdx.x;
   const int parts = DEAL == kCluster ? p.parts : 1, part = DEAL == kCluster ? (int)blockIdx.x % parts : 0;
@@ -307,14 +338,22 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
   Chunk<OP, T> c[NV];
   Sums<OP, T> sums;
   if constexpr (DEAL != kLoop) {
+    // (a part's last threads have chunks of the next part behind theirs: no chunk at all is what lies behind the row)
+    auto chunk = [&](int i) { return i * threads + tid < p.part_chunks ? first + i * threads : p.cols / 8 + 1; };
+    if constexpr (OP == kQuant) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      // (a part's last threads have chunks of the next part behind theirs: no chunk at all is what lies behind the row)
-      const int k = i * threads + tid < p.part_chunks ? first + i * threads : p.cols / 8 + 1;
-      chunk_of<OP, T, VEC>(p, row, k, false, c[i], sums);
+      for (int i = 0; i < NV; ++i) chunk_of<OP, T, VEC, ONCE>(p, row, chunk(i), false, c[i], sums);
+    } else {
+      // All loads first: none can move ahead of a store of sums, which may be in the place of an input.  4095 x 8192 with a residual 46.7 ->
+      // 36.4 us (6.5 TB/s), 16 x 8192 2.55 -> 2.05, silu_mul of 4096 x 5504 23.4 -> 20.1.
+      uint32_t a[NV][4], b[NV][4], w[NV][4];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load_chunk<OP, T, VEC, ONCE>(p, row, chunk(i), a[i], b[i], w[i]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) take_chunk<OP, T, VEC>(p, row, chunk(i), a[i], b[i], w[i], c[i], sums);
     }
   } else {
-    for (int k = tid; k * 8 < p.cols; k += threads) chunk_of<OP, T, VEC>(p, row, k, false, c[0], sums);
+    for (int k = tid; k * 8 < p.cols; k += threads) chunk_of<OP, T, VEC, ONCE>(p, row, k, false, c[0], sums);
   }
   uint32_t top = __reduce_max_sync(0xffffffffu, sums.top_bits());
   float squares = kSquares ? warp_sum(sums.squares) : 0.0f;
@@ -351,7 +390,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowsParams p) {
       if (i * threads + tid < p.part_chunks) write8(scale, q, p.q_vec, first + i * threads, p.cols, c[i]);
   } else {
     for (int k = tid; k * 8 < p.cols; k += threads) {
-      chunk_of<OP, T, VEC>(p, row, k, true, c[0], sums);
+      chunk_of<OP, T, VEC, ONCE>(p, row, k, true, c[0], sums);
       write8(scale, q, p.q_vec, k, p.cols, c[0]);
     }
   }
@@ -374,7 +413,11 @@ std::string launch_instance(RowsParams p, int parts, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = DEAL == kCluster ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, rows_kernel<OP, T, VEC, NV, MAXT, DEAL>, p);
+  // see load16; a long row's second pass wants it kept
+  constexpr bool kCanKeep = OP != kSiluMul || DEAL == kLoop, kCanDrop = VEC && OP != kNormResidual && DEAL != kLoop;
+  const bool once = kCanDrop && (!kCanKeep || (int64_t)p.rows * p.cols * 2 > (32 << 20));
+  cudaError_t e = once ? cudaLaunchKernelEx(&cfg, rows_kernel<OP, T, VEC, NV, MAXT, DEAL, kCanDrop>, p)
+                       : cudaLaunchKernelEx(&cfg, rows_kernel<OP, T, VEC, NV, MAXT, DEAL, kCanDrop && !kCanKeep>, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
 }

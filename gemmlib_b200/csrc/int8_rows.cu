@@ -423,9 +423,9 @@ std::string launch_instance(RowsParams p, int parts, cudaStream_t stream) {
 }
 
 // ---- many wide rows ----
-// A row of more than 8192 columns leaves an SM with one or two CTAs, and none of them loads while it waits at its barrier.  So
-// there persistent CTAs have a producer warp that keeps bulk copies of the next rows under way into a ring in shared memory, while
-// the other warps reduce and write the present one.  A stage holds the chunks of one step of all threads, of both inputs; copies
+// A row of more than 20480 columns leaves an SM with one CTA, which loads nothing while it waits at its barrier; rows that do not begin
+// on 16 bytes take several loads where others take one.  So there persistent CTAs have a producer warp that keeps bulk copies of the
+// next rows under way into a ring in shared memory, while the other warps reduce and write the present one.  A stage holds the chunks of one step of all threads, of both inputs; copies
 // begin and end on 16 bytes, whatever the row's place, and the threads shift what they read.  The elements of a row are dealt to
 // threads and summed in the order of rows_kernel.
 constexpr long long kWaitCycles = 4000000000ll;  // ~2 s
@@ -635,7 +635,10 @@ std::string launch_by_width(const RowsParams& p, cudaStream_t stream) {
     if constexpr (OP == kQuant || OP == kNorm) return launch_instance<OP, T, VEC, 4, 256, kCta>(p, 1, stream);
     else return launch_instance<OP, T, VEC, 2, 512, kCta>(p, 1, stream);
   }
-  if (p.cols <= 31744 && p.rows > 4 * sm_count()) return launch_stream<OP, T, 4, 1024>(p, stream);
+  // Measured, us, the stream / a CTA a row: quantize 4096 x 11008 31.1 / 23.7, 4096 x 20480 56.4 / 47.6, 4096 x 22528 56.9 / 70.0; silu_mul 4096 x 11008
+  // 49.6 / 38.0, 4096 x 18432 87 / 67, 4096 x 22528 95 / 112; with a residual 4096 x 16384 97 / 72, 4096 x 20480 113 / 101 (with up to 640 threads a second CTA
+  // fits on the SM).  Rows that begin anywhere: 4096 x 9001 30.3 / 32.7, silu_mul 2000 x 20001 51.5 / 84.5.
+  if (p.cols <= 31744 && p.rows > 4 * sm_count() && !(VEC && p.cols <= 20480)) return launch_stream<OP, T, 4, 1024>(p, stream);
   if (p.cols <= 32768) return launch_instance<OP, T, VEC, 4, 1024, kCta>(p, 1, stream);
   const int parts = (p.cols + 8191) / 8192;
   if (parts <= kMaxParts && (int64_t)p.rows * parts <= INT32_MAX) return launch_instance<OP, T, VEC, 2, 512, kCluster>(p, parts, stream);

@@ -260,6 +260,10 @@ __host__ __device__ constexpr SmemPlan make_plan(int rows, int kStages, int act_
   p.total = o + 1024;  // slack to align the dynamic base to 1024
   return p;
 }
+template <class S>
+constexpr bool keeps_tensor_memory() { return make_plan(S::MAXM, S::WS, S::RING, S::KSUB).total >= kSmemOfManyColumns; }
+static_assert(keeps_tensor_memory<ShapeSmall>() && keeps_tensor_memory<ShapeSmallLong>() && keeps_tensor_memory<ShapeMid>() &&
+              keeps_tensor_memory<ShapeLarge>());
 
 // Barrier slots (8 bytes each) inside the barrier block.  A "step full" barrier collects what the MMAs of a step
 // read: the bytes of its activation tile and the arrivals of its dequantizer warps.  An "MMA done" barrier frees the

@@ -168,6 +168,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_act, const __grid_con
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   constexpr SmemPlan plan = make_plan(kPairRows, kStages, kActStages, 1, kPairOutBytes);
+  static_assert(plan.total >= kSmemOfManyColumns);
   constexpr uint32_t act_stride = kPairRows * 128;
   const uint32_t bars = base + plan.bars;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + plan.bars + BAR_COUNT * 8);

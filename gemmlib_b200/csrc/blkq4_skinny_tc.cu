@@ -60,6 +60,7 @@ static_assert(kMaxSplit * TILE_N * 16 <= kRing * kActBytes, "the exchange of a s
 
 constexpr uint32_t kActOff = 0, kPackOff = kActOff + kRing * kActBytes, kScaleOff = kPackOff + kStages * kPackBytes,
                    kZpOff = kScaleOff + kStages * kScaleBytes, kBarOff = kZpOff + kStages * kZpBytes, kSmemBytes = kBarOff + 512 + 1024;
+static_assert(kSmemBytes >= kSmemOfManyColumns);
 
 enum : int {
   kFull = 0,                       // [kStages] packed weights and meta landed

@@ -18,6 +18,15 @@ constexpr int kPackTileBytes = (TILE_N / 2) * BLOCK_K;  // 4 KB: 64 packed colum
 constexpr int kScaleTileBytes = 1024;
 constexpr int kZpTileBytes = 512;
 
+// Tensor memory has 512 columns an SM, and tcgen05.alloc waits, without a limit, until a CTA beside it frees what it lacks.  Two
+// kernels of different streams may stand so: a CTA of each holds columns on an SM where the other's waits for them, and each
+// waits at a barrier of its cluster for its own one that cannot get them: for good.  So CTAs whose columns do not fit together must
+// not fit together in shared memory (228 KB an SM, 1 KB of each CTA the system's): one of more than 128 columns asks for at least
+// kSmemOfManyColumns, any other for kSmemOfFewColumns, of which two share an SM and a third does not fit.
+constexpr uint32_t kSmemOfManyColumns = 130u * 1024, kSmemOfFewColumns = 97u * 1024;
+static_assert(kSmemOfManyColumns + kSmemOfFewColumns + 2 * 1024 > 228 * 1024 && 2 * (kSmemOfManyColumns + 1024) > 228 * 1024 &&
+              2 * (kSmemOfFewColumns + 1024) <= 228 * 1024 && 3 * (kSmemOfFewColumns + 1024) > 228 * 1024);
+
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }

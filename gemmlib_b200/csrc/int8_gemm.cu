@@ -370,7 +370,7 @@ constexpr uint32_t kPairChunkBytes = 32u * 64u;               // 32 rows x 32 ou
 constexpr uint32_t kPairOutBytes = kEpiWarps * kPairChunkBytes;
 constexpr uint32_t kPairScaleBytes = 2u * 2u * kPairMaxN * 4u;  // scales and biases of two tiles' columns
 constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + kPairOutBytes + kPairScaleBytes + 512 + 1024;
-static_assert(kPairSmem <= 227 * 1024);
+static_assert(kPairSmem <= 227 * 1024 && kPairSmem >= tc::kSmemOfManyColumns);
 
 struct PairParams {
   int M, N;
@@ -749,7 +749,8 @@ RowsPlan plan_rows(int M, int N, int K, bool sectors, int sms) {
       t.slice = split > 1 ? ((rows + split - 1) / split + 7) / 8 * 8 : BM;
       t.exchange_bytes = (uint32_t)(split - 1) * (uint32_t)t.slice * kTileN * 4;
       t.stages = std::min<int>(kMaxStages, (int)(((per_sm == 2 ? kSmemOfTwo : kSmemAlone) - t.exchange_bytes) / stage_bytes));
-      t.smem = (uint32_t)t.stages * stage_bytes + t.exchange_bytes + kBarBytes + 1024;
+      t.smem = std::max((uint32_t)t.stages * stage_bytes + t.exchange_bytes + kBarBytes + 1024,
+                        BM <= 128 ? tc::kSmemOfFewColumns : tc::kSmemOfManyColumns);
       if (t.stages >= 3 && (best.BM == 0 || us < best.us)) best = t;
     }
   }

@@ -9,6 +9,7 @@
 
 #include <atomic>
 #include <memory>
+#include <mutex>
 
 namespace blkq4 {
 
@@ -74,15 +75,20 @@ inline bool encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, int e
 }
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize is per device and sticky: raise it only when a launch
-// needs more than an earlier one asked for.  `granted` is one table per kernel instance.
+// needs more than an earlier one asked for.  `granted` is one table per kernel instance.  A call that raises it keeps others out and
+// looks again first: the attribute is replaced by what a call sets, so that two at once could leave it at the smaller amount.
 template <typename Kernel>
 inline cudaError_t ensure_dynamic_smem(Kernel kern, size_t bytes, std::atomic<int> (&granted)[64]) {
+  static std::mutex raising;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 0 && dev < 64 && granted[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && granted[dev].load(std::memory_order_acquire) >= (int)bytes) return cudaSuccess;
+  std::lock_guard<std::mutex> lock(raising);
+  if (known && granted[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess && dev >= 0 && dev < 64) granted[dev].store((int)bytes, std::memory_order_relaxed);
+  if (e == cudaSuccess && known) granted[dev].store((int)bytes, std::memory_order_release);
   return e;
 }
 

@@ -137,6 +137,10 @@ Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor
   const int dtype = type_of("rms_norm_int8: the input", x.scalar_type());
   no_backward(x);
   no_backward(weight);
+  if (residual) {
+    no_backward(*residual);
+    if (residual_out->defined()) no_backward(*residual_out);
+  }
   const Rows a = as_rows("rms_norm_int8: the input", x, true);
   TORCH_CHECK(weight.scalar_type() == x.scalar_type() && weight.dim() == 1 && weight.size(0) == a.cols,
               "rms_norm_int8: the weight must be one row of the input's length and type");
@@ -145,7 +149,6 @@ Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor
   const Tensor w = weight.contiguous();
   Rows r, s;
   if (residual) {
-    no_backward(*residual);
     TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes(),
                 "rms_norm_int8: the residual must have the input's shape and type");
     same_device("rms_norm_int8: the residual", *residual, x);
@@ -204,6 +207,7 @@ Tensor check_scales(const char* name, const Tensor& scales, const Tensor& values
 Tensor dequantize(const Tensor& values, const Tensor& scales, torch::ScalarType type) {
   const int dtype = type_of("int8_dequantize: the output's type", type);
   TORCH_CHECK(values.scalar_type() == torch::kChar, "int8_dequantize: the values must be int8");
+  no_backward(scales);
   const Rows v = as_rows("int8_dequantize: the values", values, true);
   const c10::cuda::CUDAGuard guard(values.device());
   const Tensor s = check_scales("int8_dequantize: scales", scales, values, v.rows);
@@ -224,6 +228,10 @@ Tensor linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Te
               torch::ScalarType type, int64_t flags, const Tensor* brought) {
   const int dtype = type_of("int8_linear: the output's type", type);
   TORCH_CHECK(x.scalar_type() == torch::kChar && w.scalar_type() == torch::kChar, "int8_linear: input and weight must be int8 rows");
+  no_backward(x_scales);
+  no_backward(w_scales);
+  if (bias) no_backward(*bias);
+  if (brought) no_backward(*brought);
   Rows a = as_rows("int8_linear: the input", x, true);
   TORCH_CHECK(w.dim() == 2, "int8_linear: the weight must be [out_features, in_features]");
   const Rows b = as_rows("int8_linear: the weight", w, false);
@@ -240,7 +248,6 @@ Tensor linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Te
   const Tensor xs = check_scales("int8_linear: the input's scales", x_scales, x, a.rows);
   const Tensor ws = check_scales("int8_linear: the weight's scales", w_scales, x, b.rows);
   if (bias) {
-    no_backward(*bias);
     TORCH_CHECK(bias->scalar_type() == type && bias->dim() == 1 && bias->size(0) == b.rows && bias->is_contiguous(),
                 "int8_linear: the bias must be a contiguous [out_features] tensor of the output's type");
     same_device("int8_linear: the bias", *bias, x);

@@ -7,8 +7,8 @@ Where a product is bound by the tensor cores - prompts, large batches - 8-bit op
 
 Rows: any leading dimensions, the last one is a row.  Rows of one pitch (slices of a wider tensor among them) are read
 in place, other layouts are copied first.  Work is enqueued on the current stream of the tensors' device.  A row with an infinity
-or NaN gets the scale NaN, and is NaN in every output.  There is no backward pass: an input that requires one is refused
-while gradients are enabled.
+or NaN gets the scale NaN, and is NaN in every output.  There is no backward pass: a tensor of a call (inputs,
+scales, weights, bias, what is written) that requires one is refused while gradients are enabled.
 """
 from __future__ import annotations
 
@@ -101,7 +101,7 @@ class Int8Linear(nn.Module):
         pad = -self.in_features % 32
         # kept with whole rows of 32 bytes, so that copies of the buffer have them too
         self.register_buffer("q_weights", nn.functional.pad(rows.values, (0, pad)) if pad else rows.values)
-        self.register_buffer("q_scales", rows.scales.clone())  # (the operators' rows and scales share their memory)
+        self.register_buffer("q_scales", rows.scales.detach().clone())  # (the operators' rows and scales share their memory)
         self.bias = bias_tensor
         self.early_weight_fetch = True
         self._settled = False  # the first forward is a plain launch

@@ -71,6 +71,8 @@ int type_of(const char* name, torch::ScalarType t) {
 void no_backward(const Tensor& x) {
   TORCH_CHECK(!x.requires_grad() || !at::GradMode::is_enabled(),
               "The int8 operators have no backward pass: call them under torch.no_grad(), or detach the tensor");
+  TORCH_CHECK(!x._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+              "The int8 operators have no forward derivatives: take the primal of the dual tensor");
 }
 
 // int8 rows in the shape of `x`, every row beginning on 32 bytes (what the product copies fastest), and their scales.

@@ -8,7 +8,8 @@ Where a product is bound by the tensor cores - prompts, large batches - 8-bit op
 Rows: any leading dimensions, the last one is a row.  Rows of one pitch (slices of a wider tensor among them) are read
 in place, other layouts are copied first.  Work is enqueued on the current stream of the tensors' device.  A row with an infinity
 or NaN gets the scale NaN, and is NaN in every output.  There is no backward pass: a tensor of a call (inputs,
-scales, weights, bias, what is written) that requires one is refused while gradients are enabled.
+scales, weights, bias, what is written) that requires one is refused while gradients are enabled, and so is one with a
+forward-mode tangent.
 """
 from __future__ import annotations
 

@@ -1,5 +1,5 @@
-"""The int8 operators have no backward pass: every tensor of a call that requires a gradient is refused while gradients are enabled,
-before anything else is asked of it (so that no GPU is needed to see it)."""
+"""The int8 operators have no derivatives: a tensor of a call that requires a gradient (while gradients are enabled) or has a
+tangent is refused, before anything else is asked of it (so that no GPU is needed to see it)."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -61,3 +61,19 @@ def test_a_layer_of_given_rows_takes_their_scales_without_history():
 
     layer = Int8Linear.from_rows(rows(torch.ones(2, requires_grad=True) * 2))
     assert not layer.q_scales.requires_grad and layer.q_scales.tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_tensor_with_a_tangent_is_refused(name):
+    """Forward-mode derivatives, which no_grad does not turn off."""
+    from torch.autograd import forward_ad
+
+    tensor, call = calls()[name]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(tensor, torch.ones_like(tensor))
+        with pytest.raises(RuntimeError, match="no forward derivatives"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no forward derivatives"):
+            call(dual)
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            call(forward_ad.unpack_dual(dual).primal)

@@ -6,6 +6,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -73,6 +74,12 @@ void no_backward(const Tensor& x) {
               "The int8 operators have no backward pass: call them under torch.no_grad(), or detach the tensor");
   TORCH_CHECK(!x._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
               "The int8 operators have no forward derivatives: take the primal of the dual tensor");
+}
+
+// A caller's tensor is about to be written: what autograd has saved of it, or of a view, is not what it was.  (Tensors made under
+// inference mode have no versions.)
+void written(const Tensor& x) {
+  if (!x.is_inference()) torch::autograd::impl::bump_version(x);
 }
 
 // int8 rows in the shape of `x`, every row beginning on 32 bytes (what the product copies fastest), and their scales.
@@ -150,12 +157,13 @@ Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor w = weight.contiguous();
   Rows r, s;
+  const bool brought = residual && residual_out->defined();
   if (residual) {
     TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes(),
                 "rms_norm_int8: the residual must have the input's shape and type");
     same_device("rms_norm_int8: the residual", *residual, x);
     r = as_rows("rms_norm_int8: the residual", *residual, true);
-    if (residual_out->defined()) {
+    if (brought) {
       TORCH_CHECK(residual_out->scalar_type() == x.scalar_type() && residual_out->sizes() == x.sizes(),
                   "rms_norm_int8: residual_out must have the input's shape and type");
       same_device("rms_norm_int8: residual_out", *residual_out, x);
@@ -171,6 +179,7 @@ Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor
   }
   Int8Out o = int8_like(x);
   if (a.rows == 0) return o;
+  if (brought) written(*residual_out);
   std::string err;
   TORCH_CHECK(int8_rows_rms_norm_sm100(dtype, a.rows, a.cols, current_stream(), a.data, a.bytes, a.ld, r.data, r.bytes, r.ld,
                                        w.data_ptr(), w.nbytes(), float(eps), s.data, s.bytes, s.ld, o.values.data_ptr(),
@@ -267,6 +276,7 @@ Tensor linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Te
   }
   if (a.rows == 0) return out;
   const Rows o = as_rows("int8_linear: out", out, false);
+  if (brought) written(out);
   std::string err;
   TORCH_CHECK(int8_gemm_sm100(dtype, a.rows, b.rows, a.cols, current_stream(), a.data, a.bytes, a.ld, xs.data_ptr(), xs.nbytes(),
                               b.data, b.bytes, b.ld, ws.data_ptr(), ws.nbytes(), bias ? bias->data_ptr() : nullptr,

@@ -142,6 +142,34 @@ bool apart_or_same(const Rows& a, const Rows& b) {
   return d >= a.cols && d + a.cols <= a.ld;
 }
 
+// Whether no byte of `a` is one of `b`, whatever their types: column ranges of one wider matrix are apart, for instance.
+bool apart(const Rows& a, const Rows& b) {
+  const char *pa = static_cast<const char*>(a.data), *pb = static_cast<const char*>(b.data);
+  if (a.bytes == 0 || b.bytes == 0 || pa + a.bytes <= pb || pb + b.bytes <= pa) return true;
+  const Rows &few = a.rows <= b.rows ? a : b, &many = a.rows <= b.rows ? b : a;
+  const int64_t few_elt = few.held.element_size(), elt = many.held.element_size();
+  const int64_t pitch = many.rows > 1 ? many.ld * elt : 1, length = many.cols * elt;
+  for (int64_t i = 0; i < few.rows; ++i) {  // the last row of `many` that begins before this one's end
+    const int64_t begin = static_cast<const char*>(few.data) + i * few.ld * few_elt - static_cast<const char*>(many.data);
+    const int64_t end = begin + few.cols * few_elt;
+    if (end <= 0) continue;
+    const int64_t row = std::min<int64_t>((end - 1) / pitch, many.rows - 1);
+    if (row * pitch + length > begin) return false;
+  }
+  return true;
+}
+// A vector as one row.
+Rows as_row(const Tensor& v) {
+  Rows r;
+  r.held = v;
+  r.data = v.data_ptr();
+  r.rows = 1;
+  r.cols = int(v.numel());
+  r.ld = r.cols;
+  r.bytes = v.nbytes();
+  return r;
+}
+
 Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor* residual, Tensor* residual_out) {
   const int dtype = type_of("rms_norm_int8: the input", x.scalar_type());
   no_backward(x);
@@ -170,8 +198,7 @@ Int8Out rms_norm(const Tensor& x, const Tensor& weight, double eps, const Tensor
       s = as_rows("rms_norm_int8: residual_out", *residual_out, false);
       TORCH_CHECK(apart_or_same(s, a) && apart_or_same(s, r),
                   "rms_norm_int8: residual_out may be the input or the residual, but not overlap them otherwise");
-      const char *ws = static_cast<const char*>(w.data_ptr()), *ss = static_cast<const char*>(s.data);
-      TORCH_CHECK(s.bytes == 0 || ws + w.nbytes() <= ss || ss + s.bytes <= ws, "rms_norm_int8: residual_out overlaps the weight");
+      TORCH_CHECK(apart(s, as_row(w)), "rms_norm_int8: residual_out overlaps the weight");
     } else {
       *residual_out = at::empty(x.sizes(), x.options());
       s = as_rows("rms_norm_int8: residual_out", *residual_out, false);
@@ -276,7 +303,11 @@ Tensor linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Te
   }
   if (a.rows == 0) return out;
   const Rows o = as_rows("int8_linear: out", out, false);
-  if (brought) written(out);
+  if (brought) {
+    TORCH_CHECK(apart(o, a) && apart(o, b) && apart(o, as_row(xs)) && apart(o, as_row(ws)) && (!bias || apart(o, as_row(*bias))),
+                "int8_linear: out overlaps a tensor that the product reads");
+    written(out);
+  }
   std::string err;
   TORCH_CHECK(int8_gemm_sm100(dtype, a.rows, b.rows, a.cols, current_stream(), a.data, a.bytes, a.ld, xs.data_ptr(), xs.nbytes(),
                               b.data, b.bytes, b.ld, ws.data_ptr(), ws.nbytes(), bias ? bias->data_ptr() : nullptr,

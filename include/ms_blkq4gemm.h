@@ -383,7 +383,7 @@ int int8_rows_dequant_sm100(
  * out[m, n] = x_scales[m] * w_scales[n] * sum over k of x[m, k] w[n, k] (+ bias[n]), for any m, n and k up to 131071.  The sums
  * are exact (int32); scales and bias are applied in fp32 and the result is rounded to the 16-bit type once.  bias: [n] of that
  * type, or null.  x and w: 16-byte aligned, ldx and ldw multiples of 16
- * (of 32: up to a quarter faster).
+ * (of 32: up to a quarter faster).  out may not overlap what the call reads.
  * BLKQ4_GEMM_EARLY_WEIGHT_FETCH: the caller vouches that w (not w_scales or bias) is not written by any work still pending on
  * `stream`; its first tiles are then fetched while the preceding kernel still runs.
  */

@@ -94,14 +94,17 @@ class Int8Linear(nn.Module):
             rows = quantize_int8(weights)
         self._set(rows, bias_tensor, weights.dtype)
 
-    def _set(self, rows: Int8Rows, bias_tensor, dtype):
+    def _set(self, rows: Int8Rows, bias_tensor, dtype, copy=False):
         if rows.values.dim() != 2:
             raise ValueError("weights must be [out_features, in_features]")
         self.out_features, self.in_features = rows.values.shape
         self.dtype = dtype
-        pad = -self.in_features % 32
-        # kept with whole rows of 32 bytes, so that copies of the buffer have them too
-        self.register_buffer("q_weights", nn.functional.pad(rows.values, (0, pad)) if pad else rows.values)
+        pad, values = -self.in_features % 32, rows.values
+        if pad:  # kept with whole rows of 32 bytes, so that copies of the buffer have them too
+            values = nn.functional.pad(values, (0, pad))
+        elif copy:
+            values = values.clone(memory_format=torch.contiguous_format)
+        self.register_buffer("q_weights", values)
         self.register_buffer("q_scales", rows.scales.detach().clone())  # (the operators' rows and scales share their memory)
         self.bias = bias_tensor
         self.early_weight_fetch = True
@@ -109,10 +112,10 @@ class Int8Linear(nn.Module):
 
     @classmethod
     def from_rows(cls, weight: Int8Rows, bias_tensor: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16):
-        """A layer of weights that are int8 rows already, [out_features, in_features]."""
+        """A layer of weights that are int8 rows already, [out_features, in_features], of any layout: it keeps a copy."""
         self = cls.__new__(cls)
         nn.Module.__init__(self)
-        self._set(Int8Rows(*weight), bias_tensor, dtype)
+        self._set(Int8Rows(*weight), bias_tensor, dtype, copy=True)
         return self
 
     def _apply(self, fn, recurse=True):

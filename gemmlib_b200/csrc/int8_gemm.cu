@@ -86,11 +86,14 @@ __device__ __forceinline__ void umma_i8_x4(uint32_t d_tmem, uint32_t a_lo, uint3
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
+// Eight columns, there when it returns: load and wait are one statement, so that no use of the registers can come between them.
+__device__ __forceinline__ void tmem_ld_32x32b_x8_now(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
 }
 // 16 bytes to another CTA of the cluster, which complete on a barrier there.
 __device__ __forceinline__ void st_async_v4(uint32_t dst, uint32_t bar, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -276,8 +279,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
       while (m >= (o + 1) * p.slice) ++o;
       if (o == part) continue;
       uint32_t r[8];
-      tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
-      tc::tmem_ld_wait();
+      tmem_ld_32x32b_x8_now(tmem_row + (uint32_t)m, r);
       const uint32_t at = (uint32_t)(part - (part > o)) * part_words + (uint32_t)((m - o * p.slice) * kTileN + n_l * 4);
       const uint32_t dst = tc::map_to_cta(base + exchange_at + at * 4u, (uint32_t)o), bar = tc::map_to_cta(exchanged, (uint32_t)o);
       st_async_v4(dst, bar, r[0], r[1], r[2], r[3]);
@@ -295,8 +297,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
     const int odd = lane & 1;
     for (int m = first + turn * 8; m < end; m += 16) {
       uint32_t r[8];
-      tmem_ld_32x32b_x8(tmem_row + (uint32_t)m, r);
-      tc::tmem_ld_wait();
+      tmem_ld_32x32b_x8_now(tmem_row + (uint32_t)m, r);
       for (int q = 0; q < p.split - 1; ++q) {
         const uint32_t* at = parts + q * part_words + (m - first) * kTileN;
 #pragma unroll

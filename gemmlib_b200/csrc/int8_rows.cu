@@ -169,6 +169,11 @@ struct Sums {
       for (int e = 0; e < 8; e += 2) top = max_abs(top, c.t[e], c.t[e + 1]);
     }
   }
+  // As if a t had been NaN.
+  __device__ __forceinline__ void spoil() {
+    if constexpr (OP == kQuant) top2 = 0x7fff7fffu;
+    else top = __uint_as_float(0x7fffffffu);
+  }
   // Bits of max|t|: their order as integers puts infinities and NaN last.
   __device__ __forceinline__ uint32_t top_bits() const {
     if constexpr (OP == kQuant) {
@@ -553,16 +558,18 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
     }
   };
   int buffer = 0;
+  // 0 once a wait has given up: the rows that are left are NaN as a whole, like one with a NaN among its inputs, and no sums are stored
+  // (later waits may pass on the phase before, with nothing new behind them).
+  int stored = p.cols;
   for (int64_t row = blockIdx.x; row < p.rows; row += sp.grid, buffer ^= 1) {
     Chunk<OP, T> c[NV];
     Sums<OP, T> sums;
-    bool ok = true;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int chunk = i * threads + tid;
       uint32_t a[4] = {}, b[4] = {}, w[4] = {};
       if (i < pieces) {
-        if (!mbar_wait_bounded(smem_u32(&full[s]), parity, &abort_flag, &g_rows_error, 0x200 | s, kWaitCycles)) ok = false;
+        if (!mbar_wait_bounded(smem_u32(&full[s]), parity, &abort_flag, &g_rows_error, 0x200 | s, kWaitCycles)) stored = 0;
         const uint8_t* piece = ring + s * stage_bytes;
         from_stage(piece, p.a, p.lda, row, chunk, a);
         if constexpr (kTwo) from_stage(piece + sp.piece_bytes, p.b, p.ldb, row, chunk, b);
@@ -571,12 +578,13 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
         advance();
         if constexpr (OP == kNormResidual) {
           add8<T>(a, b);
-          store8<T, false>(reinterpret_cast<T*>(p.res_out) + row * p.ldr, chunk, p.cols, a);
+          store8<T, false>(reinterpret_cast<T*>(p.res_out) + row * p.ldr, chunk, stored, a);
         }
         if constexpr (kSquares) load8<T, false>(reinterpret_cast<const T*>(p.w), chunk, p.cols, w);
       }
       combine(c[i], sums, a, b, w);
     }
+    if (stored == 0) sums.spoil();
     uint32_t top = __reduce_max_sync(0xffffffffu, sums.top_bits());
     float squares = kSquares ? warp_sum(sums.squares) : 0.0f;
     if (lane == 0) {
@@ -589,7 +597,6 @@ __global__ void __launch_bounds__(MAXT) rows_stream_kernel(const RowsParams p, c
     if constexpr (kSquares) squares = warp_sum(lane < warps ? all[buffer][lane] : 0.0f);
     if (tid == 0) write_scale<kSquares>(p, row, top, squares);
     const Scale scale = scale_of(top);
-    if (!ok) continue;
     int8_t* q = p.q + row * p.ldq;
 #pragma unroll
     for (int i = 0; i < NV; ++i) write8(scale, q, p.q_vec, i * threads + tid, p.cols, c[i]);

@@ -29,16 +29,21 @@ _linear = ms_blkq4linear_ext.int8_linear
 
 
 class Int8Rows(NamedTuple):
-    """Rows of int8 and a float32 scale for each: row r stands for ``scales[r] * values[r]``."""
+    """Rows of int8 and a float32 scale for each: row r stands for ``scales[r] * values[r]``.  (The operators' rows and scales share
+    an allocation; what is pickled, saved or copied as ``Int8Rows`` has one of its own for each.)"""
 
     values: torch.Tensor
     scales: torch.Tensor
+
+    def __reduce__(self):  # tensors of two types in one storage cannot be saved
+        return Int8Rows, (self.values, self.scales.clone())
 
     def dequantize(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
         return _dequantize(self.values, self.scales, dtype)
 
 
 ms_blkq4linear_ext.int8_rows_type(Int8Rows)  # what the extension's functions return
+torch.serialization.add_safe_globals([Int8Rows])  # two tensors: torch.load takes them with weights_only, its default
 
 
 def quantize_int8(x: torch.Tensor) -> Int8Rows:

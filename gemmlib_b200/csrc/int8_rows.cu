@@ -252,9 +252,14 @@ template <bool SQUARES>
 __device__ __forceinline__ void write_scale(const RowsParams& p, int64_t row, uint32_t top, float squares) {
   const float amax = __uint_as_float(top);
   float scale = __fdiv_rn(amax, 127.0f);
-  if (SQUARES && top > 0) scale *= __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, (float)p.cols) + p.eps));
-  // (squares of which the sum is no float: 1 / sqrt would be 0)
-  p.scales[row] = top < 0x7f800000u && (!SQUARES || squares < INFINITY) ? scale : __uint_as_float(0x7fc00000u);
+  bool known = top < 0x7f800000u;
+  if (SQUARES) {
+    // A mean of squares that is no normal float has lost bits that 1 / sqrt needs, or all of them; one that is infinite would make it 0.
+    const float mean = __fdiv_rn(squares, (float)p.cols) + p.eps;
+    known = known && squares < INFINITY && (top == 0 || mean >= 0x1p-126f);
+    if (top > 0) scale *= __fdiv_rn(1.0f, __fsqrt_rn(mean));
+  }
+  p.scales[row] = known ? scale : __uint_as_float(0x7fc00000u);
 }
 template <int OP, class T>
 __device__ __forceinline__ void write8(const Scale& s, int8_t* q, bool vec, int chunk, int cols, const Chunk<OP, T>& c) {

@@ -329,7 +329,8 @@ int blkq4_gather_destroy(void* ctx);
  *   - A row stands for scale * values.  scale = max|t| / 127 and values[k] = round(t[k] * (127 / max|t|)), half to even, where t
  *     is the row to be quantized in fp32.  A row of zeros has scale 0.  A row with an infinity or NaN among its inputs or its t
  *     (a sum with the residual that overflows the 16-bit type, a product that overflows fp32) has scale NaN, so that whatever
- *     reads it is NaN in that row only; so has a row whose sum of squares overflows fp32 (the norm of |x| beyond 1e17).
+ *     reads it is NaN in that row only; so has a row whose sum of squares overflows fp32 (the norm of |x| beyond 1e17), or whose mean square
+ *     plus eps is below the smallest normal float (of |x| below 1e-19, without an eps to speak of).
  *   - dtype: INT8_FP16 or INT8_BF16, the type of the 16-bit operands of the call.
  *   - ld*: elements from row to row (of an int8 matrix: bytes), at least the row's length.  *_size: bytes that may be
  *     accessed, at least those from the first to the last element.  Rows that all begin on 16 bytes (int8 ones of the first

@@ -412,7 +412,7 @@ std::string launch_instance(RowsParams p, int parts, cudaStream_t stream) {
   p.parts = parts;
   p.part_chunks = (chunks + parts - 1) / parts;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(DEAL == kWarp ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows * (unsigned)parts);
+  cfg.gridDim = dim3(DEAL == kWarp ? ((unsigned)p.rows + 3) / 4 : (unsigned)p.rows * (unsigned)parts);
   cfg.blockDim = dim3((unsigned)(DEAL == kWarp ? 128 : DEAL == kLoop ? MAXT : ((p.part_chunks + NV - 1) / NV + 31) / 32 * 32));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -746,7 +746,7 @@ std::string launch_dequant_typed(int rows, int cols, const int8_t* q, int64_t ld
   int lanes = 1;
   while (lanes < 256 && lanes * (vec ? 16 : 8) < cols) lanes *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows + 256 / lanes - 1) / (256 / lanes)));
+  cfg.gridDim = dim3(((unsigned)rows + 256 / lanes - 1) / (256 / lanes));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

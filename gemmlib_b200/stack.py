@@ -29,7 +29,7 @@ class LinearStack:
     """``steps`` = [(layer, input buffer name, output buffer name), ...] executed in order.
 
     Buffer ``"x"`` is the stack's input ([M, in_features of the first reader]); every other
-    name is created on first use as an output and can be read by later steps.
+    name is created on first use as an output and can be read by later steps.  All buffers are float16, those of bfloat16 weights' layers too.
 
     ``int8_inputs``: step -> what makes the int8 rows that this step's ``Int8Linear`` multiplies, from the buffers: a norm
     (which may write the residual's buffer), a gated activation.  Int8 steps without an entry quantize the buffer they read; those that follow

@@ -87,7 +87,8 @@ def build_ext(force: bool = False) -> str:
     build_lib()
     out = ext_path()
     sources = sorted(glob.glob(os.path.join(CSRC, "*_ext.cpp")))
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(_newest(sources), os.path.getmtime(LIB)):
+    headers = glob.glob(os.path.join(CSRC, "*.h"))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(_newest(sources + headers), os.path.getmtime(LIB)):
         return out
     import sysconfig
 
@@ -101,7 +102,7 @@ def build_ext(force: bool = False) -> str:
            "-I" + os.path.join(ROOT, "include"), "-I" + sysconfig.get_paths()["include"]]
     cmd += ["-isystem" + p for p in inc]
     objs = [os.path.join(OBJ, os.path.basename(src)[:-4] + ".o") for src in sources]
-    hdr_time = _newest(glob.glob(os.path.join(ROOT, "include", "*.h")) + [os.path.abspath(__file__)])
+    hdr_time = _newest(headers + glob.glob(os.path.join(ROOT, "include", "*.h")) + [os.path.abspath(__file__)])
 
     def run(c):
         r = subprocess.run(c, capture_output=True, text=True)

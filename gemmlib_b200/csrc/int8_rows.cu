@@ -25,6 +25,7 @@
 #include "blkq4_tc.cuh"
 #include "blkq4_tma.cuh"
 #include "int8.cuh"
+#include "rows_io.cuh"
 
 namespace blkq4 {
 namespace int8 {
@@ -34,109 +35,6 @@ __device__ int g_rows_error = 0;  // 0 ok; otherwise (role << 8) | stage of the 
 namespace {
 
 constexpr int kMaxParts = 8;  // CTAs a row
-
-template <class T>
-struct Pair;
-template <>
-struct Pair<__half> {
-  using type = __half2;
-};
-template <>
-struct Pair<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
-template <class T>
-__device__ __forceinline__ typename Pair<T>::type as_pair(uint32_t v) {
-  return *reinterpret_cast<typename Pair<T>::type*>(&v);
-}
-template <class P>
-__device__ __forceinline__ uint32_t as_word(P v) {
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// A chunk is 8 consecutive elements of a row, a thread's step, packed in four words.
-template <class T>
-__device__ __forceinline__ void unpack8(const uint32_t (&r)[4], float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack2(r[i], T());
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-
-// What L2 does with inputs that have been read.  Large ones make room first, so that what is written stays: 11008 x 4096 quantized 21.3 ->
-// 18.7 us, 4095 x 8192 normed 25.7 -> 21.9.  Those that fit in L2 beside other things are kept, since they may be read again: 2048 x 4096 quantized
-// 4.4 us time after time, 5.0 if its rows have made room.  A gate and its factor, which are read for this alone, always make room (4096 x 5504 20.1 ->
-// 18.9 us); the inputs of a sum never do (4095 x 8192 36.4 us, 37.9 else).
-enum Fetch { kKept, kOnce, kInOrder };  // `kInOrder`: kept, and in the order of the program among loads of kOnce
-template <Fetch F>
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  if constexpr (F == kKept)
-    v = *reinterpret_cast<const uint4*>(p);
-  else if constexpr (F == kOnce)
-    asm volatile("ld.global.cs.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  else
-    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-
-// VEC: every row begins on 16 bytes.  Zeros behind the end of the row.
-template <class T, bool VEC, Fetch F = kKept>
-__device__ __forceinline__ void load8(const T* row, int chunk, int cols, uint32_t (&r)[4]) {
-  const T* src = row + (int64_t)chunk * 8;
-  const uint16_t* one = reinterpret_cast<const uint16_t*>(src);
-  if (VEC && chunk * 8 + 8 <= cols) {
-    const uint4 u = load16<F>(src);
-    r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
-  } else if (!VEC && (reinterpret_cast<uintptr_t>(src) & 2u) == 0 && chunk * 8 + 8 <= cols) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(one + 2 * i);
-  } else if (!VEC && chunk > 0 && chunk * 8 + 9 <= cols) {  // the five words that it lies in
-    uint32_t w[5];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = *reinterpret_cast<const uint32_t*>(one - 1 + 2 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __funnelshift_r(w[i], w[i + 1], 16u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = chunk * 8 + 2 * i < cols ? one[2 * i] : 0u, hi = chunk * 8 + 2 * i + 1 < cols ? one[2 * i + 1] : 0u;
-      r[i] = lo | hi << 16;
-    }
-  }
-}
-
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int chunk, int cols, const uint32_t (&r)[4]) {
-  T* dst = row + (int64_t)chunk * 8;
-  uint16_t* one = reinterpret_cast<uint16_t*>(dst);
-  if (VEC && chunk * 8 + 8 <= cols) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(r[0], r[1], r[2], r[3]);
-  } else if (chunk * 8 + 8 <= cols) {  // words, between two halves of one where they do not begin on 4 bytes
-    if (reinterpret_cast<uintptr_t>(dst) & 2u) {
-      one[0] = (uint16_t)r[0];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(one + 2 * i + 1) = __funnelshift_r(r[i], r[i + 1], 16u);
-      one[7] = (uint16_t)(r[3] >> 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(one + 2 * i) = r[i];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (chunk * 8 + e < cols) one[e] = (uint16_t)(r[e / 2] >> (e % 2 * 16));
-  }
-}
-
-// max(a, |b|, |c|), NaN if one of them is
-__device__ __forceinline__ float max_abs(float a, float b, float c) {
-  float d;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 
 // What a thread holds of a chunk between the reduction and the quantization, and what it adds to the row's sums.  Plain rows
 // stay packed, the others are t in fp32.

@@ -57,6 +57,26 @@ INT8_SYMBOLS = (
 )
 INT8_FP16, INT8_BF16 = 0, 1
 
+FP8_SYMBOLS = (
+    "fp8_rows_quant_sm100",
+    "fp8_rows_gather_quant_sm100",
+    "fp8_rows_silu_mul_sm100",
+    "fp8_weight_quant_sm100",
+    "fp8_rows_dequant_sm100",
+    "fp8_weight_dequant_sm100",
+    "fp8_gemm_sm100",
+    "fp8_experts_gemm_sm100",
+)
+FP8_EXPERTS_ZERO_REST = 0x100
+EXPERTS_SYMBOLS = (
+    "experts_sort_workspace_size",
+    "experts_sort_sm100",
+    "experts_gather_sm100",
+    "experts_combine_sm100",
+    "experts_combine_backward_sm100",
+)
+EXPERTS_FP32 = 2
+
 
 class BlkQ4Error(RuntimeError):
     pass
@@ -149,6 +169,21 @@ def _load() -> ctypes.CDLL:
     lib.int8_rows_dequant_sm100.argtypes = [i, i, i, vp, *matrix, *vector, *matrix, vp]
     lib.int8_gemm_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, *matrix, *vector, *vector, *matrix, ctypes.c_uint, vp]
     lib.int8_gemm_plan_sm100.argtypes = [i, i, i, ctypes.POINTER(i)]
+    lib.fp8_rows_quant_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *matrix, vp]
+    lib.fp8_rows_gather_quant_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, vp, *matrix, *matrix, vp]
+    lib.fp8_rows_silu_mul_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *matrix, *matrix, vp]
+    lib.fp8_weight_quant_sm100.argtypes = [i, i, i, i, vp, *matrix, *matrix, *matrix, vp]
+    lib.fp8_rows_dequant_sm100.argtypes = [i, i, i, vp, *matrix, *matrix, *matrix, vp]
+    lib.fp8_weight_dequant_sm100.argtypes = [i, i, i, i, vp, *matrix, *matrix, *matrix, vp]
+    lib.fp8_gemm_sm100.argtypes = [i, i, i, i, vp, *matrix, *matrix, *matrix, *matrix, *vector, *matrix, ctypes.c_uint, vp]
+    stacked = [*matrix, ctypes.c_int64]
+    lib.fp8_experts_gemm_sm100.argtypes = [i, i, i, i, i, vp, *matrix, *matrix, *stacked, *stacked, *vector, *matrix, ctypes.c_uint, vp]
+    lib.experts_sort_workspace_size.restype = ctypes.c_size_t
+    lib.experts_sort_workspace_size.argtypes = [ctypes.c_int64, i]
+    lib.experts_sort_sm100.argtypes = [ctypes.c_int64, i, i, vp, *vector, *vector, *vector, *vector, *vector, vp]
+    lib.experts_gather_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, vp, *matrix, vp]
+    lib.experts_combine_sm100.argtypes = [i, i, i, i, vp, *matrix, *vector, *vector, i, *matrix, vp]
+    lib.experts_combine_backward_sm100.argtypes = [i, i, i, i, vp, *matrix, *matrix, *vector, i, *vector, vp, *matrix, *vector, vp]
     for name in INT8_SYMBOLS:
         getattr(lib, name).restype = i
     return lib
@@ -451,3 +486,58 @@ def int8_gemm_plan(m: int, n: int, k: int) -> dict:
         raise BlkQ4Error(f"no plan for {m}x{n}x{k}")
     names = ("kernel", "tile_m", "tile_n", "tiles", "split", "steps", "stages", "smem")
     return {**dict(zip(names, out)), "kernel": ("stream", "one-cta", "pair")[out[0]]}
+
+
+# ---- 8-bit floating-point path and layers of experts ----
+def fp8_rows_quant(dtype, rows, cols, x, values, scales, stream=0):
+    _int8_call(lib.fp8_rows_quant_sm100, dtype, rows, cols, stream, *_matrix(x), *_matrix(values), *_matrix(scales))
+
+
+def fp8_rows_gather_quant(dtype, tokens, choices, cols, x, source, count, values, scales, stream=0):
+    _int8_call(lib.fp8_rows_gather_quant_sm100, dtype, tokens, choices, cols, stream, *_matrix(x), *_ptr_size(source), count,
+               *_matrix(values), *_matrix(scales))
+
+
+def fp8_rows_silu_mul(dtype, rows, cols, gate, up, values, scales, stream=0):
+    _int8_call(lib.fp8_rows_silu_mul_sm100, dtype, rows, cols, stream, *_matrix(gate), *_matrix(up), *_matrix(values), *_matrix(scales))
+
+
+def fp8_weight_quant(dtype, experts, n, k, w, values, scales, stream=0):
+    _int8_call(lib.fp8_weight_quant_sm100, dtype, experts, n, k, stream, *_matrix(w), *_matrix(values), *_matrix(scales))
+
+
+def fp8_rows_dequant(dtype, rows, cols, values, scales, out, stream=0):
+    _int8_call(lib.fp8_rows_dequant_sm100, dtype, rows, cols, stream, *_matrix(values), *_matrix(scales), *_matrix(out))
+
+
+def fp8_weight_dequant(dtype, experts, n, k, values, scales, out, stream=0):
+    _int8_call(lib.fp8_weight_dequant_sm100, dtype, experts, n, k, stream, *_matrix(values), *_matrix(scales), *_matrix(out))
+
+
+def fp8_gemm(dtype, m, n, k, x, x_scales, w, w_scales, bias, out, flags=0, stream=0):
+    _int8_call(lib.fp8_gemm_sm100, dtype, m, n, k, stream, *_matrix(x), *_matrix(x_scales), *_matrix(w), *_matrix(w_scales),
+               *_ptr_size(bias), *_matrix(out), flags)
+
+
+def fp8_experts_gemm(dtype, experts, rows, n, k, x, x_scales, w, w_stride, w_scales, ws_stride, offsets, out, flags=0, stream=0):
+    _int8_call(lib.fp8_experts_gemm_sm100, dtype, experts, rows, n, k, stream, *_matrix(x), *_matrix(x_scales), *_matrix(w), w_stride,
+               *_matrix(w_scales), ws_stride, *_ptr_size(offsets), *_matrix(out), flags)
+
+
+def experts_sort(n, n_experts, id_bytes, ids, source, places, offsets, workspace=None, stream=0):
+    _int8_call(lib.experts_sort_sm100, n, n_experts, id_bytes, stream, *_ptr_size(ids), *_ptr_size(source), *_ptr_size(places),
+               *_ptr_size(offsets), *_ptr_size(workspace))
+
+
+def experts_gather(dtype, tokens, choices, cols, x, source, count, out, stream=0):
+    _int8_call(lib.experts_gather_sm100, dtype, tokens, choices, cols, stream, *_matrix(x), *_ptr_size(source), count, *_matrix(out))
+
+
+def experts_combine(dtype, tokens, choices, cols, y, places, weights, weights_type, out, stream=0):
+    _int8_call(lib.experts_combine_sm100, dtype, tokens, choices, cols, stream, *_matrix(y), *_ptr_size(places), *_ptr_size(weights),
+               weights_type, *_matrix(out))
+
+
+def experts_combine_backward(dtype, tokens, choices, cols, d, y, weights, weights_type, source, count, d_y, d_weights, stream=0):
+    _int8_call(lib.experts_combine_backward_sm100, dtype, tokens, choices, cols, stream, *_matrix(d), *_matrix(y), *_ptr_size(weights),
+               weights_type, *_ptr_size(source), count, *_matrix(d_y), *_ptr_size(d_weights))

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "blkq4_common.cuh"
+#include "fp8.cuh"
 #include "int8.cuh"
 #include "ms_blkq4gemm.h"
 
@@ -319,7 +320,9 @@ extern "C" int blkq4_last_kernel_status(void* stream_ptr) {
   const int i8 = blkq4::int8::read_gemm_error();
   if (i8 != 0) return i8 > 0 ? (0x40000 | i8) : i8;
   const int rows = blkq4::int8::read_rows_error();
-  return rows > 0 ? (0x80000 | rows) : rows;
+  if (rows != 0) return rows > 0 ? (0x80000 | rows) : rows;
+  const int f8 = blkq4::fp8::read_gemm_error();
+  return f8 > 0 ? (0x100000 | f8) : f8;
 }
 extern "C" int blkq4_reset(void* stream_ptr) {
   auto stream = reinterpret_cast<cudaStream_t>(stream_ptr);
@@ -329,6 +332,7 @@ extern "C" int blkq4_reset(void* stream_ptr) {
   rc |= blkq4::clear_skinny_tc_error(stream);
   rc |= blkq4::int8::clear_gemm_error(stream);
   rc |= blkq4::int8::clear_rows_error(stream);
+  rc |= blkq4::fp8::clear_gemm_error(stream);
   rc |= blkq4::reset_static_scratch(stream);
   return rc == 0 ? 0 : -1;
 }

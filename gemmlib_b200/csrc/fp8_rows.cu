@@ -1,0 +1,346 @@
+// Rows and weights of e4m3 with fp32 scales, from 16-bit ones; and back.
+//
+//   t[k]   rows, weights: x[k]        gate: g[k] / (1 + exp(-g[k])) * u[k]
+//   values = e4m3(t * (448 / max|t|)), half to even         scale = max|t| / 448
+//
+// with the largest magnitude taken over 128 elements of a row, or over 128 x 128 of a weight.  One pass: a block is held in registers
+// between its reduction and its conversion.  Rows: a block is 16 lanes of 8 elements, so that half a warp reads and reduces it without
+// shared memory, and a half-warp takes up to four blocks of a row at a time to have their loads in flight together.  Weights: a CTA a block.
+// Bound by HBM: 3 bytes an element, 5 for the gate.
+//
+// Halves: 16-bit inputs often stand exactly half-way between two e4m3 numbers (wherever max|t| is a multiple of 7, for one), and the rounded
+// factor 448 / max|t| would put them to one side.  The quotient 448 x / max of numbers of 11 bits is either half-way between two numbers of 4
+// bits or at least 2^-16 of itself away from it (the difference is a fraction of integers over max times a number of 5 bits), so the product,
+// which is off by less than 2^-21, is rounded to 18 bits first: what is half-way lies there then, and nothing else does.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "fp8.cuh"
+#include "rows_io.cuh"
+
+namespace blkq4 {
+namespace fp8 {
+namespace {
+
+using namespace blkq4::int8;
+
+constexpr int kThreads = 128;
+
+// What a block's largest |t| (its bits) says.
+struct Scale {
+  bool finite;
+  float up, inverse;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t top) {
+  Scale s;
+  // A block with an infinity or NaN has no scale that its other values could be told by: it is NaN as a whole.
+  s.finite = top < 0x7f800000u;
+  const float amax = s.finite ? __uint_as_float(top) : 0.0f;
+  // 448 / amax is no float below 2^-119, and its approximation is none beyond 2^126: such blocks are moved by 2^64 first
+  s.up = amax < 0x1p-64f ? 0x1p64f : amax > 0x1p64f ? 0x1p-64f : 1.0f;
+  s.inverse = amax > 0.0f ? __fdividef(448.0f, amax * s.up) : 0.0f;
+  return s;
+}
+__device__ __forceinline__ float scale_value(uint32_t top) {
+  return top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 448.0f) : __uint_as_float(0x7fc00000u);
+}
+// v rounded to 18 bits, half up: between there and a number of 4 bits no other rounding can come.
+__device__ __forceinline__ float to_18_bits(float v) { return __uint_as_float((__float_as_uint(v) + 0x20u) & 0xffffffc0u); }
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool SHORT>  // t are 16-bit numbers
+__device__ __forceinline__ uint2 convert8(const Scale& s, float (&v)[8]) {
+  if (!s.finite || s.up != 1.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s.finite ? v[e] * s.up : 0.0f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] *= s.inverse;
+    if (SHORT) v[e] = to_18_bits(v[e]);
+  }
+  uint2 o;
+  o.x = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
+  o.y = e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16;
+  return o;
+}
+// Rows of 8-bit values: 8 of them, `chunk` times 8 behind the beginning of the row.
+__device__ __forceinline__ void store_q8(uint8_t* row, bool vec, int chunk, int cols, uint2 o) {
+  uint8_t* dst = row + (int64_t)chunk * 8;
+  if (vec && chunk * 8 + 8 <= cols) {
+    *reinterpret_cast<uint2*>(dst) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (chunk * 8 + e < cols) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (e % 4 * 8));
+  }
+}
+// Bits of the largest magnitude, NaN last.
+template <class T>
+__device__ __forceinline__ uint32_t top_of(const uint32_t (&r)[4]) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t = as_word(__hmax2_nan(as_pair<T>(t), __habs2(as_pair<T>(r[i]))));
+  const float2 f = unpack2(t, T());
+  return __float_as_uint(max_abs(f.x, f.y, 0.0f)) & 0x7fffffffu;
+}
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
+  float t = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) t = max_abs(t, v[e], v[e + 1]);
+  return __float_as_uint(t) & 0x7fffffffu;
+}
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, s));
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void gated(uint32_t (&a)[4], uint32_t (&b)[4], float (&v)[8]) {
+  float u[8];
+  unpack8<T>(a, v);
+  unpack8<T>(b, u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    // g / (1 + 2^(-g log2 e)); 1 + an infinity has the reciprocal 0
+    float p, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(v[e] * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + p));
+    v[e] = v[e] * r * u[e];
+  }
+}
+
+// The part of a row that a half-warp takes: U blocks from `block` on.
+struct Part {
+  int64_t row;
+  int block;
+};
+__device__ __forceinline__ Part part_of(int parts, int U) {
+  const int64_t i = (int64_t)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  Part p;
+  if (i < 0xffffffffll) {
+    p.row = (uint32_t)i / (uint32_t)parts;
+    p.block = (int)((uint32_t)i % (uint32_t)parts) * U;
+  } else {
+    p.row = i / parts;
+    p.block = (int)(i % parts) * U;
+  }
+  return p;
+}
+
+template <int OP, class T, bool VEC, bool GATHER, int U>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int parts, bool q_vec) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const Part at = part_of(parts, U);
+  const int lane = threadIdx.x & 15;
+  bool in = at.row < p.rows;
+  int64_t from = at.row;
+  if (GATHER && in) {
+    from = at.row < *p.count ? p.source[at.row] / p.choices : -1;
+    if (from >= p.x_rows) from = -1;  // (of an order that is none)
+  }
+  uint32_t a[U][4] = {}, b[U][4] = {};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int chunk = (at.block + u) * 16 + lane;
+    if (in && from >= 0 && chunk * 8 < p.cols) {
+      load8<T, VEC, OP == kSiluMul ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + from * p.lda, chunk, p.cols, a[u]);
+      if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.b) + from * p.ldb, chunk, p.cols, b[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int chunk = (at.block + u) * 16 + lane;
+    float v[8];
+    uint32_t top;
+    if constexpr (OP == kSiluMul) {
+      gated<T>(a[u], b[u], v);
+      top = top_of(v);
+    } else {
+      top = top_of<T>(a[u]);
+      unpack8<T>(a[u], v);
+    }
+    top = half_warp_max(top);
+    if (!in || chunk * 8 >= p.cols) continue;
+    const Scale s = scale_of(top);
+    store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, convert8<OP == kQuant>(s, v));
+    if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale_value(top);
+  }
+}
+
+// A CTA a block of 128 x 128: 16 lanes a row, 16 rows at a time.
+constexpr int kWeightThreads = 256;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const RowsParams p, int k_blocks, int n_blocks, bool q_vec) {
+  __shared__ uint32_t tops[kWeightThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t block = blockIdx.x;
+  const int kb = (int)(block % k_blocks);
+  const int64_t eb = block / k_blocks;
+  const int nb = (int)(eb % n_blocks);
+  const int64_t expert = eb / n_blocks;
+  const int chunk = kb * 16 + (threadIdx.x & 15), n0 = nb * kBlock + (threadIdx.x >> 4);
+  const bool in_cols = chunk * 8 < p.cols;
+  const int64_t row0 = expert * p.expert_rows + n0;
+  uint32_t a[8][4] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (in_cols && n0 + 16 * i < p.expert_rows)
+      load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.a) + (row0 + 16 * i) * p.lda, chunk, p.cols, a[i]);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, top_of<T>(a[i]));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWeightThreads / 32; ++i) top = max(top, tops[i]);
+  const Scale s = scale_of(top);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!in_cols || n0 + 16 * i >= p.expert_rows) continue;
+    float v[8];
+    unpack8<T>(a[i], v);
+    store_q8(p.q + (row0 + 16 * i) * p.ldq, q_vec, chunk, p.cols, convert8<true>(s, v));
+  }
+  if (threadIdx.x == 0) p.scales[(expert * n_blocks + nb) * p.lds + kb] = scale_value(top);
+}
+
+// out = scale * values
+template <class T, bool WEIGHTS, int U>
+__global__ void __launch_bounds__(kThreads) dequant_kernel(const DequantParams p, int parts, bool q_vec, bool out_vec) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const Part at = part_of(parts, U);
+  if (at.row >= p.rows) return;
+  int64_t scale_row = at.row;
+  if (WEIGHTS) {
+    const int64_t expert = at.row / p.expert_rows, n_blocks = (p.expert_rows + kBlock - 1) / kBlock;
+    scale_row = expert * n_blocks + (at.row - expert * p.expert_rows) / kBlock;
+  }
+  const uint8_t* q = p.q + at.row * p.ldq;
+  T* out = reinterpret_cast<T*>(p.out) + at.row * p.ldo;
+  uint2 r[U];
+  float scale[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int chunk = (at.block + u) * 16 + (threadIdx.x & 15);
+    r[u] = make_uint2(0u, 0u);
+    if (chunk * 8 >= p.cols) continue;
+    scale[u] = p.scales[scale_row * p.lds + at.block + u];
+    if (q_vec && chunk * 8 + 8 <= p.cols) {
+      r[u] = *reinterpret_cast<const uint2*>(q + (int64_t)chunk * 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (chunk * 8 + e < p.cols) (e < 4 ? r[u].x : r[u].y) |= (uint32_t)q[(int64_t)chunk * 8 + e] << (e % 4 * 8);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int chunk = (at.block + u) * 16 + (threadIdx.x & 15);
+    if (chunk * 8 >= p.cols) continue;
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = (i < 2 ? r[u].x : r[u].y) >> (i % 2 * 16);
+      uint32_t h;  // e4m3 is exact in fp16
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)w));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      o[i] = pack2<T>(f.x * scale[u], f.y * scale[u]);
+    }
+    if (out_vec) store8<T, true>(out, chunk, p.cols, o);
+    else store8<T, false>(out, chunk, p.cols, o);
+  }
+}
+
+template <class... Params, class... Args>
+std::string launch(void (*kernel)(Params...), int64_t ctas, int threads, cudaStream_t stream, Args... args) {
+  if (ctas > 0x7fffffffll) return "too many rows";
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
+}
+bool rows_on(const void* ptr, int64_t pitch_bytes, int rows, int bytes) {
+  return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && (rows <= 1 || pitch_bytes % bytes == 0);
+}
+
+// Blocks that a half-warp takes at a time: what hides the latency of many rows, one where they are few.
+int blocks_at_a_time(int rows, int cols) {
+  const int64_t blocks = (int64_t)rows * blocks_of(cols);
+  const int most = blocks_of(cols);
+  return blocks >= 8 * 148 * 16 && most >= 4 ? 4 : blocks >= 4 * 148 * 16 && most >= 2 ? 2 : 1;
+}
+template <int OP, class T, bool VEC, bool GATHER>
+std::string launch_rows_u(const RowsParams& p, cudaStream_t stream) {
+  const int U = blocks_at_a_time(p.rows, p.cols), parts = (blocks_of(p.cols) + U - 1) / U;
+  const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
+  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8);
+  if (U == 4) return launch(rows_kernel<OP, T, VEC, GATHER, 4>, ctas, kThreads, stream, p, parts, q_vec);
+  if (U == 2) return launch(rows_kernel<OP, T, VEC, GATHER, 2>, ctas, kThreads, stream, p, parts, q_vec);
+  return launch(rows_kernel<OP, T, VEC, GATHER, 1>, ctas, kThreads, stream, p, parts, q_vec);
+}
+template <class T>
+std::string launch_rows_t(RowsOp op, const RowsParams& p, cudaStream_t stream) {
+  if (op == kSiluMul) {
+    const bool vec = rows_on(p.a, p.lda * 2, p.rows, 16) && rows_on(p.b, p.ldb * 2, p.rows, 16);
+    return vec ? launch_rows_u<kSiluMul, T, true, false>(p, stream) : launch_rows_u<kSiluMul, T, false, false>(p, stream);
+  }
+  if (p.source) {
+    const bool vec = rows_on(p.a, p.lda * 2, p.x_rows, 16);
+    return vec ? launch_rows_u<kQuant, T, true, true>(p, stream) : launch_rows_u<kQuant, T, false, true>(p, stream);
+  }
+  const bool vec = rows_on(p.a, p.lda * 2, p.rows, 16);
+  return vec ? launch_rows_u<kQuant, T, true, false>(p, stream) : launch_rows_u<kQuant, T, false, false>(p, stream);
+}
+template <class T>
+std::string launch_weights_t(const RowsParams& p, cudaStream_t stream) {
+  const int k_blocks = blocks_of(p.cols), n_blocks = blocks_of(p.expert_rows);
+  const int64_t ctas = (int64_t)(p.rows / p.expert_rows) * n_blocks * k_blocks;
+  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8);
+  return rows_on(p.a, p.lda * 2, p.rows, 16) ? launch(weights_kernel<T, true>, ctas, kWeightThreads, stream, p, k_blocks, n_blocks, q_vec)
+                                             : launch(weights_kernel<T, false>, ctas, kWeightThreads, stream, p, k_blocks, n_blocks, q_vec);
+}
+template <class T, bool WEIGHTS>
+std::string launch_dequant_t(const DequantParams& p, cudaStream_t stream) {
+  const int U = blocks_at_a_time(p.rows, p.cols), parts = (blocks_of(p.cols) + U - 1) / U;
+  const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
+  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8), out_vec = rows_on(p.out, p.ldo * 2, p.rows, 16);
+  if (U == 4) return launch(dequant_kernel<T, WEIGHTS, 4>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
+  if (U == 2) return launch(dequant_kernel<T, WEIGHTS, 2>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
+  return launch(dequant_kernel<T, WEIGHTS, 1>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
+}
+
+}  // namespace
+
+std::string launch_rows(RowsOp op, Dtype dtype, const RowsParams& p, cudaStream_t stream) {
+  return dtype == kFp16 ? launch_rows_t<__half>(op, p, stream) : launch_rows_t<__nv_bfloat16>(op, p, stream);
+}
+std::string launch_weights(Dtype dtype, const RowsParams& p, cudaStream_t stream) {
+  return dtype == kFp16 ? launch_weights_t<__half>(p, stream) : launch_weights_t<__nv_bfloat16>(p, stream);
+}
+std::string launch_dequant(Dtype dtype, const DequantParams& p, cudaStream_t stream) {
+  if (p.expert_rows > 0)
+    return dtype == kFp16 ? launch_dequant_t<__half, true>(p, stream) : launch_dequant_t<__nv_bfloat16, true>(p, stream);
+  return dtype == kFp16 ? launch_dequant_t<__half, false>(p, stream) : launch_dequant_t<__nv_bfloat16, false>(p, stream);
+}
+
+}  // namespace fp8
+}  // namespace blkq4

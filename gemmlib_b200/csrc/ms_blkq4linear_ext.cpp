@@ -31,6 +31,7 @@
 #include "ms_blkq4gemm.h"
 
 bool add_int8_functions(PyObject* module);  // ms_int8linear_ext.cpp
+bool add_fp8_functions(PyObject* module);   // ms_fp8linear_ext.cpp
 
 namespace {
 
@@ -391,7 +392,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("block_size"), py::arg("col_wise"), py::arg("in_features"), py::arg("out_features"),
         py::arg("input"), py::arg("q_weights"), py::arg("q_scales"), py::arg("q_zp"), py::arg("output"),
         py::arg("bias") = py::none(), py::arg("flags") = 0, py::arg("workspace") = py::none());
-  if (PyModule_AddFunctions(m.ptr(), g_methods) != 0 || !add_int8_functions(m.ptr())) throw py::error_already_set();
+  if (PyModule_AddFunctions(m.ptr(), g_methods) != 0 || !add_int8_functions(m.ptr()) || !add_fp8_functions(m.ptr())) throw py::error_already_set();
   m.def("workspace_source",
         [](py::dict eager, py::function provide) {
           g_eager_workspaces = eager.release().ptr();

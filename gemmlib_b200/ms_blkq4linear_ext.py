@@ -49,3 +49,14 @@ rms_norm_int8 = _mod.rms_norm_int8
 silu_mul_int8 = _mod.silu_mul_int8
 int8_dequantize = _mod.int8_dequantize
 int8_linear = _mod.int8_linear
+fp8_types = _mod.fp8_types
+fp8_quantize = _mod.fp8_quantize
+fp8_quantize_weight = _mod.fp8_quantize_weight
+silu_mul_fp8 = _mod.silu_mul_fp8
+fp8_dequantize = _mod.fp8_dequantize
+fp8_linear = _mod.fp8_linear
+fp8_expert_linear = _mod.fp8_expert_linear
+experts_sort = _mod.experts_sort
+experts_gather = _mod.experts_gather
+experts_combine = _mod.experts_combine
+experts_combine_backward = _mod.experts_combine_backward

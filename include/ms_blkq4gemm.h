@@ -406,6 +406,151 @@ int int8_gemm_sm100(
 int int8_gemm_plan_sm100(int m, int n, int k, int* out8);
 
 /*
+ * The 8-bit floating-point path: e4m3 rows with an fp32 scale for each block of 128 elements, e4m3 weights [n, k] with one for each block of
+ * 128 x 128, what produces them, and their product; blocks at an edge hold what is left.  No counterpart in the reference.
+ *
+ *   - A block stands for scale * values.  scale = max|t| / 448 and values = e4m3(t * 448 / max|t|), half to even, where t is the block to be
+ *     quantized.  A block of zeros has scale 0.  A block with an infinity or NaN among its t has scale NaN and values 0, so that what
+ *     is computed from it is NaN: all outputs of that row, or of the 128 outputs of that weight's block.
+ *   - Arguments as for the int8 path: dtype INT8_FP16 or INT8_BF16, ld* in elements from row to row, *_size in bytes.  scales of rows: [rows,
+ *     ceil(cols / 128)] with lds; of a weight: [ceil(n / 128), ceil(k / 128)].  Weights of several experts: their rows, and the rows of
+ *     their scales, follow one another.
+ */
+
+/** values, scales = rows of x [rows, cols]. */
+int fp8_rows_quant_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size, int64_t lds,
+  void* error_message);
+
+/** The same of the rows that experts_gather_sm100 would write, [tokens * choices, cols], without writing those. */
+int fp8_rows_gather_quant_sm100(
+  int dtype, int tokens, int choices, int cols, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* source, size_t source_size, void const* count,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size, int64_t lds,
+  void* error_message);
+
+/** t = gate / (1 + exp(-gate)) * up, in fp32. */
+int fp8_rows_silu_mul_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* gate, size_t gate_size, int64_t ldg,
+  void const* up, size_t up_size, int64_t ldu,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size, int64_t lds,
+  void* error_message);
+
+/** values, scales = weights w [experts, n, k], a scale for each 128 x 128 of an expert. */
+int fp8_weight_quant_sm100(
+  int dtype, int experts, int n, int k, void* stream,
+  void const* w, size_t w_size, int64_t ldw,
+  void* values, size_t values_size, int64_t ldv,
+  void* scales, size_t scales_size, int64_t lds,
+  void* error_message);
+
+/** out = scale * values, rounded to the 16-bit type: of rows, and of weights. */
+int fp8_rows_dequant_sm100(
+  int dtype, int rows, int cols, void* stream,
+  void const* values, size_t values_size, int64_t ldv,
+  void const* scales, size_t scales_size, int64_t lds,
+  void* out, size_t out_size, int64_t ldo,
+  void* error_message);
+int fp8_weight_dequant_sm100(
+  int dtype, int experts, int n, int k, void* stream,
+  void const* values, size_t values_size, int64_t ldv,
+  void const* scales, size_t scales_size, int64_t lds,
+  void* out, size_t out_size, int64_t ldo,
+  void* error_message);
+
+/**
+ * out[m, n] = sum over the blocks b of k of x_scales[m, b] * w_scales[n / 128, b] * (sum over k in b of x[m, k] w[n, k]) (+ bias[n]), for any m, n
+ * and k.  All sums are held in fp32 and the result is rounded to the 16-bit type once.  The product of two scales has to be a float32.
+ * bias: [n] of that type, or null.  x and w: 16-byte aligned, ldx and ldw multiples of 16.  out may not overlap what the call reads.
+ * BLKQ4_GEMM_EARLY_WEIGHT_FETCH: as for int8_gemm_sm100.
+ */
+int fp8_gemm_sm100(
+  int dtype, int m, int n, int k, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* x_scales, size_t x_scales_size, int64_t ldxs,
+  void const* w, size_t w_size, int64_t ldw,
+  void const* w_scales, size_t w_scales_size, int64_t ldws,
+  void const* bias, size_t bias_size,
+  void* out, size_t out_size, int64_t ldo,
+  unsigned flags,
+  void* error_message);
+
+/**
+ * The same for a layer of experts: rows [offsets[e], offsets[e + 1]) of x are multiplied with weight e of [experts, n, k] (w_stride bytes and
+ * ws_stride floats from expert to expert).  offsets: experts + 1 int32 on the device, rising, within [0, rows]; the call does not wait for
+ * them, and offsets that are none of these lead to no access out of bounds (a value is taken for the nearest that fits behind those before).
+ * Rows of no expert are left as they are, or set to zero with FP8_EXPERTS_ZERO_REST.  Up to 2048 experts.
+ */
+#define FP8_EXPERTS_ZERO_REST 0x100u
+int fp8_experts_gemm_sm100(
+  int dtype, int experts, int rows, int n, int k, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* x_scales, size_t x_scales_size, int64_t ldxs,
+  void const* w, size_t w_size, int64_t ldw, int64_t w_stride,
+  void const* w_scales, size_t w_scales_size, int64_t ldws, int64_t ws_stride,
+  void const* offsets, size_t offsets_size,
+  void* out, size_t out_size, int64_t ldo,
+  unsigned flags,
+  void* error_message);
+
+/*
+ * Tokens sorted by expert and back.  ids [tokens, choices] (int32 or int64, id_bytes each) names the expert of every choice; one that is none of
+ * 0 .. n_experts - 1 belongs to no expert here (padding, another GPU's).  The order is stable: an expert's rows follow the choices' order.
+ *   offsets [n_experts + 1]     first place of each expert; offsets[n_experts]: number of choices that belong to one
+ *   source [tokens * choices]   the choice (token * choices + number) at each place; those of no expert come last
+ *   places [tokens, choices]    the place of each choice, -1 for those of no expert
+ * All int32.  workspace: of experts_sort_workspace_size bytes (0: may be null), free again once the call's work is done.
+ * Up to 2048 experts and 2^28 choices.
+ */
+size_t experts_sort_workspace_size(int64_t n, int n_experts);
+int experts_sort_sm100(
+  int64_t n, int n_experts, int id_bytes, void* stream,
+  void const* ids, size_t ids_size,
+  void* source, size_t source_size,
+  void* places, size_t places_size,
+  void* offsets, size_t offsets_size,
+  void* workspace, size_t workspace_size,
+  void* error_message);
+
+/** out[p] = x[source[p] / choices] for p < *count (offsets + n_experts, on the device), zeros behind: [tokens * choices, cols]. */
+int experts_gather_sm100(
+  int dtype, int tokens, int choices, int cols, void* stream,
+  void const* x, size_t x_size, int64_t ldx,
+  void const* source, size_t source_size, void const* count,
+  void* out, size_t out_size, int64_t ldo,
+  void* error_message);
+
+/** out[t] = sum over j of weights[t, j] * y[places[t, j]], in fp32 in the order of j, rounded once; choices of no expert add nothing.  weights:
+ *  [tokens, choices] of weights_type (INT8_FP16, INT8_BF16, EXPERTS_FP32), or null for ones (the gradient of experts_gather_sm100). */
+#define EXPERTS_FP32 2
+int experts_combine_sm100(
+  int dtype, int tokens, int choices, int cols, void* stream,
+  void const* y, size_t y_size, int64_t ldy,
+  void const* places, size_t places_size,
+  void const* weights, size_t weights_size, int weights_type,
+  void* out, size_t out_size, int64_t ldo,
+  void* error_message);
+
+/** The gradient of experts_combine_sm100: d_y[p] = weights[source[p]] * d[token of p] (zeros behind *count), d_weights[source[p]] = sum of y[p] * d[token
+ *  of p] in fp32 (0 for choices of no expert). */
+int experts_combine_backward_sm100(
+  int dtype, int tokens, int choices, int cols, void* stream,
+  void const* d, size_t d_size, int64_t ldd,
+  void const* y, size_t y_size, int64_t ldy,
+  void const* weights, size_t weights_size, int weights_type,
+  void const* source, size_t source_size, void const* count,
+  void* d_y, size_t d_y_size, int64_t lddy,
+  void* d_weights, size_t d_weights_size,
+  void* error_message);
+
+/*
  * Additions with no counterpart in the reference.  The reference reports errors
  * through a std::string*, which only a C++ caller can supply.  These three let
  * a C, ctypes, cgo or JNI caller own such an object.

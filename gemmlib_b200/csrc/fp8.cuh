@@ -15,7 +15,7 @@ namespace fp8 {
 using int8::Dtype;
 
 constexpr int kBlock = 128;   // elements that share a scale, along k and along n
-constexpr int kMaxExperts = 2048;
+constexpr int kMaxExperts = 1024;
 
 struct RowsParams {
   const void* a;      // x, or gate

@@ -8,7 +8,7 @@
 // in fp32 registers under the MMAs of the next steps.  The scales' product goes to a value with one multiply-add of its own.
 //
 // Two kernels.  fp8_rows_kernel (here): 128 weight rows (TMEM lanes) x 16 to 128 activation rows a tile, for few rows, where the weights'
-// bytes are what counts.  fp8_pair_kernel (fp8_gemm_pair.cuh): 256 activation rows (TMEM lanes of two CTAs) x up to 256 weight rows, for many.
+// bytes are what counts.  fp8_wide_kernel (fp8_gemm_wide.cuh): 128 activation rows (TMEM lanes) x 256 weight rows, for many.
 //
 // Experts: the offsets are on the device and stay there.  Every CTA reads them once, counts the tiles of each expert, and walks through every
 // gridDim-th tile of them all; so the launch does not depend on them.  They are read as a rising sequence within the rows (a value that is none
@@ -48,6 +48,22 @@ constexpr long long kWaitCycles = 4000000000ll;  // ~2 s: far beyond any legitim
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
   return mbar_wait_bounded(bar, parity, abort_flag, &g_fp8_error, who, kWaitCycles);
 }
+// `wait` of a whole warp, with one answer for all of it.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 1000u))) return true;
+    const bool late = clock64() - t0 > kWaitCycles;
+    if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+      if (late) {
+        *abort_flag = 1;
+        atomicCAS(&g_fp8_error, 0, who);
+      }
+      return false;
+    }
+  }
+}
 // `wait` on a barrier that other CTAs of the cluster arrive on.
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
   const long long t0 = clock64();
@@ -85,7 +101,6 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int umma_m, int umma_n) {
         : "memory");                                                                                                               \
   }
 FP8_UMMA_X4(umma_e4m3_x4, "1")
-FP8_UMMA_X4(umma_e4m3_x4_pair, "2")
 #undef FP8_UMMA_X4
 
 // Groups of eight columns, 16 columns apart, there when it returns: loads and wait are one statement, so that no use of the registers can
@@ -134,6 +149,10 @@ __device__ __forceinline__ void prefetch_l2_3d(const CUtensorMap* map, int x, in
 // Four bytes, or zeros in their place.
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// 16 bytes, of which the first `bytes` are copied and the others zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // Arrives on the barrier once this thread's copies so far have landed.
 __device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
@@ -559,6 +578,8 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   }
 }
 
+#include "fp8_gemm_wide.cuh"
+
 // ---- plans ----
 struct RowsPlan {
   int BN, n_tiles, split, k_per_cta, slice, stages, ctas;
@@ -664,9 +685,48 @@ std::string launch_rows_kernel(const GemmArgs& g, const RowsPlan& r, unsigned fl
 }
 
 template <class T>
+std::string launch_wide_kernel(const GemmArgs& g, int ctas, unsigned flags, cudaStream_t stream) {
+  WideParams p{};
+  p.M = g.M; p.N = g.N;
+  p.n_tiles = (g.N + kWideN - 1) / kWideN;
+  p.k_steps = (g.K + kStepK - 1) / kStepK;
+  p.experts = g.experts; p.offsets = g.offsets; p.zero_rest = g.zero_rest;
+  p.early = (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0;
+  p.scales_on_16 = reinterpret_cast<uintptr_t>(g.x_scales) % 16 == 0 && (g.M == 1 || g.ldxs % 4 == 0);
+  const auto begins_on = [&](int n) { return reinterpret_cast<uintptr_t>(g.out) % (2 * n) == 0 && (g.M == 1 || g.ldo % n == 0) && g.N % n == 0; };
+  p.vector = begins_on(16) ? 16 : begins_on(8) ? 8 : 1;
+  p.out = g.out; p.ldo = g.ldo;
+  p.x_scales = g.x_scales; p.ldxs = g.ldxs;
+  p.w_scales = g.w_scales; p.ldws = g.ldws; p.ws_stride = g.ws_stride;
+  p.bias = g.bias;
+  CUtensorMap tm_x, tm_w;
+  if (!encode_rows(&tm_x, g.x, g.ldx, g.K, g.M, kWideM) || !encode_weights(&tm_w, g, kWideN)) return "cuTensorMapEncodeTiled failed";
+  static std::atomic<int> granted[64];
+  const uint32_t smem = wide_smem(g.experts);
+  cudaError_t e = ensure_dynamic_smem(fp8_wide_kernel<T>, smem, granted);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kWideThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<T>, tm_x, tm_w, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? std::string() : std::string(cudaGetErrorString(e));
+}
+
+template <class T>
 std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
   const int sms = std::max(2, sm_count());
   RowsPlan r;
+  const int mean_rows = (g.M + g.experts - 1) / g.experts;
+  const int64_t wide_tiles = ((int64_t)g.M / kWideM + g.experts) * ((g.N + kWideN - 1) / kWideN);
+  if (mean_rows > 128 && wide_tiles >= sms / 2) return launch_wide_kernel<T>(g, (int)std::min<int64_t>(sms, wide_tiles), flags, stream);
   if (g.offsets) {
     const int64_t mean = (g.M + g.experts - 1) / g.experts;
     r = rows_plan(g.M, g.N, g.K, g.experts, mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128, 1, sms);

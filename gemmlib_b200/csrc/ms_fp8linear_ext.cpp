@@ -295,7 +295,7 @@ Tensor expert_linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, c
   TORCH_CHECK(x.dim() == 2, "fp8_expert_linear: the input must be [rows, in_features]");
   TORCH_CHECK(w.dim() == 3 && w.numel() > 0, "fp8_expert_linear: the weight must be [experts, out_features, in_features]");
   same_device("fp8_expert_linear: the weight", w, x);
-  TORCH_CHECK(w.size(0) <= 2048 && w.size(1) <= (1 << 28) && w.size(2) <= (1 << 28), "fp8_expert_linear: the weight is too large: ", w.sizes());
+  TORCH_CHECK(w.size(0) <= 1024 && w.size(1) <= (1 << 28) && w.size(2) <= (1 << 28), "fp8_expert_linear: the weight is too large: ", w.sizes());
   TORCH_CHECK(x.size(1) == w.size(2), "fp8_expert_linear: rows of ", x.size(1), " cannot be multiplied with weights of ", w.size(2),
               " in_features");
   TORCH_CHECK(is_stack(w), "fp8_expert_linear: the weight must have contiguous rows of one pitch, and experts behind one another");
@@ -335,7 +335,7 @@ Order sort_choices(const Tensor& experts, int64_t n_experts) {
   TORCH_CHECK(experts.scalar_type() == torch::kInt || experts.scalar_type() == torch::kLong,
               "sort_by_expert: the experts must be int32 or int64, instead got ", toString(experts.scalar_type()));
   TORCH_CHECK(experts.dim() >= 1 && experts.size(-1) > 0, "sort_by_expert: the experts must be [..., choices of a token]");
-  TORCH_CHECK(n_experts >= 1 && n_experts <= 2048, "sort_by_expert: 1 to 2048 experts are taken, not ", n_experts);
+  TORCH_CHECK(n_experts >= 1 && n_experts <= 1024, "sort_by_expert: 1 to 1024 experts are taken, not ", n_experts);
   const int64_t n = experts.numel();
   TORCH_CHECK(n <= (1 << 28), "sort_by_expert: too many choices: ", n);
   const c10::cuda::CUDAGuard guard(experts.device());

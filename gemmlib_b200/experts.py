@@ -46,7 +46,7 @@ torch.serialization.add_safe_globals([ExpertOrder])
 
 
 def sort_by_expert(experts: torch.Tensor, n_experts: int) -> ExpertOrder:
-    """The order of the choices ``experts`` [..., choices], for up to 2048 experts."""
+    """The order of the choices ``experts`` [..., choices], for up to 1024 experts."""
     return _sort(experts, n_experts)
 
 

@@ -486,7 +486,7 @@ int fp8_gemm_sm100(
  * The same for a layer of experts: rows [offsets[e], offsets[e + 1]) of x are multiplied with weight e of [experts, n, k] (w_stride bytes and
  * ws_stride floats from expert to expert).  offsets: experts + 1 int32 on the device, rising, within [0, rows]; the call does not wait for
  * them, and offsets that are none of these lead to no access out of bounds (a value is taken for the nearest that fits behind those before).
- * Rows of no expert are left as they are, or set to zero with FP8_EXPERTS_ZERO_REST.  Up to 2048 experts.
+ * Rows of no expert are left as they are, or set to zero with FP8_EXPERTS_ZERO_REST.  Up to 1024 experts.
  */
 #define FP8_EXPERTS_ZERO_REST 0x100u
 int fp8_experts_gemm_sm100(
@@ -507,7 +507,7 @@ int fp8_experts_gemm_sm100(
  *   source [tokens * choices]   the choice (token * choices + number) at each place; those of no expert come last
  *   places [tokens, choices]    the place of each choice, -1 for those of no expert
  * All int32.  workspace: of experts_sort_workspace_size bytes (0: may be null), free again once the call's work is done.
- * Up to 2048 experts and 2^28 choices.
+ * Up to 1024 experts and 2^28 choices.
  */
 size_t experts_sort_workspace_size(int64_t n, int n_experts);
 int experts_sort_sm100(

@@ -48,16 +48,18 @@ constexpr long long kWaitCycles = 4000000000ll;  // ~2 s: far beyond any legitim
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
   return mbar_wait_bounded(bar, parity, abort_flag, &g_fp8_error, who, kWaitCycles);
 }
-// `wait` of a whole warp, with one answer for all of it.
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int who) {
+// `wait` of a whole warp, with one answer for all of it.  abort_at: the flag's address in shared memory.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, uint32_t abort_at, int who) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const long long t0 = clock64();
   for (;;) {
     if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 1000u))) return true;
     const bool late = clock64() - t0 > kWaitCycles;
-    if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+    int given_up;
+    asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(given_up) : "r"(abort_at) : "memory");
+    if (__any_sync(0xffffffffu, late || given_up != 0)) {
       if (late) {
-        *abort_flag = 1;
+        asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(abort_at), "r"(1) : "memory");
         atomicCAS(&g_fp8_error, 0, who);
       }
       return false;
@@ -183,30 +185,38 @@ struct Params {
 };
 
 // ---- which tiles there are ----
-// begins[e]: first row of expert e (begins[experts]: the end); firsts[e]: number of tile rows of the experts before e.
+// begin(e): first row of expert e (begin(experts): the end); first(e): number of tile rows of the experts before e.  Shared memory, by addresses of
+// 32 bits: the sums leave few registers.
+__device__ __forceinline__ int lds(uint32_t at) {
+  int v;
+  asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts(uint32_t at, int v) { asm volatile("st.shared.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 struct Experts {
-  int* begins;
-  int* firsts;
+  uint32_t begins, firsts;
+  __device__ __forceinline__ int begin(int e) const { return lds(begins + 4u * (uint32_t)e); }
+  __device__ __forceinline__ int first(int e) const { return lds(firsts + 4u * (uint32_t)e); }
 };
 __host__ __device__ inline uint32_t experts_bytes(int experts) { return 8u * (uint32_t)(experts + 1); }
 // All threads of the CTA; behind griddep_wait where there are offsets.  `high`: rows of a tile.
 __device__ __forceinline__ void count_tiles(const Experts& t, const int* offsets, int experts, int rows, int high) {
   if (offsets == nullptr) {
     if (threadIdx.x == 0) {
-      t.begins[0] = 0, t.begins[1] = rows;
-      t.firsts[0] = 0, t.firsts[1] = (rows + high - 1) / high;
+      sts(t.begins, 0), sts(t.begins + 4u, rows);
+      sts(t.firsts, 0), sts(t.firsts + 4u, (rows + high - 1) / high);
     }
     __syncthreads();
     return;
   }
-  for (int e = threadIdx.x; e <= experts; e += blockDim.x) t.begins[e] = min(max(offsets[e], 0), rows);
+  for (int e = threadIdx.x; e <= experts; e += blockDim.x) sts(t.begins + 4u * (uint32_t)e, min(max(offsets[e], 0), rows));
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int top = 0, tiles = 0;  // of the experts before
     for (int e0 = 0; e0 <= experts; e0 += 32) {
       const int e = e0 + lane;
-      int v = max(top, e <= experts ? t.begins[e] : 0);
+      int v = max(top, e <= experts ? t.begin(e) : 0);
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, v, s);
@@ -222,8 +232,8 @@ __device__ __forceinline__ void count_tiles(const Experts& t, const int* offsets
         if (lane >= s) sum += o;
       }
       if (e <= experts) {
-        t.begins[e] = v;
-        t.firsts[e] = tiles + sum;
+        sts(t.begins + 4u * (uint32_t)e, v);
+        sts(t.firsts + 4u * (uint32_t)e, tiles + sum);
       }
       top = __shfl_sync(0xffffffffu, v, 31);
       tiles += __shfl_sync(0xffffffffu, sum, 31);
@@ -236,16 +246,16 @@ struct Walk {
   Experts t;
   int tile, step, count, n_tiles, e;
   __device__ __forceinline__ Walk(const Experts& t, int experts, int n_tiles, int first, int step)
-      : t(t), tile(first), step(step), count(t.firsts[experts] * n_tiles), n_tiles(n_tiles), e(0) {}
+      : t(t), tile(first), step(step), count(t.first(experts) * n_tiles), n_tiles(n_tiles), e(0) {}
   // `high` rows a tile: m0 .. end
   __device__ __forceinline__ bool next(int high, int& expert, int& n_tile, int& m0, int& end) {
     if (tile >= count) return false;
-    while (t.firsts[e + 1] * n_tiles <= tile) ++e;
-    const int m_tiles = t.firsts[e + 1] - t.firsts[e], in = tile - t.firsts[e] * n_tiles;
+    while (t.first(e + 1) * n_tiles <= tile) ++e;
+    const int m_tiles = t.first(e + 1) - t.first(e), in = tile - t.first(e) * n_tiles;
     n_tile = in / m_tiles;
     expert = e;
-    m0 = t.begins[e] + (in - n_tile * m_tiles) * high;
-    end = min(t.begins[e + 1], m0 + high);
+    m0 = t.begin(e) + (in - n_tile * m_tiles) * high;
+    end = min(t.begin(e + 1), m0 + high);
     tile += step;
     return true;
   }
@@ -253,9 +263,9 @@ struct Walk {
 // Rows of no expert, by some of the CTA's threads.
 template <class T>
 __device__ __forceinline__ void zero_rows(const Experts& t, int experts, int M, int N, T* out, int64_t ldo, int thread, int threads) {
-  const int first = t.begins[0], rest = M - t.begins[experts];
+  const int first = t.begin(0), behind = t.begin(experts), rest = M - behind;
   for (int i = blockIdx.x; i < first + rest; i += gridDim.x) {
-    uint16_t* row = reinterpret_cast<uint16_t*>(out) + (int64_t)(i < first ? i : t.begins[experts] + i - first) * ldo;
+    uint16_t* row = reinterpret_cast<uint16_t*>(out) + (int64_t)(i < first ? i : behind + i - first) * ldo;
     for (int n = thread; n < N; n += threads) row[n] = 0;
   }
 }
@@ -296,7 +306,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const uint32_t exchanged = bars + kWords;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + kWords + 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + kWords + 12);
-  const Experts table{reinterpret_cast<int*>(bars_ptr + kBarBytes), reinterpret_cast<int*>(bars_ptr + kBarBytes) + p.experts + 1};
+  const Experts table{bars + kBarBytes, bars + kBarBytes + 4u * (uint32_t)(p.experts + 1)};
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = (int)blockIdx.x % p.split, first_tile = (int)blockIdx.x / p.split, tile_step = (int)gridDim.x / p.split;
@@ -329,7 +339,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   tc::tc_fence_before();
   count_tiles(table, p.offsets, p.experts, p.M, BN);
   // of a split tile, the only one of its CTA
-  const int split_rows = p.split > 1 ? min(BN, p.M - first_tile % table.firsts[1] * BN) : BN;
+  const int split_rows = p.split > 1 ? min(BN, p.M - first_tile % table.first(1) * BN) : BN;
   const int first_row = min(split_rows, part * p.slice), end_row = min(split_rows, first_row + p.slice);  // whose sums end up here
   if (p.split > 1) {
     if (threadIdx.x == 0)

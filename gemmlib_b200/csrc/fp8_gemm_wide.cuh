@@ -12,8 +12,9 @@
 // instead of WIDE).
 #pragma once
 
-// Warps 0 to 3: weights, MMAs, activations, scales; the other two warpgroups: the sums, whose threads hold 128 of them.  So those take 224
-// registers and leave 56 to the first: 128 * 56 + 256 * 224 are the 384 * 168 that the block is launched with.
+// Warps 0 to 3: weights, MMAs, activations, scales; the other two warpgroups: the sums, whose threads hold 128 of them.  So those take 232
+// registers and leave 40 to the first: 128 * 40 + 256 * 232 are the 384 * 168 that the block is launched with.  (With fewer, a few are spilled to
+// local memory, which has next to no L1 beside this shared memory: a reload takes 300 cycles of a step's 600.)
 constexpr int kWideXWarp = 2, kWideScaleWarp = 3, kWideSumWarp = 4, kWideThreads = 32 * (kWideSumWarp + kEpiWarps);
 constexpr int kWideM = 128, kWideN = 256;
 constexpr uint32_t kWideXBytes = kWideM * kStepK, kWideStageBytes = kWideXBytes + kWideN * kStepK;
@@ -74,23 +75,27 @@ __device__ __forceinline__ void add_scaled2(float& a0, float& a1, uint32_t t0, u
 // rows of both operands in L2.
 struct WideWalk {
   Experts t;
-  int tile, step, count, n_tiles, e;
-  __device__ __forceinline__ WideWalk(const Experts& t, int experts, int n_tiles)
-      : t(t), tile((int)blockIdx.x), step((int)gridDim.x), count(t.firsts[experts] * n_tiles), n_tiles(n_tiles), e(0) {}
-  __device__ __forceinline__ bool next(int& expert, int& n_tile, int& m0, int& end) {
-    if (tile >= count) return false;
-    while (t.firsts[e + 1] * n_tiles <= tile) ++e;
+  int tile, e;
+  __device__ __forceinline__ explicit WideWalk(const Experts& t) : t(t), tile((int)blockIdx.x), e(0) {}
+  __device__ __forceinline__ bool next(int experts, int n_tiles, int& expert, int& n_tile, int& m0, int& end) {
+    if (tile >= t.first(experts) * n_tiles) return false;
+    while (t.first(e + 1) * n_tiles <= tile) ++e;
     constexpr int kBand = 16;
-    const int m_tiles = t.firsts[e + 1] - t.firsts[e], in = tile - t.firsts[e] * n_tiles;
+    const int m_tiles = t.first(e + 1) - t.first(e), in = tile - t.first(e) * n_tiles;
     const int band = in / (kBand * n_tiles), high = min(kBand, m_tiles - band * kBand), in_band = in - band * kBand * n_tiles;
     n_tile = in_band / high;
     expert = e;
-    m0 = t.begins[e] + (band * kBand + in_band - n_tile * high) * kWideM;
-    end = t.begins[e + 1];
-    tile += step;
+    m0 = t.begin(e) + (band * kBand + in_band - n_tile * high) * kWideM;
+    end = t.begin(e + 1);
+    tile += (int)gridDim.x;
     return true;
   }
 };
+__device__ __forceinline__ float4 lds4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
 
 template <class T>
 __global__ void __launch_bounds__(kWideThreads, 1)
@@ -110,8 +115,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   static_assert(kWords + 8 <= kBars + kWideBarBytes);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + kWords);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kWords + 4);
-  int* table_ptr = reinterpret_cast<int*>(base_ptr + kBars + kWideBarBytes);
-  const Experts table{table_ptr, table_ptr + p.experts + 1};
+  const Experts table{base + kBars + kWideBarBytes, base + kBars + kWideBarBytes + 4u * (uint32_t)(p.experts + 1)};
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -142,10 +146,10 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   int expert, n_tile, m0, end;
-  WideWalk walk(table, p.experts, p.n_tiles);
+  WideWalk walk(table);
 
   if (warp < kWideSumWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0 || warp == kWideXWarp) {
       // two producers, each with its operand
       if (elect_one()) {
@@ -161,7 +165,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           if (++s == kWideStages) s = 0, parity ^= 1u;
         };
         bool first = true;
-        while (walk.next(expert, n_tile, m0, end)) {
+        while (walk.next(p.experts, p.n_tiles, expert, n_tile, m0, end)) {
           int ks = 0;
           if (first) {
             first = false;
@@ -191,7 +195,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc | ((base >> 4) & 0x3FFFu);
         int s = 0, b = 0;
         uint32_t parity = 0, acc_parity = 1;
-        while (walk.next(expert, n_tile, m0, end)) {
+        while (walk.next(p.experts, p.n_tiles, expert, n_tile, m0, end)) {
           for (int ks = 0; ks < p.k_steps; ++ks) {
             if (!wait(full(s), parity, abort_flag, 0x1210 | s)) goto mma_done;
             if (!wait(acc_empty(b), acc_parity, abort_flag, 0x1200 | b)) goto mma_done;
@@ -208,37 +212,29 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
     } else {
       griddep_wait();
-      const int last_block = (p.N - 1) / kBlock;
       int s = 0;
       uint32_t parity = 1;
-      while (walk.next(expert, n_tile, m0, end)) {
-        const float* src[4];
-        bool in[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = m0 + lane + 32 * i;
-          in[i] = row < end;
-          src[i] = p.x_scales + (in[i] ? (int64_t)row * p.ldxs : 0);
-        }
-        const float* w_src = p.w_scales + expert * p.ws_stride + (int64_t)min(n_tile * (kWideN / kBlock) + lane / 4, last_block) * p.ldws;
+      while (walk.next(p.experts, p.n_tiles, expert, n_tile, m0, end)) {
         for (int ks = 0; ks < p.k_steps; ks += 4) {
           if (!wait(scale_empty(s), parity, abort_flag, 0x1120)) goto scales_done;
           const uint32_t dst = base + kSlots + (uint32_t)s * kWideSlotBytes;
           const int left = p.k_steps - ks;
-          if (p.scales_on_16 && left >= 4) {
+#pragma unroll 1
+          for (int i = lane; i < kWideM; i += 32) {
+            const bool in = m0 + i < end;
+            const float* src = p.x_scales + (in ? (int64_t)(m0 + i) * p.ldxs + ks : 0);
+            if (p.scales_on_16 && left >= 4) {
+              copy16(dst + (uint32_t)i * 16u, src, in ? 16u : 0u);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(dst + (uint32_t)(lane + 32 * i) * 16u, src[i] + (in[i] ? ks : 0), in[i] ? 16u : 0u);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              for (int q = 0; q < 4; ++q) {
-                const bool here = in[i] && q < left;
-                copy4(dst + (uint32_t)(lane + 32 * i) * 16u + 4u * (uint32_t)q, src[i] + (here ? ks + q : 0), here);
-              }
+              for (int q = 0; q < 4; ++q) copy4(dst + (uint32_t)i * 16u + 4u * (uint32_t)q, src + (in && q < left ? q : 0), in && q < left);
+            }
           }
           if (lane < 8) {
-            const bool here = lane % 4 < left;
-            copy4(dst + kWideM * 16u + (uint32_t)lane * 4u, w_src + (here ? ks + lane % 4 : 0), here);
+            const int block = min(n_tile * (kWideN / kBlock) + lane / 4, (p.N - 1) / kBlock);
+            const bool in = lane % 4 < left;
+            copy4(dst + kWideM * 16u + (uint32_t)lane * 4u,
+                  p.w_scales + expert * p.ws_stride + (int64_t)block * p.ldws + (in ? ks + lane % 4 : 0), in);
           }
           arrive_behind_copies(scale_full(s));
           if (++s == kWideSlots) s = 0, parity ^= 1u;
@@ -248,33 +244,30 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ---- sums and outputs: a warp has the 32 rows of its quarter of the lanes and half of the columns, in chunks of 32
     constexpr int kChunks = kWideChunks;
     const int quarter = warp & 3, half = (warp - kWideSumWarp) >> 2;
     const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kBlock);
-    uint8_t* stage = base_ptr + kOut + (warp - kWideSumWarp) * kWideChunkBytes;
-    T* out = reinterpret_cast<T*>(p.out);
     griddep_wait();
     int slot = 0, b = 0;
     uint32_t parity = 0, slot_parity = 0;
-    while (walk.next(expert, n_tile, m0, end)) {
-      const int n0 = n_tile * kWideN + half * kBlock, row0 = m0 + quarter * 32;
+    while (walk.next(p.experts, p.n_tiles, expert, n_tile, m0, end)) {
       float acc[kChunks][32];
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
 #pragma unroll
         for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
-      float x, w;  // the scales of the next step
-      auto next_scales = [&](int ks) {
-        if (ks % 4 == 0 && !wait_warp(scale_full(slot), slot_parity, abort_flag, 0x1310)) return false;
-        const float* scales = reinterpret_cast<const float*>(base_ptr + kSlots + slot * kWideSlotBytes) + ks % 4;
-        x = scales[(quarter * 32 + lane) * 4], w = scales[(kWideM + half) * 4];
-        if (ks % 4 == 3 || ks + 1 == p.k_steps) {
-          __syncwarp();
-          arrive_lane0(scale_empty(slot));
-          if (++slot == kWideSlots) slot = 0, slot_parity ^= 1u;
-        }
+      // The scales of four steps at once, and well ahead of their use: shared memory is busy with the MMAs' operands, and a load from it takes
+      // 250 to 500 cycles.
+      float4 x, w;
+      auto next_scales = [&] {
+        if (!wait_warp(scale_full(slot), slot_parity, base + kWords, 0x1310)) return false;
+        const uint32_t scales = base + kSlots + (uint32_t)slot * kWideSlotBytes;
+        x = lds4(scales + (uint32_t)(quarter * 32 + lane) * 16u), w = lds4(scales + (uint32_t)(kWideM + half) * 16u);
+        __syncwarp();
+        arrive_lane0(scale_empty(slot));
+        if (++slot == kWideSlots) slot = 0, slot_parity ^= 1u;
         return true;
       };
       uint32_t r[2][32];
@@ -283,16 +276,17 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < 32; j += 2) add_scaled2(acc[c][j], acc[c][j + 1], r[c % 2][j], r[c % 2][j + 1], s);
       };
-      if (!next_scales(0)) goto sums_done;
+#pragma unroll 1
       for (int ks = 0; ks < p.k_steps; ++ks) {
-        const float s = x * w;
-        const bool ok = wait_warp(acc_full(b), parity, abort_flag, 0x1300 | b);
-        if (!ok) goto sums_done;
+        if (ks % 4 == 0 && !next_scales()) goto sums_done;
+        if (!wait_warp(acc_full(b), parity, base + kWords, 0x1300)) goto sums_done;
         tc::tc_fence_after();
         load(0);
         load(1);
         tmem_ld_wait_for(r[0]);
         tmem_ld_wait_for(r[1]);
+        const float s = x.x * w.x;
+        x = make_float4(x.y, x.z, x.w, 0.0f), w = make_float4(w.y, w.z, w.w, 0.0f);
         add(0, s);
         load(2);
         add(1, s);
@@ -304,10 +298,12 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         __syncwarp();
         arrive_lane0(acc_empty(b));
         if (++b == 2) b = 0, parity ^= 1u;
-        if (ks + 1 < p.k_steps && !next_scales(ks + 1)) goto sums_done;
         add(2, s);
         add(3, s);
       }
+      const int n0 = n_tile * kWideN + half * kBlock, row0 = m0 + quarter * 32;
+      uint8_t* stage = base_ptr + kOut + (warp - kWideSumWarp) * kWideChunkBytes;
+      T* out = reinterpret_cast<T*>(p.out);
       // A lane has a row's outputs, 64 bytes a chunk, and stores them itself: whole sectors of 32 bytes where they begin on such.  ((What
       // goes by way of shared memory and TMA has to wait for the copy of the chunk before.)
 #pragma unroll
@@ -361,7 +357,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         }
       }
     }
-    if (p.zero_rest) zero_rows<T>(table, p.experts, p.M, p.N, out, p.ldo, (int)threadIdx.x - 32 * kWideSumWarp, 32 * kEpiWarps);
+    if (p.zero_rest) zero_rows<T>(table, p.experts, p.M, p.N, reinterpret_cast<T*>(p.out), p.ldo, (int)threadIdx.x - 32 * kWideSumWarp, 32 * kEpiWarps);
   sums_done:;
   }
   __syncwarp();

@@ -66,6 +66,7 @@ FP8_SYMBOLS = (
     "fp8_weight_dequant_sm100",
     "fp8_gemm_sm100",
     "fp8_experts_gemm_sm100",
+    "fp8_gemm_plan_sm100",
 )
 FP8_EXPERTS_ZERO_REST = 0x100
 EXPERTS_SYMBOLS = (
@@ -178,6 +179,7 @@ def _load() -> ctypes.CDLL:
     lib.fp8_gemm_sm100.argtypes = [i, i, i, i, vp, *matrix, *matrix, *matrix, *matrix, *vector, *matrix, ctypes.c_uint, vp]
     stacked = [*matrix, ctypes.c_int64]
     lib.fp8_experts_gemm_sm100.argtypes = [i, i, i, i, i, vp, *matrix, *matrix, *stacked, *stacked, *vector, *matrix, ctypes.c_uint, vp]
+    lib.fp8_gemm_plan_sm100.argtypes = [i, i, i, i, ctypes.POINTER(i)]
     lib.experts_sort_workspace_size.restype = ctypes.c_size_t
     lib.experts_sort_workspace_size.argtypes = [ctypes.c_int64, i]
     lib.experts_sort_sm100.argtypes = [ctypes.c_int64, i, i, vp, *vector, *vector, *vector, *vector, *vector, vp]
@@ -522,6 +524,15 @@ def fp8_gemm(dtype, m, n, k, x, x_scales, w, w_scales, bias, out, flags=0, strea
 def fp8_experts_gemm(dtype, experts, rows, n, k, x, x_scales, w, w_stride, w_scales, ws_stride, offsets, out, flags=0, stream=0):
     _int8_call(lib.fp8_experts_gemm_sm100, dtype, experts, rows, n, k, stream, *_matrix(x), *_matrix(x_scales), *_matrix(w), w_stride,
                *_matrix(w_scales), ws_stride, *_ptr_size(offsets), *_matrix(out), flags)
+
+
+def fp8_gemm_plan(m: int, n: int, k: int, experts: int = 0) -> dict:
+    """The work plan of ``fp8_gemm``, or of ``fp8_experts_gemm`` (host only; see fp8_gemm_plan_sm100)."""
+    out = (ctypes.c_int * 8)()
+    if lib.fp8_gemm_plan_sm100(experts, m, n, k, out) != 0:
+        raise BlkQ4Error(f"no plan for {m}x{n}x{k}, {experts} experts")
+    names = ("kernel", "tile_m", "tile_n", "split", "steps", "stages", "smem", "columns")
+    return {**dict(zip(names, out)), "kernel": ("few", "many")[out[0]]}
 
 
 def experts_sort(n, n_experts, id_bytes, ids, source, places, offsets, workspace=None, stream=0):

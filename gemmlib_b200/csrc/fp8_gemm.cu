@@ -198,7 +198,7 @@ struct Experts {
   __device__ __forceinline__ int begin(int e) const { return lds(begins + 4u * (uint32_t)e); }
   __device__ __forceinline__ int first(int e) const { return lds(firsts + 4u * (uint32_t)e); }
 };
-__host__ __device__ inline uint32_t experts_bytes(int experts) { return 8u * (uint32_t)(experts + 1); }
+__host__ __device__ constexpr uint32_t experts_bytes(int experts) { return 8u * (uint32_t)(experts + 1); }
 // All threads of the CTA; behind griddep_wait where there are offsets.  `high`: rows of a tile.
 __device__ __forceinline__ void count_tiles(const Experts& t, const int* offsets, int experts, int rows, int high) {
   if (offsets == nullptr) {
@@ -273,15 +273,17 @@ __device__ __forceinline__ void zero_rows(const Experts& t, int experts, int M, 
 constexpr int kMaxStages = 16, kMaxBuffers = 8, kScaleSlots = 8;
 constexpr int kEpiWarps = 8, kXWarp = 2 + kEpiWarps, kScaleWarp = kXWarp + 1, kRowsThreads = 32 * (kScaleWarp + 1);
 constexpr uint32_t kBarBytes = 1024;  // barriers, abort flag, TMEM address
+constexpr uint32_t kSmemAlone = 200u * 1024, kSmemOfTwo = 100u * 1024;  // stages and exchange of a CTA alone on its SM, of one of two
+__host__ __device__ constexpr uint32_t smem_room(int BN) { return BN <= 32 ? kSmemOfTwo : kSmemAlone; }
 
 template <int BN>
 struct RowsShape {
   static constexpr int kGroups = BN / 16;                 // of eight columns, of a warp
-  static constexpr int kBuffers = BN <= 64 ? 128 / BN : 2;  // accumulators
+  static constexpr int kBuffers = BN <= 32 ? 128 / BN : 256 / BN;  // accumulators
   static constexpr uint32_t kColumns = BN * kBuffers;
   static constexpr uint32_t kStageBytes = kWeightBytes + BN * kStepK;
   static constexpr uint32_t kScaleBytes = kScaleSlots * BN * 4;
-  static constexpr int kPerSm = BN <= 64 ? 2 : 1;
+  static constexpr int kPerSm = BN <= 32 ? 2 : 1;
 };
 
 // Grid: the tiles of a walk, or tiles * split CTAs, those of a tile a cluster.
@@ -302,8 +304,9 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   auto scale_full = [&](int s) { return bars + 16u * (uint32_t)(kMaxStages + kMaxBuffers + s); };
   auto scale_empty = [&](int s) { return bars + 16u * (uint32_t)(kMaxStages + kMaxBuffers + s) + 8u; };
   constexpr uint32_t kWords = 16u * (kMaxStages + kMaxBuffers + kScaleSlots);
-  static_assert(kWords + 16 <= kBarBytes);
+  static_assert(kWords + 16 <= kBarBytes && smem_room(BN) + S::kScaleBytes + kBarBytes + experts_bytes(kMaxExperts) + 1024 <= (BN <= 32 ? 113u : 227u) * 1024);
   const uint32_t exchanged = bars + kWords;
+  const uint32_t abort_at = bars + kWords + 8u;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + kWords + 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars_ptr + kWords + 12);
   const Experts table{bars + kBarBytes, bars + kBarBytes + 4u * (uint32_t)(p.experts + 1)};
@@ -471,11 +474,11 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[g][j] = 0.0f;
       float next = w_scale[0];
+#pragma unroll 1
       for (int ks = 0; ks < steps; ++ks) {
         const float ws = next;
         if (ks + 1 < steps) next = w_scale[ks + 1];
-        const bool ok = wait(scale_full(s), s_parity, abort_flag, 0x300) && wait(acc_full(b), b_parity, abort_flag, 0x310);
-        if (__any_sync(0xffffffffu, !ok)) goto sums_done;
+        if (!wait_warp(scale_full(s), s_parity, abort_at, 0x300) || !wait_warp(acc_full(b), b_parity, abort_at, 0x310)) goto sums_done;
         tc::tc_fence_after();
         constexpr int kAtOnce = S::kGroups < 4 ? S::kGroups : 4;
 #pragma unroll
@@ -592,44 +595,112 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 
 // ---- plans ----
 struct RowsPlan {
-  int BN, n_tiles, split, k_per_cta, slice, stages, ctas;
+  int BN, tiles, split, k_per_cta, slice, stages, ctas;
   uint32_t exchange_bytes, smem;
   float us;
 };
-constexpr uint32_t kSmemAlone = 200u * 1024, kSmemOfTwo = 100u * 1024;  // stages and exchange of a CTA alone on its SM, of one of two
 
-uint32_t stage_bytes(int BN) { return kWeightBytes + (uint32_t)BN * kStepK; }
+// CTAs that run at a time in clusters of `split`, one on an SM: a cluster lies within one GPC, so that clusters of three and more leave SMs over.
+int resident_ctas(int split, int sms) {
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  if (split == 1 || cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
+    cudaGetLastError();
+    return sms;
+  }
+  std::atomic<int>& slot = known[dev][split];
+  int ctas = slot.load(std::memory_order_relaxed);
+  if (ctas > 0) return ctas;
+  static std::atomic<int> granted[64];
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = kSmemAlone + 8192;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(sms * split));
+  int clusters = 0;
+  if (ensure_dynamic_smem(fp8_rows_kernel<__half, 64>, cfg.dynamicSmemBytes, granted) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, fp8_rows_kernel<__half, 64>, &cfg) != cudaSuccess || clusters <= 0) {
+    cudaGetLastError();
+    clusters = sms / split;
+  }
+  ctas = clusters * split;
+  slot.store(ctas, std::memory_order_relaxed);
+  return ctas;
+}
 
-RowsPlan rows_plan(int M, int N, int K, int experts, int BN, int split, int sms) {
+// The sizes of a problem as the plans see it: `groups` weights that have `M` rows each.
+struct Problem {
+  int M, N, K, groups, experts;
+  bool dense;
+  int64_t tile_rows(int high) const { return (int64_t)groups * ((M + high - 1) / high); }
+  // the call's bytes, us at a TB/s; more where few SMs ask for them
+  float bytes() const { return (float)groups * ((float)N * (float)K + (float)M * (float)K + 2.0f * (float)M * (float)N) * 1e-6f; }
+  static float few(int64_t ctas, int sms) { return ctas < sms ? 1.3f - 0.3f * (float)ctas / (float)sms : 1.0f; }
+};
+
+// Estimates, us.  Launch and latencies; as the sides of a right angle, the steps of the busiest CTA (with its tiles' outputs) and the call's
+// bytes; the exchange of split tiles; the beginning of further rounds.  Fitted to 2000 timings (M 1 to 2048, 300 x 300 to 28672 x 1024, every tile
+// height, K in 1 to 8 parts; graphs of calls whose weights come from HBM): 11 % rms off for the kernel of few rows, 7 % for the other, and the
+// choices by them are 0.7 % slower than the best of all that were timed.
+RowsPlan plan_tiles(const Problem& q, int BN, int split, int sms) {
   RowsPlan t{};
-  const int k_steps = (K + kStepK - 1) / kStepK;
+  const int k_steps = (q.K + kStepK - 1) / kStepK, per_sm = BN <= 32 ? 2 : 1, rows = std::min(q.M, BN);
   t.BN = BN;
-  t.n_tiles = (N + kTileN - 1) / kTileN;
   t.k_per_cta = (k_steps + split - 1) / split;
   t.split = (k_steps + t.k_per_cta - 1) / t.k_per_cta;
-  const int rows = std::min(M, BN);
   t.slice = t.split > 1 ? ((rows + t.split - 1) / t.split + 7) / 8 * 8 : BN;
   t.exchange_bytes = (uint32_t)(t.split - 1) * (uint32_t)t.slice * kTileN * 4;
-  const int per_sm = BN <= 64 ? 2 : 1;
-  const uint32_t room = per_sm == 2 ? kSmemOfTwo : kSmemAlone;
-  t.stages = t.exchange_bytes < room ? std::min<int>(kMaxStages, (int)((room - t.exchange_bytes) / stage_bytes(BN))) : 0;
-  const int64_t tiles = ((int64_t)M / BN + experts) * t.n_tiles;  // at most
-  t.ctas = experts > 1 || t.split == 1 ? (int)std::min<int64_t>(tiles, (int64_t)per_sm * sms) : (int)(((M + BN - 1) / BN) * (int64_t)t.n_tiles * t.split);
-  t.smem = (uint32_t)t.stages * stage_bytes(BN) + t.exchange_bytes + kScaleSlots * (uint32_t)BN * 4 + kBarBytes + experts_bytes(experts) + 1024;
-  t.smem = std::max(t.smem, BN <= 64 ? tc::kSmemOfFewColumns : tc::kSmemOfManyColumns);
+  const uint32_t stage_bytes = kWeightBytes + (uint32_t)BN * kStepK;
+  t.stages = t.exchange_bytes < smem_room(BN) ? std::min<int>(kMaxStages, (int)((smem_room(BN) - t.exchange_bytes) / stage_bytes)) : 0;
+  t.smem = std::max((uint32_t)t.stages * stage_bytes + t.exchange_bytes + kScaleSlots * (uint32_t)BN * 4 + kBarBytes + experts_bytes(q.experts) + 1024,
+                    BN <= 32 ? tc::kSmemOfFewColumns : tc::kSmemOfManyColumns);
+  const int64_t tiles = q.tile_rows(BN) * ((q.N + kTileN - 1) / kTileN), all = tiles * t.split;
+  const int64_t slots = (int64_t)per_sm * (t.split > 1 ? resident_ctas(t.split, sms) : sms), ctas = t.split > 1 ? all : std::min(all, slots);
+  const int64_t rounds = (all + (t.split > 1 ? slots : ctas) - 1) / (t.split > 1 ? slots : ctas);
+  const int together = (int)std::min<int64_t>(per_sm, (ctas + sms - 1) / sms);
+  t.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+  t.ctas = (int)std::min<int64_t>(ctas, INT32_MAX);
+  const float step = BN == 16 ? 0.22f * (float)together : BN == 32 ? std::max(0.296f, 0.201f * (float)together) : BN == 64 ? 0.294f : 0.47f;
+  const float run = (float)rounds * (step * (float)t.k_per_cta + 0.0217f * (float)rows / (float)t.split);
+  const float memory = q.bytes() / 7.4f * Problem::few(ctas, sms);
+  t.us = 2.3f + std::sqrt(run * run + memory * memory) + 4.17f * (float)(rounds - 1);
+  if (t.split > 1) t.us += 0.45f + 0.039f * (float)together * (float)(t.split - 1) / (float)t.split * (float)rows;
   return t;
 }
-RowsPlan plan_rows(int M, int N, int K, int sms) {
-  const int BN = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const int k_steps = (K + kStepK - 1) / kStepK;
-  const int64_t tiles = (int64_t)((M + BN - 1) / BN) * ((N + kTileN - 1) / kTileN);
-  RowsPlan best = rows_plan(M, N, K, 1, BN, 1, sms);
-  for (int split : {2, 3, 4, 6, 8}) {
-    if (split * 2 > k_steps || tiles * split > sms) break;
-    RowsPlan t = rows_plan(M, N, K, 1, BN, split, sms);
-    if (t.split == split && t.stages >= 3) best = t;
+float wide_us(const Problem& q, int sms) {
+  const int64_t tiles = q.tile_rows(kWideM) * ((q.N + kWideN - 1) / kWideN), rounds = (tiles + sms - 1) / sms;
+  const float run = (float)rounds * (0.373f * (float)((q.K + kStepK - 1) / kStepK) + 3.28f);
+  const float memory = q.bytes() / 7.6f * Problem::few(tiles, sms);
+  return 1.3f + std::sqrt(run * run + memory * memory);
+}
+
+struct Plan {
+  bool wide;
+  RowsPlan rows;  // if not
+};
+Plan plan_gemm(const Problem& q, int sms) {
+  Plan p{};
+  for (int BN : {16, 32, 64, 128}) {
+    if (BN > 16 && BN >= 2 * q.M) break;
+    for (int split : {1, 2, 3, 4, 6, 8}) {
+      const int64_t all = q.tile_rows(BN) * ((q.N + kTileN - 1) / kTileN) * split;
+      if (split > 1 && (!q.dense || split * 2 > (q.K + kStepK - 1) / kStepK || all > (BN <= 32 ? 2 : 1) * sms)) break;
+      const RowsPlan t = plan_tiles(q, BN, split, sms);
+      if (t.split == split && t.stages >= 3 && (p.rows.BN == 0 || t.us < p.rows.us)) p.rows = t;
+    }
   }
-  return best;
+  p.wide = q.M > 16 && wide_us(q, sms) < p.rows.us;
+  return p;
+}
+// Experts: the offsets are on the device, so the plan takes it that every expert has as many rows as another.
+Problem problem_of(int experts, int M, int N, int K, bool dense) {
+  const int used = std::min(experts, M);
+  return Problem{(M + used - 1) / used, N, K, used, experts, dense};
 }
 
 // ---- launches ----
@@ -662,7 +733,7 @@ std::string launch_rows_kernel(const GemmArgs& g, const RowsPlan& r, unsigned fl
   if (!encode_rows(&tm_x, g.x, g.ldx, g.K, g.M, BN) || !encode_weights(&tm_w, g, kTileN)) return "cuTensorMapEncodeTiled failed";
   Params p{};
   p.M = g.M; p.N = g.N;
-  p.n_tiles = r.n_tiles;
+  p.n_tiles = (g.N + kTileN - 1) / kTileN;
   p.k_steps = (g.K + kStepK - 1) / kStepK;
   p.experts = g.experts; p.offsets = g.offsets; p.zero_rest = g.zero_rest;
   p.split = r.split; p.k_per_cta = r.k_per_cta; p.slice = r.slice; p.stages = r.stages;
@@ -674,7 +745,7 @@ std::string launch_rows_kernel(const GemmArgs& g, const RowsPlan& r, unsigned fl
   p.w_scales = g.w_scales; p.ldws = g.ldws; p.ws_stride = g.ws_stride;
   p.bias = g.bias;
   static std::atomic<int> granted[64];
-  cudaError_t e = ensure_dynamic_smem(fp8_rows_kernel<T, BN>, std::max(r.smem, (BN <= 64 ? kSmemOfTwo : kSmemAlone) + 8192u), granted);
+  cudaError_t e = ensure_dynamic_smem(fp8_rows_kernel<T, BN>, r.smem, granted);
   if (e != cudaSuccess) return cudaGetErrorString(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)r.ctas);
@@ -733,16 +804,26 @@ std::string launch_wide_kernel(const GemmArgs& g, int ctas, unsigned flags, cuda
 template <class T>
 std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream) {
   const int sms = std::max(2, sm_count());
-  RowsPlan r;
-  const int mean_rows = (g.M + g.experts - 1) / g.experts;
-  const int64_t wide_tiles = ((int64_t)g.M / kWideM + g.experts) * ((g.N + kWideN - 1) / kWideN);
-  if (mean_rows > 128 && wide_tiles >= sms / 2) return launch_wide_kernel<T>(g, (int)std::min<int64_t>(sms, wide_tiles), flags, stream);
-  if (g.offsets) {
-    const int64_t mean = (g.M + g.experts - 1) / g.experts;
-    r = rows_plan(g.M, g.N, g.K, g.experts, mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128, 1, sms);
-  } else {
-    r = plan_rows(g.M, g.N, g.K, sms);
+  // the plan of the latest problem: a function of the sizes alone
+  struct Kept {
+    int M = 0, N = 0, K = 0, experts = 0, sms = 0;
+    bool dense = false;
+    Plan plan;
+  };
+  static thread_local Kept kept[16];
+  const bool dense = g.offsets == nullptr;
+  Kept& k = kept[((unsigned)g.M * 31u + (unsigned)g.N * 7u + (unsigned)g.K) / 8u % 16u];
+  if (k.M != g.M || k.N != g.N || k.K != g.K || k.experts != g.experts || k.dense != dense || k.sms != sms) {
+    k.plan = plan_gemm(problem_of(g.experts, g.M, g.N, g.K, dense), sms);
+    k.M = g.M, k.N = g.N, k.K = g.K, k.experts = g.experts, k.dense = dense, k.sms = sms;
   }
+  // as many CTAs as there may be tiles
+  const int high = k.plan.wide ? kWideM : k.plan.rows.BN, wide = k.plan.wide ? kWideN : kTileN;
+  const int64_t tiles = ((int64_t)g.M / high + g.experts) * ((g.N + wide - 1) / wide);
+  if (tiles > INT32_MAX) return "the problem has too many tiles";
+  if (k.plan.wide) return launch_wide_kernel<T>(g, (int)std::min<int64_t>(sms, tiles), flags, stream);
+  RowsPlan r = k.plan.rows;
+  if (r.split == 1) r.ctas = (int)std::min<int64_t>((int64_t)(r.BN <= 32 ? 2 : 1) * sms, tiles);
   switch (r.BN) {
     case 16: return launch_rows_kernel<T, 16>(g, r, flags, stream);
     case 32: return launch_rows_kernel<T, 32>(g, r, flags, stream);
@@ -769,3 +850,19 @@ int clear_gemm_error(cudaStream_t stream) {
 
 }  // namespace fp8
 }  // namespace blkq4
+
+extern "C" int fp8_gemm_plan_sm100(int experts, int m, int n, int k, int* out8) {
+  using namespace blkq4::fp8;
+  if (!out8 || m <= 0 || n <= 0 || k <= 0 || m > (1 << 28) || n > (1 << 28) || k > (1 << 28) || experts < 0 || experts > kMaxExperts) return -1;
+  const int sms = blkq4::sm_count() > 0 ? blkq4::sm_count() : 148;
+  const Plan p = plan_gemm(problem_of(std::max(1, experts), m, n, k, experts == 0), sms);
+  const int k_steps = (k + kStepK - 1) / kStepK;
+  if (p.wide) {
+    const int v[8] = {1, kWideM, kWideN, 1, k_steps, kWideStages, (int)wide_smem(std::max(1, experts)), 512};
+    std::copy(v, v + 8, out8);
+  } else {
+    const int v[8] = {0, p.rows.BN, kTileN, p.rows.split, p.rows.k_per_cta, p.rows.stages, (int)p.rows.smem, p.rows.BN <= 32 ? 128 : 256};
+    std::copy(v, v + 8, out8);
+  }
+  return 0;
+}

@@ -482,6 +482,11 @@ int fp8_gemm_sm100(
   unsigned flags,
   void* error_message);
 
+/* Host-only description of the work plan of fp8_gemm_sm100 (experts = 0) and fp8_experts_gemm_sm100 for operand rows that begin on 16 bytes (nothing
+ * is launched; 148 SMs are assumed without a device): out8[0] kernel (0 = few rows, 1 = many), [1] activation rows and [2] weight rows of a
+ * tile, [3] parts of K, [4] steps of 128 k a part, [5] stages, [6] bytes of shared memory, [7] columns of tensor memory. */
+int fp8_gemm_plan_sm100(int experts, int m, int n, int k, int* out8);
+
 /**
  * The same for a layer of experts: rows [offsets[e], offsets[e + 1]) of x are multiplied with weight e of [experts, n, k] (w_stride bytes and
  * ws_stride floats from expert to expert).  offsets: experts + 1 int32 on the device, rising, within [0, rows]; the call does not wait for

@@ -1,4 +1,5 @@
-"""B200-native blockwise-int4 weight-only GEMM/GEMV (W4A16), and an 8-bit path beside it (W8A8: ``int8_linear``).
+"""B200-native blockwise-int4 weight-only GEMM/GEMV (W4A16), and 8-bit paths beside it (W8A8: ``int8_linear``, ``fp8_linear``;
+layers of experts: ``experts``).
 
 The product is the C-ABI shared library ``libms_blkq4gemm.so`` (entry points
 declared in ``include/ms_blkq4gemm.h``) built from the CUDA sources in
@@ -13,7 +14,7 @@ before the library exists.
 """
 import importlib
 
-__all__ = ["capi", "build", "ms_blkq4linear", "ms_blkq4linear_ext", "sharded", "int8_linear", "stack"]
+__all__ = ["capi", "build", "ms_blkq4linear", "ms_blkq4linear_ext", "sharded", "int8_linear", "fp8_linear", "experts", "stack"]
 
 
 def __getattr__(name):

@@ -9,7 +9,8 @@ an output buffer, captures the whole pass once per row count M on its own stream
 replays it.  Inside the graph the skinny kernels are launched with
 ``BLKQ4_GEMM_EARLY_WEIGHT_FETCH``: the weights of layer i+1 stream in while layer i
 drains.  Consecutive layers that read the same buffer (q, k and v; gate and up) are one launch where a kernel
-takes them together with every bit of their own calls' results; ``Int8Linear`` layers that do share the int8 rows of the buffer.
+takes them together with every bit of their own calls' results; ``Int8Linear`` layers that do share the int8 rows of the buffer, and
+``Fp8Linear`` layers its e4m3 rows.
 
 It runs the linears only: what sits between them in a model (attention, activation
 functions, norms) is the caller's and can be captured into the same graph by passing
@@ -21,6 +22,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .fp8_linear import Fp8Linear, Fp8Rows, quantize_fp8
 from .int8_linear import Int8Linear, Int8Rows, RMSNormInt8, quantize_int8, silu_mul_int8
 from .ms_blkq4linear import MAX_GROUP, BlkQ4Linear, can_share_launch, group_workspace_bytes, run_as_one, shares_launch, workspaces_owned_by
 
@@ -33,18 +35,23 @@ class LinearStack:
 
     ``int8_inputs``: step -> what makes the int8 rows that this step's ``Int8Linear`` multiplies, from the buffers: a norm
     (which may write the residual's buffer), a gated activation.  Int8 steps without an entry quantize the buffer they read; those that follow
-    one another and read the same buffer share its rows.
+    one another and read the same buffer share its rows.  ``fp8_inputs``: the same for the e4m3 rows of ``Fp8Linear`` steps.
     """
 
-    def __init__(self, steps: Sequence[Tuple[BlkQ4Linear | Int8Linear, str, str]],
+    def __init__(self, steps: Sequence[Tuple[BlkQ4Linear | Int8Linear | Fp8Linear, str, str]],
                  between: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], None]]] = None,
-                 int8_inputs: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], Int8Rows]]] = None):
+                 int8_inputs: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], Int8Rows]]] = None,
+                 fp8_inputs: Optional[Dict[int, Callable[[Dict[str, torch.Tensor]], Fp8Rows]]] = None):
         self.steps = list(steps)
         self.between = dict(between or {})
         self.int8_inputs = dict(int8_inputs or {})
         for i in self.int8_inputs:
             if not 0 <= i < len(self.steps) or not isinstance(self.steps[i][0], Int8Linear):
                 raise ValueError(f"int8_inputs names step {i}, which has no Int8Linear")
+        self.fp8_inputs = dict(fp8_inputs or {})
+        for i in self.fp8_inputs:
+            if not 0 <= i < len(self.steps) or not isinstance(self.steps[i][0], Fp8Linear):
+                raise ValueError(f"fp8_inputs names step {i}, which has no Fp8Linear")
         self._graphs: Dict[int, Tuple[torch.cuda.CUDAGraph, Dict[str, torch.Tensor]]] = {}
         self._split_k: Dict[int, dict] = {}  # row count -> split-K workspaces of its graph
         self.device = self.steps[0][0].q_weights.device
@@ -94,19 +101,20 @@ class LinearStack:
         return launches
 
     def _run_eager(self, bufs, launches):
-        held = None  # the buffer that was quantized last and its rows, as long as nothing may have written it
+        held = None  # the buffer that was quantized last, how, and its rows, as long as nothing may have written it
         for run in launches:
             members = [self.steps[i] for i in run]
             lyr, src, dst = members[0]
             if len(members) > 1:
                 run_as_one([lyr for lyr, _, _ in members], bufs[src], [bufs[dst] for _, _, dst in members])
-            elif isinstance(lyr, Int8Linear):
-                make = self.int8_inputs.get(run[0])
+            elif isinstance(lyr, (Int8Linear, Fp8Linear)):
+                fp8 = isinstance(lyr, Fp8Linear)
+                make = (self.fp8_inputs if fp8 else self.int8_inputs).get(run[0])
                 if make is not None:
-                    held = src, make(bufs)
-                elif held is None or held[0] != src:
-                    held = src, quantize_int8(bufs[src])
-                lyr(held[1], out=bufs[dst])
+                    held = src, fp8, make(bufs)
+                elif held is None or held[:2] != (src, fp8):
+                    held = src, fp8, (quantize_fp8 if fp8 else quantize_int8)(bufs[src])
+                lyr(held[2], out=bufs[dst])
             else:
                 lyr(bufs[src], out=bufs[dst])
             hook = self.between.get(run[-1])
@@ -165,7 +173,7 @@ class LinearStack:
         return len(self.steps)
 
     def weight_bytes(self) -> int:
-        return sum(l.weight_bytes() if isinstance(l, Int8Linear) else
+        return sum(l.weight_bytes() if isinstance(l, (Int8Linear, Fp8Linear)) else
                    l.q_weights.numel() + 2 * l.q_scales.numel() + l.q_zp.numel() for l, _, _ in self.steps)
 
 

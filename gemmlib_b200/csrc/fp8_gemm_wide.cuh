@@ -97,6 +97,19 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
   return v;
 }
 
+// Two lanes that differ in one bit (BIT) of their number: the one without it keeps a and gets the other's a for its b; the one with it keeps b and
+// gets the other's b for its a.
+template <int BIT>
+__device__ __forceinline__ void trade(uint32_t (&a)[8], uint32_t (&b)[8], int lane) {
+  const bool has = lane & BIT;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, has ? a[j] : b[j], BIT);
+    a[j] = has ? got : a[j];
+    b[j] = has ? b[j] : got;
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kWideThreads, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const WideParams p) {
@@ -304,40 +317,57 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       const int n0 = n_tile * kWideN + half * kBlock, row0 = m0 + quarter * 32;
       uint8_t* stage = base_ptr + kOut + (warp - kWideSumWarp) * kWideChunkBytes;
       T* out = reinterpret_cast<T*>(p.out);
-      // A lane has a row's outputs, 64 bytes a chunk, and stores them itself: whole sectors of 32 bytes where they begin on such.  ((What
-      // goes by way of shared memory and TMA has to wait for the copy of the chunk before.)
+      if (p.bias) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int n = n0 + 32 * c, row = row0 + lane;
-        if (p.bias) {
-          const float mine = n + lane < p.N ? to_float(reinterpret_cast<const T*>(p.bias)[n + lane]) : 0.0f;
+        for (int c = 0; c < kChunks; ++c) {
+          const float mine = n0 + 32 * c + lane < p.N ? to_float(reinterpret_cast<const T*>(p.bias)[n0 + 32 * c + lane]) : 0.0f;
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[c][j] += __shfl_sync(0xffffffffu, mine, j);
         }
-        uint32_t v[16];
+      }
+      if (p.vector > 1) {
+        // A lane has a row's outputs.  Stored as they are, 32 bytes a lane, an instruction would touch 32 lines, one a cycle, and a tile's
+        // outputs take 2000 cycles, for which the MMAs have to wait.  So four lanes trade first: of 64 columns each gets a quarter, of its
+        // own row and of the three others'; an instruction then stores whole lines of eight rows.
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = pack2<T>(acc[c][2 * j], acc[c][2 * j + 1]);
-        if (p.vector > 1) {
-          T* at = out + (int64_t)row * p.ldo + n;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (row >= end || n + 16 * q >= p.N) continue;
-            const uint32_t* from = v + 8 * q;
-            if (p.vector == 16) {  // N is a multiple of it
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at + 16 * q), "r"(from[0]), "r"(from[1]),
-                           "r"(from[2]), "r"(from[3]), "r"(from[4]), "r"(from[5]), "r"(from[6]), "r"(from[7])
-                           : "memory");
-            } else {
-              *reinterpret_cast<uint4*>(at + 16 * q) = make_uint4(from[0], from[1], from[2], from[3]);
-              if (n + 16 * q + 8 < p.N) *reinterpret_cast<uint4*>(at + 16 * q + 8) = make_uint4(from[4], from[5], from[6], from[7]);
-            }
-          }
-        } else {
-          // rows that begin anywhere: through a block of the warp's own, so that neighbouring lanes have neighbouring outputs of a row
+        for (int c = 0; c < kChunks; c += 2) {
+          uint32_t v[4][8];  // 16 columns each
 #pragma unroll
           for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[q][j] = pack2<T>(acc[c + q / 2][16 * (q % 2) + 2 * j], acc[c + q / 2][16 * (q % 2) + 2 * j + 1]);
+          trade<1>(v[0], v[1], lane);
+          trade<1>(v[2], v[3], lane);
+          trade<2>(v[0], v[2], lane);
+          trade<2>(v[1], v[3], lane);
+          const int n = n0 + 32 * c + 16 * (lane & 3), row = row0 + (lane & ~3);
+          T* at = out + (int64_t)row * p.ldo + n;
+          if (n < p.N) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q, at += p.ldo) {
+              if (row + q >= end) continue;
+              if (p.vector == 16) {  // N is a multiple of it
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[q][0]), "r"(v[q][1]), "r"(v[q][2]),
+                             "r"(v[q][3]), "r"(v[q][4]), "r"(v[q][5]), "r"(v[q][6]), "r"(v[q][7])
+                             : "memory");
+              } else {
+                *reinterpret_cast<uint4*>(at) = make_uint4(v[q][0], v[q][1], v[q][2], v[q][3]);
+                if (n + 8 < p.N) *reinterpret_cast<uint4*>(at + 8) = make_uint4(v[q][4], v[q][5], v[q][6], v[q][7]);
+              }
+            }
+          }
+        }
+      } else {
+        // rows that begin anywhere: through a block of the warp's own, so that neighbouring lanes have neighbouring outputs of a row
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int n = n0 + 32 * c;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float* a = acc[c] + 8 * q;
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
-                make_uint4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+                make_uint4(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(a[4], a[5]), pack2<T>(a[6], a[7]));
+          }
           __syncwarp();
           T* at = out + (int64_t)row0 * p.ldo + n + lane;
           const uint8_t* from[4];  // the lane's output in rows of each place of its piece

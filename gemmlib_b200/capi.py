@@ -495,8 +495,8 @@ def fp8_rows_quant(dtype, rows, cols, x, values, scales, stream=0):
     _int8_call(lib.fp8_rows_quant_sm100, dtype, rows, cols, stream, *_matrix(x), *_matrix(values), *_matrix(scales))
 
 
-def fp8_rows_gather_quant(dtype, tokens, choices, cols, x, source, count, values, scales, stream=0):
-    _int8_call(lib.fp8_rows_gather_quant_sm100, dtype, tokens, choices, cols, stream, *_matrix(x), *_ptr_size(source), count,
+def fp8_rows_gather_quant(dtype, tokens, choices, cols, x, places, count, values, scales, stream=0):
+    _int8_call(lib.fp8_rows_gather_quant_sm100, dtype, tokens, choices, cols, stream, *_matrix(x), *_ptr_size(places), count,
                *_matrix(values), *_matrix(scales))
 
 

@@ -1,10 +1,10 @@
 // Tokens sorted by expert and back: the order of the choices, the rows of each expert behind one another, the weighted sum of a token's
 // rows, and the gradients of both moves.
 //
-// Sort: a stable counting sort.  Every warp has a run of choices and a counter for each expert in shared memory; it counts its run, the counters
-// become the places where its choices of an expert begin (behind those of the experts, the CTAs and the warps before), and it goes through
-// the run again, 32 choices at a time, the lanes of one expert ranked by a match.  Stable since runs, steps and lanes follow the choices'
-// order; no atomic decides a place.  Up to 8192 choices are one CTA's; more are split over CTAs, whose counts a kernel before writes.
+// Sort: a stable counting sort.  Every warp has a run of choices and a counter for each expert in shared memory; it goes through its run 32
+// choices at a time, the lanes of one expert ranked by a match, and counts; then the counters become the places where its choices of an expert
+// begin (behind those of the experts, the CTAs and the warps before), and each choice's place is that and its rank.  Stable since runs, steps
+// and lanes follow the choices' order; no atomic decides a place.  Up to 8192 choices are one CTA's; more are split over CTAs, whose counts a kernel before writes.
 //
 // Moves: bound by HBM and L2, 16 bytes a lane, a warp a stretch of a row.  The weighted sum is gathered (a token reads its rows, in the order
 // of its choices, fp32), not scattered: no atomics, one rounding, the same result every time.  The gradient of the weighted sum reads y and the
@@ -29,6 +29,7 @@ using namespace blkq4::int8;
 // ---- sort ----
 constexpr int kMaxWarps = 32;
 constexpr int64_t kOneCta = 8192;
+constexpr int kItems = 8;  // choices of a lane that are under way at a time
 
 template <class Id>
 __device__ __forceinline__ int key_of(const Id* ids, int64_t i, int n_experts) {
@@ -62,7 +63,28 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Id* ids, int64_t n, in
   __syncthreads();
   const int64_t run = chunk / warps, begin = (int64_t)blockIdx.x * chunk + warp * run, end = min(n, begin + run);
   int* mine = cells + warp * width;
-  for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&mine[key_of(ids, i, n_experts)], 1);
+  // 32 choices at a time: how many of a choice's expert are ahead of it in the run, by a match of the lanes and the counter so far
+  auto take = [&](bool in, int key) {
+    const unsigned same = __match_any_sync(0xffffffffu, key);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    const int ahead = in ? mine[key] : 0;
+    __syncwarp();
+    if (in && rank == 0) mine[key] = ahead + __popc(same);
+    __syncwarp();
+    return ahead + rank;
+  };
+  int keys[kItems], ahead[kItems];
+  auto load = [&](int64_t i0) {
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) keys[t] = i0 + 32 * t + lane < end ? key_of(ids, i0 + 32 * t + lane, n_experts) : width;
+  };
+  const bool held = run <= 32 * kItems;  // the run stays in registers between its two passes
+  for (int64_t i0 = begin; i0 < end; i0 += 32 * kItems) {
+    load(i0);
+#pragma unroll
+    for (int t = 0; t < kItems; ++t)
+      if (i0 + 32 * t < end) ahead[t] = take(keys[t] < width, keys[t]);
+  }
   __syncthreads();
   int carry = 0;
   for (int e0 = 0; e0 < width; e0 += blockDim.x) {  // places of e0 + thread: behind all choices of the experts before
@@ -103,20 +125,18 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Id* ids, int64_t n, in
     }
     __syncthreads();
   }
-  for (int64_t i0 = begin; i0 < end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const bool in = i < end;
-    const int key = in ? key_of(ids, i, n_experts) : width;
-    const unsigned same = __match_any_sync(0xffffffffu, key);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    if (in) {
-      const int place = mine[key] + rank;
+  for (int64_t i0 = begin; i0 < end; i0 += 32 * kItems) {
+    if (!held) load(i0);
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      const int64_t i = i0 + 32 * t + lane;
+      if (i0 + 32 * t >= end) break;
+      const bool in = keys[t] < width;
+      const int place = held ? (in ? mine[keys[t]] + ahead[t] : 0) : take(in, keys[t]);
+      if (!in) continue;
       source[place] = (int)i;
-      places[i] = key < n_experts ? place : -1;
+      places[i] = keys[t] < n_experts ? place : -1;
     }
-    __syncwarp();
-    if (in && rank == 0) mine[key] += __popc(same);
-    __syncwarp();
   }
 }
 
@@ -296,7 +316,7 @@ SortPlan plan_sort(int64_t n, int n_experts) {
   } else {
     s.warps = most;
     const int64_t step = 32 * s.warps;
-    s.chunk = std::max<int64_t>(4 * step, ((n + 147) / 148 + step - 1) / step * step);
+    s.chunk = std::max<int64_t>(2 * step, ((n + 147) / 148 + step - 1) / step * step);
     s.ctas = (n + s.chunk - 1) / s.chunk;
   }
   return s;

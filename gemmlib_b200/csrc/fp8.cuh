@@ -20,9 +20,9 @@ constexpr int kMaxExperts = 1024;
 struct RowsParams {
   const void* a;      // x, or gate
   const void* b;      // up
-  const int* source;  // row p is made from row source[p] / choices of x; null: from row p
-  const int* count;   // with source: how many rows there are, the others are zero
-  int choices, x_rows;
+  const int* places;  // [rows, choices]: the rows of q that row r of x is written to; null: row r
+  const int* count;   // with places: how many rows of q are written so, the others are set to zero
+  int choices;
   uint8_t* q;
   float* scales;
   int64_t lda, ldb, ldq, lds;  // elements from row to row

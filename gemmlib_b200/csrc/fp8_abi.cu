@@ -73,7 +73,7 @@ extern "C" int fp8_rows_quant_sm100(int dtype, int rows, int cols, void* stream,
 }
 
 extern "C" int fp8_rows_gather_quant_sm100(int dtype, int tokens, int choices, int cols, void* stream, void const* x, size_t x_size,
-                                           int64_t ldx, void const* source, size_t source_size, void const* count, void* values,
+                                           int64_t ldx, void const* places, size_t places_size, void const* count, void* values,
                                            size_t values_size, int64_t ldv, void* scales, size_t scales_size, int64_t lds, void* err) {
   const int rows = tokens > 0 && choices > 0 && (int64_t)tokens * choices <= kMaxRows ? tokens * choices : 0;
   return guarded(
@@ -82,7 +82,7 @@ extern "C" int fp8_rows_gather_quant_sm100(int dtype, int tokens, int choices, i
         std::string e = check_choices(dtype, tokens, choices, cols);
         if (e.empty())
           e = check_all({{"x", x, x_size, ldx, tokens, cols, 2},
-                         {"source", source, source_size, rows, 1, rows, 4},
+                         {"places", places, places_size, rows, 1, rows, 4},
                          {"values", values, values_size, ldv, rows, cols, 1},
                          {"scales", scales, scales_size, lds, rows, blocks_of(cols), 4}});
         return e.empty() ? check_count(count) : e;
@@ -91,15 +91,14 @@ extern "C" int fp8_rows_gather_quant_sm100(int dtype, int tokens, int choices, i
         blkq4::fp8::RowsParams p{};
         p.a = x;
         p.lda = pitch_of(ldx, tokens, cols);
-        p.x_rows = tokens;
         p.choices = choices;
-        p.source = reinterpret_cast<const int*>(source);
+        p.places = reinterpret_cast<const int*>(places);
         p.count = reinterpret_cast<const int*>(count);
         p.q = reinterpret_cast<uint8_t*>(values);
         p.ldq = pitch_of(ldv, rows, cols);
         p.scales = reinterpret_cast<float*>(scales);
         p.lds = pitch_of(lds, rows, blocks_of(cols));
-        p.rows = rows;
+        p.rows = tokens;
         p.cols = cols;
         return blkq4::fp8::launch_rows(blkq4::fp8::kQuant, Dtype(dtype), p, reinterpret_cast<cudaStream_t>(stream));
       });

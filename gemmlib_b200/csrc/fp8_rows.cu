@@ -134,25 +134,25 @@ __device__ __forceinline__ Part part_of(int parts, int U) {
   return p;
 }
 
-template <int OP, class T, bool VEC, bool GATHER, int U>
+// SCATTER: a row is written to the places of its choices, so that it is read and converted once, whatever their number; the rows behind the
+// last place are set to zero by all half-warps in turn.
+template <int OP, class T, bool VEC, bool SCATTER, int U>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int parts, bool q_vec) {
   griddep_wait();
   griddep_launch_dependents();
   const Part at = part_of(parts, U);
   const int lane = threadIdx.x & 15;
-  bool in = at.row < p.rows;
-  int64_t from = at.row;
-  if (GATHER && in) {
-    from = at.row < *p.count ? p.source[at.row] / p.choices : -1;
-    if (from >= p.x_rows) from = -1;  // (of an order that is none)
-  }
+  const bool in = at.row < p.rows;
+  const int places = SCATTER ? p.rows * p.choices : 0;
+  int first_zero = places;
+  if constexpr (SCATTER) first_zero = max(0, *p.count);
   uint32_t a[U][4] = {}, b[U][4] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int chunk = (at.block + u) * 16 + lane;
-    if (in && from >= 0 && chunk * 8 < p.cols) {
-      load8<T, VEC, OP == kSiluMul ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + from * p.lda, chunk, p.cols, a[u]);
-      if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.b) + from * p.ldb, chunk, p.cols, b[u]);
+    if (in && chunk * 8 < p.cols) {
+      load8<T, VEC, OP == kSiluMul ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + at.row * p.lda, chunk, p.cols, a[u]);
+      if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.b) + at.row * p.ldb, chunk, p.cols, b[u]);
     }
   }
 #pragma unroll
@@ -169,9 +169,29 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
     }
     top = half_warp_max(top);
     if (!in || chunk * 8 >= p.cols) continue;
-    const Scale s = scale_of(top);
-    store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, convert8<OP == kQuant>(s, v));
-    if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale_value(top);
+    const uint2 q = convert8<OP == kQuant>(scale_of(top), v);
+    if constexpr (SCATTER) {
+      const float scale = scale_value(top);
+      for (int j = 0; j < p.choices; ++j) {
+        const int place = p.places[at.row * p.choices + j];
+        if (place < 0 || place >= places) continue;  // of no expert (or of an order that is none)
+        store_q8(p.q + place * p.ldq, q_vec, chunk, p.cols, q);
+        if (lane == 0) p.scales[place * p.lds + at.block + u] = scale;
+      }
+    } else {
+      store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, q);
+      if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale_value(top);
+    }
+  }
+  if constexpr (SCATTER) {
+    const int64_t halves = (int64_t)gridDim.x * (kThreads / 16), blocks = (p.cols + kBlock - 1) / kBlock;
+    const int64_t end = ((int64_t)places - first_zero) * blocks;
+    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); i < end; i += halves) {
+      const int64_t row = first_zero + i / blocks;
+      const int block = (int)(i % blocks), chunk = block * 16 + lane;
+      if (chunk * 8 < p.cols) store_q8(p.q + row * p.ldq, q_vec, chunk, p.cols, make_uint2(0u, 0u));
+      if (lane == 0) p.scales[row * p.lds + block] = 0.0f;
+    }
   }
 }
 
@@ -288,14 +308,14 @@ int blocks_at_a_time(int rows, int cols) {
   const int most = blocks_of(cols);
   return blocks >= 8 * 148 * 16 && most >= 4 ? 4 : blocks >= 4 * 148 * 16 && most >= 2 ? 2 : 1;
 }
-template <int OP, class T, bool VEC, bool GATHER>
+template <int OP, class T, bool VEC, bool SCATTER>
 std::string launch_rows_u(const RowsParams& p, cudaStream_t stream) {
   const int U = blocks_at_a_time(p.rows, p.cols), parts = (blocks_of(p.cols) + U - 1) / U;
   const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
-  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8);
-  if (U == 4) return launch(rows_kernel<OP, T, VEC, GATHER, 4>, ctas, kThreads, stream, p, parts, q_vec);
-  if (U == 2) return launch(rows_kernel<OP, T, VEC, GATHER, 2>, ctas, kThreads, stream, p, parts, q_vec);
-  return launch(rows_kernel<OP, T, VEC, GATHER, 1>, ctas, kThreads, stream, p, parts, q_vec);
+  const bool q_vec = rows_on(p.q, p.ldq, SCATTER ? p.rows * p.choices : p.rows, 8);
+  if (U == 4) return launch(rows_kernel<OP, T, VEC, SCATTER, 4>, ctas, kThreads, stream, p, parts, q_vec);
+  if (U == 2) return launch(rows_kernel<OP, T, VEC, SCATTER, 2>, ctas, kThreads, stream, p, parts, q_vec);
+  return launch(rows_kernel<OP, T, VEC, SCATTER, 1>, ctas, kThreads, stream, p, parts, q_vec);
 }
 template <class T>
 std::string launch_rows_t(RowsOp op, const RowsParams& p, cudaStream_t stream) {
@@ -303,11 +323,8 @@ std::string launch_rows_t(RowsOp op, const RowsParams& p, cudaStream_t stream) {
     const bool vec = rows_on(p.a, p.lda * 2, p.rows, 16) && rows_on(p.b, p.ldb * 2, p.rows, 16);
     return vec ? launch_rows_u<kSiluMul, T, true, false>(p, stream) : launch_rows_u<kSiluMul, T, false, false>(p, stream);
   }
-  if (p.source) {
-    const bool vec = rows_on(p.a, p.lda * 2, p.x_rows, 16);
-    return vec ? launch_rows_u<kQuant, T, true, true>(p, stream) : launch_rows_u<kQuant, T, false, true>(p, stream);
-  }
   const bool vec = rows_on(p.a, p.lda * 2, p.rows, 16);
+  if (p.places) return vec ? launch_rows_u<kQuant, T, true, true>(p, stream) : launch_rows_u<kQuant, T, false, true>(p, stream);
   return vec ? launch_rows_u<kQuant, T, true, false>(p, stream) : launch_rows_u<kQuant, T, false, false>(p, stream);
 }
 template <class T>

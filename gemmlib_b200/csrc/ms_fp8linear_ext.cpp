@@ -93,7 +93,7 @@ Fp8Out quantize(const Tensor& x, const Tensor* source, const Tensor* places, con
   Fp8Out o = rows_like(sizes, order.rows, x.device());
   if (order.rows == 0) return o;
   TORCH_CHECK(fp8_rows_gather_quant_sm100(dtype, a.rows, int(order.choices), a.cols, current_stream(), a.data, a.bytes, a.ld,
-                                          order.source.data_ptr(), order.source.nbytes(), order.count, o.values.data_ptr(), o.bytes, o.ld,
+                                          order.places.data_ptr(), order.places.nbytes(), order.count, o.values.data_ptr(), o.bytes, o.ld,
                                           o.scales.data_ptr(), o.scale_bytes, o.lds, &err) == 0,
               err);
   return o;

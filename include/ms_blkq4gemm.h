@@ -425,11 +425,11 @@ int fp8_rows_quant_sm100(
   void* scales, size_t scales_size, int64_t lds,
   void* error_message);
 
-/** The same of the rows that experts_gather_sm100 would write, [tokens * choices, cols], without writing those. */
+/** The same of the rows that experts_gather_sm100 would write, [tokens * choices, cols], without writing those: row t of x goes to rows places[t, j]. */
 int fp8_rows_gather_quant_sm100(
   int dtype, int tokens, int choices, int cols, void* stream,
   void const* x, size_t x_size, int64_t ldx,
-  void const* source, size_t source_size, void const* count,
+  void const* places, size_t places_size, void const* count,
   void* values, size_t values_size, int64_t ldv,
   void* scales, size_t scales_size, int64_t lds,
   void* error_message);

@@ -222,11 +222,13 @@ def test_refusals():
     ]:
         with pytest.raises(RuntimeError, match=text):
             call()
-    # an order of the caller's own that names no token: no access out of bounds, zero rows
+    # an order of the caller's own that names no token or place: no access out of bounds
     wrong = order._replace(source=torch.full_like(order.source, 1 << 30))
-    assert (gather_rows(p["x"], wrong) == 0).all() and (quantize_fp8(p["x"], wrong).values.float() == 0).all()
-    wrong = order._replace(places=torch.full_like(order.places, 1 << 30))
-    assert (combine_rows(p["y"], wrong, p["weights"]) == 0).all()
+    assert (gather_rows(p["x"], wrong) == 0).all()
+    for far in (1 << 30, -(1 << 30), 20):
+        wrong = order._replace(places=torch.full_like(order.places, far))
+        assert (combine_rows(p["y"], wrong, p["weights"]) == 0).all()
+        assert quantize_fp8(p["x"], wrong).values.shape == (20, 64)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

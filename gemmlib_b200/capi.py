@@ -532,7 +532,7 @@ def fp8_gemm_plan(m: int, n: int, k: int, experts: int = 0) -> dict:
     if lib.fp8_gemm_plan_sm100(experts, m, n, k, out) != 0:
         raise BlkQ4Error(f"no plan for {m}x{n}x{k}, {experts} experts")
     names = ("kernel", "tile_m", "tile_n", "split", "steps", "stages", "smem", "columns")
-    return {**dict(zip(names, out)), "kernel": ("few", "many")[out[0]]}
+    return {**dict(zip(names, out)), "kernel": ("few", "many", "stream")[out[0]]}
 
 
 def experts_sort(n, n_experts, id_bytes, ids, source, places, offsets, workspace=None, stream=0):

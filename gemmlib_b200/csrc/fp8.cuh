@@ -61,6 +61,9 @@ struct GemmArgs {
   const int* offsets;  // null: all rows are those of one weight
   bool zero_rest;      // rows of no expert are set to zero
 };
+// The kernel of one or two rows, and the problems it is for (without offsets).
+bool gemv_takes(int M, int N, int K);
+std::string launch_gemv(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream);
 std::string launch_gemm(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream);
 int read_gemm_error();
 int clear_gemm_error(cudaStream_t stream);

@@ -835,6 +835,7 @@ std::string launch_typed(const GemmArgs& g, unsigned flags, cudaStream_t stream)
 }  // namespace
 
 std::string launch_gemm(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream) {
+  if (!g.offsets && gemv_takes(g.M, g.N, g.K)) return launch_gemv(dtype, g, flags, stream);
   return dtype == kFp16 ? launch_typed<__half>(g, flags, stream) : launch_typed<__nv_bfloat16>(g, flags, stream);
 }
 
@@ -854,6 +855,11 @@ int clear_gemm_error(cudaStream_t stream) {
 extern "C" int fp8_gemm_plan_sm100(int experts, int m, int n, int k, int* out8) {
   using namespace blkq4::fp8;
   if (!out8 || m <= 0 || n <= 0 || k <= 0 || m > (1 << 28) || n > (1 << 28) || k > (1 << 28) || experts < 0 || experts > kMaxExperts) return -1;
+  for (int i = 0; i < 8; ++i) out8[i] = 0;
+  if (experts == 0 && blkq4::fp8::gemv_takes(m, n, k)) {
+    out8[0] = 2;
+    return 0;
+  }
   const int sms = blkq4::sm_count() > 0 ? blkq4::sm_count() : 148;
   const Plan p = plan_gemm(problem_of(std::max(1, experts), m, n, k, experts == 0), sms);
   const int k_steps = (k + kStepK - 1) / kStepK;

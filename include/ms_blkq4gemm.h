@@ -483,7 +483,8 @@ int fp8_gemm_sm100(
   void* error_message);
 
 /* Host-only description of the work plan of fp8_gemm_sm100 (experts = 0) and fp8_experts_gemm_sm100 for operand rows that begin on 16 bytes (nothing
- * is launched; 148 SMs are assumed without a device): out8[0] kernel (0 = few rows, 1 = many), [1] activation rows and [2] weight rows of a
+ * is launched; 148 SMs are assumed without a device): out8[0] kernel (0 = few rows, 1 = many, 2 = weights streamed
+ * through registers), and for kernels 0 and 1 [1] activation rows and [2] weight rows of a
  * tile, [3] parts of K, [4] steps of 128 k a part, [5] stages, [6] bytes of shared memory, [7] columns of tensor memory. */
 int fp8_gemm_plan_sm100(int experts, int m, int n, int k, int* out8);
 

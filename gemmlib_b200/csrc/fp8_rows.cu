@@ -10,8 +10,8 @@
 //
 // Halves: 16-bit inputs often stand exactly half-way between two e4m3 numbers (wherever max|t| is a multiple of 7, for one), and the rounded
 // factor 448 / max|t| would put them to one side.  The quotient 448 x / max of numbers of 11 bits is either half-way between two numbers of 4
-// bits or at least 2^-16 of itself away from it (the difference is a fraction of integers over max times a number of 5 bits), so the product,
-// which is off by less than 2^-21, is rounded to 18 bits first: what is half-way lies there then, and nothing else does.
+// bits or at least 2^-16 of itself away from it (the difference is a fraction of integers over max times a number of 5 bits).  So the product,
+// which is off by less than 2^-21, is made a little too large and cut to 18 bits first: what is half-way lies there then, and nothing else does.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,46 +29,64 @@ using namespace blkq4::int8;
 
 constexpr int kThreads = 128;
 
-// What a block's largest |t| (its bits) says.
+// What a block's largest |t| (its bits) says.  `up`: blocks whose factor is no float are moved by 2^64 first.
 struct Scale {
-  bool finite;
-  float up, inverse;
+  float inverse, up;
+  bool plain;  // finite, and up is 1
 };
-__device__ __forceinline__ Scale scale_of(uint32_t top) {
-  Scale s;
-  // A block with an infinity or NaN has no scale that its other values could be told by: it is NaN as a whole.
-  s.finite = top < 0x7f800000u;
-  const float amax = s.finite ? __uint_as_float(top) : 0.0f;
-  // 448 / amax is no float below 2^-119, and its approximation is none beyond 2^126: such blocks are moved by 2^64 first
-  s.up = amax < 0x1p-64f ? 0x1p64f : amax > 0x1p64f ? 0x1p-64f : 1.0f;
-  s.inverse = amax > 0.0f ? __fdividef(448.0f, amax * s.up) : 0.0f;
-  return s;
-}
-__device__ __forceinline__ float scale_value(uint32_t top) {
-  return top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 448.0f) : __uint_as_float(0x7fc00000u);
-}
-// v rounded to 18 bits, half up: between there and a number of 4 bits no other rounding can come.
-__device__ __forceinline__ float to_18_bits(float v) { return __uint_as_float((__float_as_uint(v) + 0x20u) & 0xffffffc0u); }
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+__device__ __forceinline__ float reciprocal(float v) {  // 2^-23 off, of 2^-125 to 2^125
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-template <bool SHORT>  // t are 16-bit numbers
+// SHORT: t are 16-bit numbers; the factor is 2^-20 too large for them (see short_of).
+template <bool SHORT>
+__device__ __forceinline__ Scale scale_of(uint32_t top) {
+  constexpr float kTop = SHORT ? 448.0f * (1.0f + 0x1p-20f) : 448.0f;
+  Scale s;
+  s.plain = top - 0x20000000u < 0x40000000u;  // 2^-63 .. 2^65
+  s.up = 1.0f;
+  if (s.plain) {
+    s.inverse = kTop * reciprocal(__uint_as_float(top));
+  } else {
+    // A block with an infinity or NaN has no scale that its other values could be told by: it is NaN as a whole, with zeros for values.  448 / max
+    // is no float below 2^-119, and the reciprocal none beyond 2^126.
+    const float amax = top < 0x7f800000u ? __uint_as_float(top) : 0.0f;
+    s.up = top >= 0x7f800000u ? 0.0f : amax < 1.0f ? 0x1p64f : 0x1p-64f;
+    s.inverse = amax > 0.0f ? kTop * reciprocal(amax * s.up) : 0.0f;
+  }
+  return s;
+}
+// max / 448, rounded once: the quotient by the rounded reciprocal, put right by its remainder.
+__device__ __forceinline__ float scale_value(uint32_t top) {
+  const float amax = __uint_as_float(top);
+  if (top - 0x20000000u >= 0x40000000u) return top < 0x7f800000u ? __fdiv_rn(amax, 448.0f) : __uint_as_float(0x7fc00000u);
+  constexpr float kInverse = 1.0f / 448.0f;
+  const float q = amax * kInverse;
+  return fmaf(fmaf(-448.0f, q, amax), kInverse, q);
+}
+// v * (1 + 2^-20), give or take 2^-21, cut to 18 bits: what is half-way between two e4m3 numbers (a number of 5 bits) becomes just that; what is not
+// is at least 2^-16 away and stays on its side.
+__device__ __forceinline__ float short_of(float v) { return __uint_as_float(__float_as_uint(v) & 0xffffffc0u); }
+__device__ __forceinline__ uint32_t e4m3x4(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+  return r;
+}
+template <bool SHORT>
 __device__ __forceinline__ uint2 convert8(const Scale& s, float (&v)[8]) {
-  if (!s.finite || s.up != 1.0f) {
+  if (!s.plain) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = s.finite ? v[e] * s.up : 0.0f;
+    for (int e = 0; e < 8; ++e) v[e] = s.up > 0.0f ? v[e] * s.up : 0.0f;
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     v[e] *= s.inverse;
-    if (SHORT) v[e] = to_18_bits(v[e]);
+    if (SHORT) v[e] = short_of(v[e]);
   }
-  uint2 o;
-  o.x = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
-  o.y = e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16;
-  return o;
+  return make_uint2(e4m3x4(v), e4m3x4(v + 4));
 }
 // Rows of 8-bit values: 8 of them, `chunk` times 8 behind the beginning of the row.
 __device__ __forceinline__ void store_q8(uint8_t* row, bool vec, int chunk, int cols, uint2 o) {
@@ -136,7 +154,8 @@ __device__ __forceinline__ Part part_of(int parts, int U) {
 
 // SCATTER: a row is written to the places of its choices, so that it is read and converted once, whatever their number; the rows behind the
 // last place are set to zero by all half-warps in turn.
-template <int OP, class T, bool VEC, bool SCATTER, int U>
+// ONCE: large inputs make room in L2 for what is written (16000 x 2752 25.6 -> 24.7 us); others are kept, since they may be read again.
+template <int OP, class T, bool VEC, bool SCATTER, int U, bool ONCE>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int parts, bool q_vec) {
   griddep_wait();
   griddep_launch_dependents();
@@ -151,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
   for (int u = 0; u < U; ++u) {
     const int chunk = (at.block + u) * 16 + lane;
     if (in && chunk * 8 < p.cols) {
-      load8<T, VEC, OP == kSiluMul ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + at.row * p.lda, chunk, p.cols, a[u]);
+      load8<T, VEC, OP == kSiluMul || ONCE ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + at.row * p.lda, chunk, p.cols, a[u]);
       if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.b) + at.row * p.ldb, chunk, p.cols, b[u]);
     }
   }
@@ -169,9 +188,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
     }
     top = half_warp_max(top);
     if (!in || chunk * 8 >= p.cols) continue;
-    const uint2 q = convert8<OP == kQuant>(scale_of(top), v);
+    const uint2 q = convert8<OP == kQuant>(scale_of<OP == kQuant>(top), v);
+    const float scale = scale_value(top);
     if constexpr (SCATTER) {
-      const float scale = scale_value(top);
       for (int j = 0; j < p.choices; ++j) {
         const int place = p.places[at.row * p.choices + j];
         if (place < 0 || place >= places) continue;  // of no expert (or of an order that is none)
@@ -180,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
       }
     } else {
       store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, q);
-      if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale_value(top);
+      if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale;
     }
   }
   if constexpr (SCATTER) {
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const RowsParam
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWeightThreads / 32; ++i) top = max(top, tops[i]);
-  const Scale s = scale_of(top);
+  const Scale s = scale_of<true>(top);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (!in_cols || n0 + 16 * i >= p.expert_rows) continue;
@@ -234,9 +253,10 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const RowsParam
   if (threadIdx.x == 0) p.scales[(expert * n_blocks + nb) * p.lds + kb] = scale_value(top);
 }
 
-// out = scale * values
-template <class T, bool WEIGHTS, int U>
-__global__ void __launch_bounds__(kThreads) dequant_kernel(const DequantParams p, int parts, bool q_vec, bool out_vec) {
+// out = scale * values.  Rows of the output that begin anywhere are written by 16 aligned bytes, whose values lie in two pieces of 8 and may have
+// two scales.
+template <class T, bool WEIGHTS, bool VEC, int U>
+__global__ void __launch_bounds__(kThreads) dequant_kernel(const DequantParams p, int parts, bool q_vec) {
   griddep_wait();
   griddep_launch_dependents();
   const Part at = part_of(parts, U);
@@ -247,38 +267,51 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(const DequantParams p
     scale_row = expert * n_blocks + (at.row - expert * p.expert_rows) / kBlock;
   }
   const uint8_t* q = p.q + at.row * p.ldq;
+  const float* scales = p.scales + scale_row * p.lds;
   T* out = reinterpret_cast<T*>(p.out) + at.row * p.ldo;
-  uint2 r[U];
-  float scale[U];
+  const int before = VEC ? 0 : (int)(reinterpret_cast<uintptr_t>(out) & 15u) / 2;  // elements that the row's first 16 bytes lack
+  const uint32_t shift = (uint32_t)(8 - before) % 8u * 8u;                         // bits of q to drop from the 16 bytes it is read by
+  const int last = (p.cols - 1) / kBlock;
+  uint64_t v[U];
+  float s0[U], s1[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int chunk = (at.block + u) * 16 + (threadIdx.x & 15);
-    r[u] = make_uint2(0u, 0u);
-    if (chunk * 8 >= p.cols) continue;
-    scale[u] = p.scales[scale_row * p.lds + at.block + u];
-    if (q_vec && chunk * 8 + 8 <= p.cols) {
-      r[u] = *reinterpret_cast<const uint2*>(q + (int64_t)chunk * 8);
+    const int c = (at.block + u) * 16 + (threadIdx.x & 15), k0 = c * 8 - before;
+    v[u] = 0, s0[u] = s1[u] = 0.0f;
+    if (k0 >= p.cols) continue;
+    s0[u] = scales[max(k0, 0) / kBlock];
+    s1[u] = VEC ? s0[u] : scales[min((k0 + 7) / kBlock, last)];
+    if (q_vec && k0 >= 0 && c * 8 + 8 <= p.cols) {
+      const uint64_t hi = *reinterpret_cast<const uint64_t*>(q + (int64_t)c * 8);
+      if (VEC || before == 0) v[u] = hi;
+      else v[u] = *reinterpret_cast<const uint64_t*>(q + (int64_t)(c - 1) * 8) >> shift | hi << (64u - shift);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (chunk * 8 + e < p.cols) (e < 4 ? r[u].x : r[u].y) |= (uint32_t)q[(int64_t)chunk * 8 + e] << (e % 4 * 8);
+        if (k0 + e >= 0 && k0 + e < p.cols) v[u] |= (uint64_t)q[(int64_t)k0 + e] << (e * 8);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int chunk = (at.block + u) * 16 + (threadIdx.x & 15);
-    if (chunk * 8 >= p.cols) continue;
+    const int c = (at.block + u) * 16 + (threadIdx.x & 15), k0 = c * 8 - before;
+    if (k0 >= p.cols) continue;
+    const int turn = VEC || k0 < 0 ? 8 : kBlock - (k0 & (kBlock - 1));  // elements of the first scale, from k0 on
     uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = (i < 2 ? r[u].x : r[u].y) >> (i % 2 * 16);
       uint32_t h;  // e4m3 is exact in fp16
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)w));
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(v[u] >> (16 * i))));
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      o[i] = pack2<T>(f.x * scale[u], f.y * scale[u]);
+      o[i] = pack2<T>(f.x * (2 * i < turn ? s0[u] : s1[u]), f.y * (2 * i + 1 < turn ? s0[u] : s1[u]));
     }
-    if (out_vec) store8<T, true>(out, chunk, p.cols, o);
-    else store8<T, false>(out, chunk, p.cols, o);
+    if (k0 >= 0 && k0 + 8 <= p.cols) {
+      *reinterpret_cast<uint4*>(out + (int64_t)k0) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      uint16_t* one = reinterpret_cast<uint16_t*>(out) + (int64_t)k0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k0 + e >= 0 && k0 + e < p.cols) one[e] = (uint16_t)(o[e / 2] >> (e % 2 * 16));
+    }
   }
 }
 
@@ -313,9 +346,12 @@ std::string launch_rows_u(const RowsParams& p, cudaStream_t stream) {
   const int U = blocks_at_a_time(p.rows, p.cols), parts = (blocks_of(p.cols) + U - 1) / U;
   const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
   const bool q_vec = rows_on(p.q, p.ldq, SCATTER ? p.rows * p.choices : p.rows, 8);
-  if (U == 4) return launch(rows_kernel<OP, T, VEC, SCATTER, 4>, ctas, kThreads, stream, p, parts, q_vec);
-  if (U == 2) return launch(rows_kernel<OP, T, VEC, SCATTER, 2>, ctas, kThreads, stream, p, parts, q_vec);
-  return launch(rows_kernel<OP, T, VEC, SCATTER, 1>, ctas, kThreads, stream, p, parts, q_vec);
+  if constexpr (OP == kQuant && VEC && !SCATTER) {
+    if (U == 4 && (int64_t)p.rows * p.cols * 2 > (32 << 20)) return launch(rows_kernel<OP, T, VEC, SCATTER, 4, true>, ctas, kThreads, stream, p, parts, q_vec);
+  }
+  if (U == 4) return launch(rows_kernel<OP, T, VEC, SCATTER, 4, false>, ctas, kThreads, stream, p, parts, q_vec);
+  if (U == 2) return launch(rows_kernel<OP, T, VEC, SCATTER, 2, false>, ctas, kThreads, stream, p, parts, q_vec);
+  return launch(rows_kernel<OP, T, VEC, SCATTER, 1, false>, ctas, kThreads, stream, p, parts, q_vec);
 }
 template <class T>
 std::string launch_rows_t(RowsOp op, const RowsParams& p, cudaStream_t stream) {
@@ -335,14 +371,19 @@ std::string launch_weights_t(const RowsParams& p, cudaStream_t stream) {
   return rows_on(p.a, p.lda * 2, p.rows, 16) ? launch(weights_kernel<T, true>, ctas, kWeightThreads, stream, p, k_blocks, n_blocks, q_vec)
                                              : launch(weights_kernel<T, false>, ctas, kWeightThreads, stream, p, k_blocks, n_blocks, q_vec);
 }
+template <class T, bool WEIGHTS, bool VEC>
+std::string launch_dequant_u(const DequantParams& p, cudaStream_t stream) {
+  // (outputs that begin inside 16 bytes: up to 7 elements more)
+  const int U = blocks_at_a_time(p.rows, p.cols), blocks = blocks_of(p.cols + (VEC ? 0 : 7)), parts = (blocks + U - 1) / U;
+  const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
+  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8);
+  if (U == 4) return launch(dequant_kernel<T, WEIGHTS, VEC, 4>, ctas, kThreads, stream, p, parts, q_vec);
+  if (U == 2) return launch(dequant_kernel<T, WEIGHTS, VEC, 2>, ctas, kThreads, stream, p, parts, q_vec);
+  return launch(dequant_kernel<T, WEIGHTS, VEC, 1>, ctas, kThreads, stream, p, parts, q_vec);
+}
 template <class T, bool WEIGHTS>
 std::string launch_dequant_t(const DequantParams& p, cudaStream_t stream) {
-  const int U = blocks_at_a_time(p.rows, p.cols), parts = (blocks_of(p.cols) + U - 1) / U;
-  const int64_t ctas = ((int64_t)p.rows * parts + kThreads / 16 - 1) / (kThreads / 16);
-  const bool q_vec = rows_on(p.q, p.ldq, p.rows, 8), out_vec = rows_on(p.out, p.ldo * 2, p.rows, 16);
-  if (U == 4) return launch(dequant_kernel<T, WEIGHTS, 4>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
-  if (U == 2) return launch(dequant_kernel<T, WEIGHTS, 2>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
-  return launch(dequant_kernel<T, WEIGHTS, 1>, ctas, kThreads, stream, p, parts, q_vec, out_vec);
+  return rows_on(p.out, p.ldo * 2, p.rows, 16) ? launch_dequant_u<T, WEIGHTS, true>(p, stream) : launch_dequant_u<T, WEIGHTS, false>(p, stream);
 }
 
 }  // namespace

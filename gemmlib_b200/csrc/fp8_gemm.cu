@@ -286,6 +286,11 @@ struct RowsShape {
   static constexpr int kPerSm = BN <= 32 ? 2 : 1;
 };
 
+// The most that a plan asks for: what a kernel is allowed, once a device.  (Every caller allows the same, since a call replaces what one before allowed.)
+__host__ __device__ constexpr uint32_t rows_most_smem(int BN) {
+  return smem_room(BN) + (uint32_t)kScaleSlots * (uint32_t)BN * 4 + kBarBytes + experts_bytes(kMaxExperts) + 1024;
+}
+
 // Grid: the tiles of a walk, or tiles * split CTAs, those of a tile a cluster.
 template <class T, int BN>
 __global__ void __launch_bounds__(kRowsThreads, RowsShape<BN>::kPerSm)
@@ -304,7 +309,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   auto scale_full = [&](int s) { return bars + 16u * (uint32_t)(kMaxStages + kMaxBuffers + s); };
   auto scale_empty = [&](int s) { return bars + 16u * (uint32_t)(kMaxStages + kMaxBuffers + s) + 8u; };
   constexpr uint32_t kWords = 16u * (kMaxStages + kMaxBuffers + kScaleSlots);
-  static_assert(kWords + 16 <= kBarBytes && smem_room(BN) + S::kScaleBytes + kBarBytes + experts_bytes(kMaxExperts) + 1024 <= (BN <= 32 ? 113u : 227u) * 1024);
+  static_assert(kWords + 16 <= kBarBytes && rows_most_smem(BN) <= (BN <= 32 ? 113u : 227u) * 1024);
   const uint32_t exchanged = bars + kWords;
   const uint32_t abort_at = bars + kWords + 8u;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars_ptr + kWords + 8);
@@ -614,7 +619,7 @@ int resident_ctas(int split, int sms) {
   static std::atomic<int> granted[64];
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kRowsThreads);
-  cfg.dynamicSmemBytes = kSmemAlone + 8192;
+  cfg.dynamicSmemBytes = rows_most_smem(64);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split;
@@ -745,7 +750,7 @@ std::string launch_rows_kernel(const GemmArgs& g, const RowsPlan& r, unsigned fl
   p.w_scales = g.w_scales; p.ldws = g.ldws; p.ws_stride = g.ws_stride;
   p.bias = g.bias;
   static std::atomic<int> granted[64];
-  cudaError_t e = ensure_dynamic_smem(fp8_rows_kernel<T, BN>, r.smem, granted);
+  cudaError_t e = ensure_dynamic_smem(fp8_rows_kernel<T, BN>, rows_most_smem(BN), granted);
   if (e != cudaSuccess) return cudaGetErrorString(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)r.ctas);

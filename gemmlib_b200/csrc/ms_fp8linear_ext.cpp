@@ -2,6 +2,8 @@
 // byte sizes and leading dimensions, and handed to the fp8_* and experts_* calls of the C ABI on PyTorch's current stream.
 #include "ext_tensors.h"
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+
 namespace {
 
 using namespace ext_tensors;
@@ -437,6 +439,19 @@ std::pair<Tensor, Tensor> combine_backward(const Tensor& d, const Tensor& y, con
   return {d_y, d_weights};
 }
 
+// While a graph is captured: a leaf whose node for its gradient was made on another stream, and lives because an eager graph of the leaf does, makes
+// the backward pass wait for that stream, which ends the capture with an error that is not one to go on after.  Refused while it can be.
+void check_captured_leaf(const Tensor& x) {
+  if (!x.is_cuda() || !x.requires_grad() || !x.is_leaf()) return;
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
+  const c10::Stream now = c10::cuda::getCurrentCUDAStream();
+  TORCH_CHECK(!node || !node->stream().has_value() || *node->stream() == now,
+              "An eager graph of a tensor that requires a gradient lives on another stream than the one that is captured: delete it (its outputs) first, or "
+              "make it on this stream");
+}
+
 // ---- the calls' arguments, by position ----
 // Fp8Rows, Fp8Weight and ExpertOrder, named tuples of the Python modules: made here, since their own constructors are Python functions.
 PyTypeObject* g_types[3] = {};
@@ -560,7 +575,15 @@ PyObject* py_combine_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_check_captured_leaves(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < nargs; ++i) check_captured_leaf(tensor(args[i], "experts_check_captured_leaves"));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"experts_check_captured_leaves", fast<py_check_captured_leaves>(), METH_FASTCALL, "Refuses leaves whose backward pass a capture would not outlive"},
     {"fp8_types", fast<py_types>(), METH_FASTCALL, "The tuple's subclasses that rows, weights and orders are returned as"},
     {"fp8_quantize", fast<py_quantize>(), METH_FASTCALL, "The rows of x in e4m3, in the order of their experts where one is given"},
     {"fp8_quantize_weight", fast<py_quantize_weight>(), METH_FASTCALL, "Weights in e4m3, a scale for each 128 x 128"},

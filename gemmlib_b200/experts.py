@@ -9,7 +9,9 @@ expert that is none of 0 .. n_experts - 1 (-1 for padding, or another GPU's expe
     out = combine_rows(y, order, weights)       # [..., features]
 
 ``gather_rows`` and ``combine_rows`` have a backward pass (of one order).  All sums are float32, taken in the order of a token's choices, and
-rounded once; nothing depends on the order of atomics.  Offsets stay on the device: no call waits for the GPU, and all of them can be captured.
+rounded once; nothing depends on the order of atomics.  Offsets stay on the device: no call waits for the GPU, and all of them can be captured, with
+their backward pass (not while an eager graph of the same leaves lives on another stream: autograd would make the capture wait for it; such a
+call is refused).
 """
 from __future__ import annotations
 
@@ -27,6 +29,7 @@ _gather = ms_blkq4linear_ext.experts_gather
 _combine = ms_blkq4linear_ext.experts_combine
 _combine_backward = ms_blkq4linear_ext.experts_combine_backward
 _expert_linear = ms_blkq4linear_ext.fp8_expert_linear
+_check_captured_leaves = ms_blkq4linear_ext.experts_check_captured_leaves
 
 
 class ExpertOrder(NamedTuple):
@@ -81,6 +84,7 @@ def gather_rows(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The row of ``x`` [..., features] (float16 or bfloat16) of every choice, in the order's places: [n, features]; zeros behind
     ``order.offsets[-1]``.  A token's gradient is the sum of its rows'."""
     if x.requires_grad and torch.is_grad_enabled():
+        _check_captured_leaves(x)
         return _Gather.apply(x, *order)
     return _gather(x, *order)
 
@@ -89,6 +93,7 @@ def combine_rows(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor) -> 
     """The sum of each token's rows of ``y`` [n, features], with ``weights`` (float32, float16 or bfloat16) of the shape of ``order.places``:
     [..., features], in the type of ``y``.  What stands behind ``order.offsets[-1]`` is not read."""
     if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
+        _check_captured_leaves(y, weights)
         return _Combine.apply(y, weights, *order)
     return _combine(y, *order, weights)
 

@@ -419,3 +419,152 @@ def test_a_captured_backward_pass():
         torch.cuda.synchronize()
         want = step(new[0], new[1].requires_grad_(), new[2].requires_grad_(), new[3])
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_tokens():
+    from gemmlib_b200.experts import combine_rows, gather_rows, sort_by_expert
+    from gemmlib_b200.fp8_linear import quantize_fp8
+
+    m = layer(3, 64, 32, torch.float16, 1)
+    x, ids, weights = (torch.empty(0, n, device="cuda") for n in (64, 2, 2))
+    x, ids = x.half().requires_grad_(), ids.long()
+    order = sort_by_expert(ids, 3)
+    rows, out = gather_rows(x, order), combine_rows(torch.empty(0, 64, dtype=torch.float16, device="cuda"), order, weights.requires_grad_())
+    assert rows.shape == (0, 64) and out.shape == (0, 64) and quantize_fp8(x.detach(), order).values.shape == (0, 64)
+    grads = torch.autograd.grad((rows, out), (x, weights), (torch.empty_like(rows), torch.empty_like(out)))
+    assert grads[0].shape == (0, 64) and grads[1].shape == (0, 2)
+    assert m(x.detach(), ids, weights.detach()).shape == (0, 64)
+
+
+def test_products_of_many_experts_after_products_of_split_tiles():
+    """What a kernel may have of shared memory is the most that any call asks for, whichever came first."""
+    from gemmlib_b200.experts import fp8_expert_linear
+    from gemmlib_b200.fp8_linear import fp8_linear
+
+    for m in (16, 30, 60, 100):  # split tiles of every height
+        x, w = rows_of(m, 4096, 1), weight_of(512, 4096, 2)
+        check_close(fp8_linear(x, w), x, w)
+    w = stack_of(1024, 40, 64, 2)
+    for each in (1, 20, 40, 80):
+        offsets = torch.arange(0, 1025 * each, each, device="cuda").int()
+        x = rows_of(1024 * each, 64, 1)
+        out = fp8_expert_linear(x, w, offsets)
+        for e in (0, 511, 1023):
+            lo, hi = e * each, (e + 1) * each
+            check_close(out[lo:hi], type(x)(x.values[lo:hi], x.scales[lo:hi]), type(w)(w.values[e], w.scales[e]))
+
+
+def test_first_calls_from_several_threads():
+    import threading
+
+    from gemmlib_b200.experts import fp8_expert_linear
+    from gemmlib_b200.fp8_linear import fp8_linear
+
+    problems = [(rows_of(m, k, i), weight_of(n, k, 10 + i)) for i, (m, k, n) in enumerate([(5, 999, 333), (70, 2048, 500), (200, 1111, 800), (900, 640, 640)])]
+    offsets = torch.tensor([0, 100, 900], dtype=torch.int32, device="cuda")
+    stack = stack_of(2, 640, 640, 5)
+    want = [fp8_linear(x, w) for x, w in problems] + [fp8_expert_linear(problems[3][0], stack, offsets)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = fp8_linear(*problems[i]) if i < 4 else fp8_expert_linear(problems[3][0], stack, offsets)
+                    torch.cuda.current_stream().synchronize()
+                    assert torch.equal(got, want[i])
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(5)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed
+
+
+def test_a_backward_pass_captured_while_an_eager_graph_of_the_same_leaves_lives():
+    """On another stream that is refused (autograd's node for a leaf's gradient has the eager stream, and its wait would end the capture), for
+    either leaf, and the process goes on; on the same stream, and once the eager graph is gone, it is captured."""
+    from gemmlib_b200.experts import combine_rows, gather_rows
+
+    p = problem(40, 3, 6, 200, torch.float16, 1)
+    order = p["order"]
+    x, weights = p["x"].clone().requires_grad_(), p["weights"].clone().requires_grad_()
+    stream = torch.cuda.Stream()
+
+    def step():
+        out = combine_rows(gather_rows(x, order), order, weights)
+        return out, lambda: torch.autograd.grad(out, (x, weights), p["d_out"])
+
+    eager, backward = step()
+    stream.wait_stream(torch.cuda.current_stream())
+    for call in (lambda: gather_rows(x, order), lambda: combine_rows(p["y"], order, weights)):
+        with pytest.raises(RuntimeError, match="lives on another stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                call()
+    want = [t.clone() for t in backward()]
+    del eager, backward
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        eager, backward = step()
+        backward()
+        eager, backward = step()  # lives, on the stream that is captured
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        got = step()[1]()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and eager is not None
+
+
+def test_more_than_2_to_the_31_elements():
+    """Rows, outputs and weights whose last elements lie beyond: compared at both ends and in the middle."""
+    from gemmlib_b200.experts import combine_rows, fp8_expert_linear, gather_rows, sort_by_expert
+    from gemmlib_b200.fp8_linear import Fp8Rows, Fp8Weight, fp8_linear, quantize_fp8, quantize_fp8_weight, silu_mul_fp8
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, k = 70000, 32768
+    few = torch.tensor([0, 1, 40000, 65535, 65536, 69999], device="cuda")
+    x = torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+    x[:1000].normal_(generator=g)
+    for at in range(1000, n, 1000):
+        x[at:at + 1000] = x[:1000] * (1 + at / n)
+    own = x[few]
+    q, want = quantize_fp8(x), quantize_fp8(own)
+    assert torch.equal(q.values[few].float(), want.values.float()) and torch.equal(q.scales[few], want.scales)
+    assert torch.equal(q.dequantize(torch.bfloat16)[few], want.dequantize(torch.bfloat16))
+    assert torch.equal(silu_mul_fp8(x, x).values[few].float(), silu_mul_fp8(own, own).values.float())
+    w = quantize_fp8_weight(x)
+    last = quantize_fp8_weight(x[-(n % 128):])
+    assert torch.equal(w.values[-(n % 128):].float(), last.values.float()) and torch.equal(w.scales[-1:], last.scales)
+    # weights beyond 2^31 bytes, then outputs beyond 2^31 elements
+    a = rows_of(5, k, 1)
+    out = fp8_linear(a, w, dtype=torch.bfloat16)
+    tail = Fp8Weight(w.values[-(n % 128):], w.scales[-1:])
+    check_close(out[:, -(n % 128):], a, tail)
+    del out
+    b, c = rows_of(n, 128, 2), weight_of(k, 128, 3)
+    out = fp8_linear(b, c, dtype=torch.bfloat16)
+    check_close(out[few], Fp8Rows(b.values[few], b.scales[few]), c)
+    offsets = torch.tensor([0, 66000, n], dtype=torch.int32, device="cuda")
+    two = Fp8Weight(torch.stack([c.values.view(torch.uint8), c.values.view(torch.uint8).flip(0)]).view(torch.float8_e4m3fn), torch.stack([c.scales, c.scales]))
+    fp8_expert_linear(b, two, offsets, torch.bfloat16, out=out)
+    check_close(out[few[:5]], Fp8Rows(b.values[few[:5]], b.scales[few[:5]]), c)
+    check_close(out[few[5:]], Fp8Rows(b.values[few[5:]], b.scales[few[5:]]), Fp8Weight(two.values[1], two.scales[1]))
+    del out, two, q, want
+    # tokens to experts: 35000 of two choices
+    ids = torch.randint(-1, 5, (n // 2, 2), generator=g, device="cuda")
+    order = sort_by_expert(ids, 5)
+    rows = gather_rows(x[:n // 2], order)
+    kept = int(order.offsets[-1])
+    at = torch.tensor([0, kept // 2, kept - 1], device="cuda")
+    assert torch.equal(rows[at], x[order.source[at].long() // 2]) and (rows[kept:kept + 3] == 0).all() and (rows[-1] == 0).all()
+    weights = torch.rand(n // 2, 2, generator=g, device="cuda")
+    out = combine_rows(rows, order, weights)
+    t = torch.tensor([0, 20000, n // 2 - 1], device="cuda")
+    used = torch.where(order.places[t] >= 0, weights[t], 0.0).double().sum(1, keepdim=True)
+    rounded_close(out[t], x[t].double() * used, x[t].double().abs() * used, 3)
+    q = quantize_fp8(x[:n // 2], order)
+    assert torch.equal(q.values[at].float(), quantize_fp8(rows[at]).values.float()) and (q.scales[kept:] == 0).all()

@@ -2,9 +2,9 @@
 // rows, and the gradients of both moves.
 //
 // Sort: a stable counting sort.  Every warp has a run of choices and a counter for each expert in shared memory; it goes through its run 32
-// choices at a time, the lanes of one expert ranked by a match, and counts; then the counters become the places where its choices of an expert
+// choices at a time, the lanes of one expert ranked among themselves, and counts; then the counters become the places where its choices of an expert
 // begin (behind those of the experts, the CTAs and the warps before), and each choice's place is that and its rank.  Stable since runs, steps
-// and lanes follow the choices' order; no atomic decides a place.  Up to 8192 choices are one CTA's; more are split over CTAs, whose counts a kernel before writes.
+// and lanes follow the choices' order; no atomic decides a place.  Up to 4096 choices are one CTA's; more are split over CTAs, whose counts a kernel before writes.
 //
 // Moves: bound by HBM and L2, 16 bytes a lane, a warp a stretch of a row.  The weighted sum is gathered (a token reads its rows, in the order
 // of its choices, fp32), not scattered: no atomics, one rounding, the same result every time.  The gradient of the weighted sum reads y and the
@@ -28,7 +28,7 @@ using namespace blkq4::int8;
 
 // ---- sort ----
 constexpr int kMaxWarps = 32;
-constexpr int64_t kOneCta = 8192;
+constexpr int64_t kOneCta = 4096;  // (8192 choices: 12.1 us, by several CTAs 8.0; 4096: 8.7 and 8.6)
 constexpr int kItems = 8;  // choices of a lane that are under way at a time
 
 template <class Id>
@@ -63,9 +63,17 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Id* ids, int64_t n, in
   __syncthreads();
   const int64_t run = chunk / warps, begin = (int64_t)blockIdx.x * chunk + warp * run, end = min(n, begin + run);
   int* mine = cells + warp * width;
-  // 32 choices at a time: how many of a choice's expert are ahead of it in the run, by a match of the lanes and the counter so far
+  // 32 choices at a time: how many of a choice's expert are ahead of it in the run, by the lanes that have the same one and the counter so far.
+  // (The lanes by a vote for each bit of the number: the instruction that matches them takes a round for every expert among them, 8192 choices
+  // of 32 experts 14.0 us instead of 12.1.)
+  const int bits = 32 - __clz(width);
   auto take = [&](bool in, int key) {
-    const unsigned same = __match_any_sync(0xffffffffu, key);
+    unsigned same = 0xffffffffu;
+    for (int i = 0; i < bits; ++i) {
+      const bool set = key >> i & 1;
+      const unsigned with = __ballot_sync(0xffffffffu, set);
+      same &= set ? with : ~with;
+    }
     const int rank = __popc(same & ((1u << lane) - 1u));
     const int ahead = in ? mine[key] : 0;
     __syncwarp();

@@ -200,17 +200,17 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const MoveParams p, in
     if ((at.chunk + 32 * u) * 8 < p.cols) store8<T, VEC>(to, at.chunk + 32 * u, p.cols, r[u]);
 }
 
-template <class T, bool VEC>
+template <class T, bool VEC, int U>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveParams p, int parts) {
   griddep_wait();
   griddep_launch_dependents();
-  const Part at = part_of(parts, 1);
-  if (at.row >= p.tokens || at.chunk * 8 >= p.cols) return;
+  const Part at = part_of(parts, U);
+  if (at.row >= p.tokens) return;
   const int64_t first = at.row * p.choices, rows = (int64_t)p.tokens * p.choices;
-  float sum[8] = {};
+  float sum[U][8] = {};
   constexpr int kAhead = 4;  // rows under way at a time
   for (int j0 = 0; j0 < p.choices; j0 += kAhead) {
-    uint32_t r[kAhead][4] = {};
+    uint32_t r[kAhead][U][4] = {};
     float w[kAhead] = {};
     bool taken[kAhead];
 #pragma unroll
@@ -218,23 +218,33 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveParams p, i
       const int place = j0 + j < p.choices ? p.places[first + j0 + j] : -1;
       taken[j] = place >= 0 && place < rows;
       if (taken[j]) {
-        load8<T, VEC>(reinterpret_cast<const T*>(p.from) + (int64_t)place * p.ldf, at.chunk, p.cols, r[j]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if ((at.chunk + 32 * u) * 8 < p.cols)
+            load8<T, VEC>(reinterpret_cast<const T*>(p.from) + (int64_t)place * p.ldf, at.chunk + 32 * u, p.cols, r[j][u]);
         w[j] = p.weights ? weight_at(p, first + j0 + j) : 1.0f;
       }
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (!taken[j]) continue;  // a choice that was dropped has no row, whatever its weight is
-      float v[8];
-      unpack8<T>(r[j], v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[j], v[e], sum[e]);
+      for (int u = 0; u < U; ++u) {
+        float v[8];
+        unpack8<T>(r[j][u], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[u][e] = fmaf(w[j], v[e], sum[u][e]);
+      }
     }
   }
-  uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = pack2<T>(sum[2 * i], sum[2 * i + 1]);
-  store8<T, VEC>(reinterpret_cast<T*>(p.to) + at.row * p.ldt, at.chunk, p.cols, o);
+  for (int u = 0; u < U; ++u) {
+    if ((at.chunk + 32 * u) * 8 >= p.cols) continue;
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pack2<T>(sum[u][2 * i], sum[u][2 * i + 1]);
+    store8<T, VEC>(reinterpret_cast<T*>(p.to) + at.row * p.ldt, at.chunk + 32 * u, p.cols, o);
+  }
 }
 
 // A warp a place: to[p] = weight * d, dots[choice] = sum of y[p] * d, with d the row of the place's token.
@@ -347,12 +357,14 @@ std::string sort_typed(const Id* ids, int64_t n, int n_experts, int* source, int
                 source, places, offsets);
 }
 
+bool many_cols(int64_t rows, int cols) { return rows * cols >= 148 * 16 * 1024; }  // elements for 64 warps an SM, by stretches of 256
+
 template <class T>
 std::string gather_typed(const MoveParams& p, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.tokens * p.choices;
   const bool vec = rows_on_16(p.from, p.ldf, p.tokens) && rows_on_16(p.to, p.ldt, rows);
   // four loads of a lane under way where there are enough of them for that
-  const bool many = rows * p.cols >= 148 * 16 * 1024 && p.cols > 512;
+  const bool many = many_cols(rows, p.cols) && p.cols > 512;
   const int U = many ? 4 : 1, parts = (p.cols + 256 * U - 1) / (256 * U);
   const int64_t ctas = (rows * parts + kThreads / 32 - 1) / (kThreads / 32);
   if (many)
@@ -361,11 +373,14 @@ std::string gather_typed(const MoveParams& p, cudaStream_t stream) {
 }
 template <class T>
 std::string combine_typed(const MoveParams& p, cudaStream_t stream) {
-  const int parts = (p.cols + 255) / 256;
+  const bool vec = rows_on_16(p.from, p.ldf, (int64_t)p.tokens * p.choices) && rows_on_16(p.to, p.ldt, p.tokens);
+  // two stretches a warp where that leaves enough of them: 8192 tokens of four, 4096 wide, 63.9 -> 57.3 us, but 16 of eight 2.9 -> 3.3; rows that
+  // begin off 16 bytes take more registers and are slower by it, 4095 wide 96 -> 126 us
+  const bool two = vec && many_cols(p.tokens, p.cols) && p.cols > 256;
+  const int parts = (p.cols + 256 * (1 + two) - 1) / (256 * (1 + two));
   const int64_t ctas = ((int64_t)p.tokens * parts + kThreads / 32 - 1) / (kThreads / 32);
-  return rows_on_16(p.from, p.ldf, (int64_t)p.tokens * p.choices) && rows_on_16(p.to, p.ldt, p.tokens)
-             ? launch(combine_kernel<T, true>, ctas, kThreads, 0, stream, p, parts)
-             : launch(combine_kernel<T, false>, ctas, kThreads, 0, stream, p, parts);
+  if (two) return launch(combine_kernel<T, true, 2>, ctas, kThreads, 0, stream, p, parts);
+  return vec ? launch(combine_kernel<T, true, 1>, ctas, kThreads, 0, stream, p, parts) : launch(combine_kernel<T, false, 1>, ctas, kThreads, 0, stream, p, parts);
 }
 template <class T>
 std::string weigh_typed(const MoveParams& p, cudaStream_t stream) {

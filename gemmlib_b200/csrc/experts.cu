@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveParams p, i
   }
 }
 
-// A warp a place: to[p] = weight * d, dots[choice] = sum of y[p] * d, with d the row of the place's token.
+// A warp a place: to[p] = weight * d, dots[choice] = sum of y[p] * d, with d the row of the place's token; either may be left out (null), and its
+// reads or writes with it (8192 tokens of four, 4096 wide: both 112 us, the first 69, the second 64).
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kThreads) weigh_kernel(const MoveParams p) {
   griddep_wait();
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const MoveParams p) {
       const int c = c0 + 32 * u;
       if (choice >= 0 && c < chunks) {
         load8<T, VEC>(from, c, p.cols, a[u]);
-        load8<T, VEC>(y, c, p.cols, b[u]);
+        if (p.dots) load8<T, VEC>(y, c, p.cols, b[u]);
       }
     }
 #pragma unroll
@@ -285,9 +286,10 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const MoveParams p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (choice >= 0) o[i] = pack2<T>(w * d[2 * i], w * d[2 * i + 1]);
-      store8<T, VEC>(to, c, p.cols, o);
+      if (p.to) store8<T, VEC>(to, c, p.cols, o);
     }
   }
+  if (!p.dots) return;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
   if (lane == 0) {
@@ -385,7 +387,7 @@ std::string combine_typed(const MoveParams& p, cudaStream_t stream) {
 template <class T>
 std::string weigh_typed(const MoveParams& p, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.tokens * p.choices, ctas = (rows + kThreads / 32 - 1) / (kThreads / 32);
-  return rows_on_16(p.from, p.ldf, p.tokens) && rows_on_16(p.y, p.ldy, rows) && rows_on_16(p.to, p.ldt, rows)
+  return rows_on_16(p.from, p.ldf, p.tokens) && (!p.dots || rows_on_16(p.y, p.ldy, rows)) && (!p.to || rows_on_16(p.to, p.ldt, rows))
              ? launch(weigh_kernel<T, true>, ctas, kThreads, 0, stream, p)
              : launch(weigh_kernel<T, false>, ctas, kThreads, 0, stream, p);
 }

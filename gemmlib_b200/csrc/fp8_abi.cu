@@ -426,9 +426,9 @@ extern "C" int experts_combine_backward_sm100(int dtype, int tokens, int choices
         if (e.empty())
           e = check_all({{"d", d, d_size, ldd, tokens, cols, 2},
                          {"y", y, y_size, ldy, rows, cols, 2},
-                         {"source", source, source_size, rows, 1, rows, 4},
-                         {"d_y", d_y, d_y_size, lddy, rows, cols, 2},
-                         {"d_weights", d_weights, d_weights_size, rows, 1, rows, 4}});
+                         {"source", source, source_size, rows, 1, rows, 4}});
+        if (e.empty() && d_y) e = check_all({{"d_y", d_y, d_y_size, lddy, rows, cols, 2}});
+        if (e.empty() && (d_weights || !d_y)) e = check_all({{"d_weights", d_weights, d_weights_size, rows, 1, rows, 4}});
         if (e.empty()) e = check_weights(weights, weights_size, weights_type, rows);
         return e.empty() ? check_count(count) : e;
       },

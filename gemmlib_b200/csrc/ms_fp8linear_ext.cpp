@@ -3,10 +3,16 @@
 #include "ext_tensors.h"
 
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <tuple>
 
 namespace {
 
 using namespace ext_tensors;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 constexpr int64_t kBlock = 128;
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
@@ -413,8 +419,9 @@ Tensor combine(const Tensor& y, const Tensor& source, const Tensor& places, cons
   return out;
 }
 
-std::pair<Tensor, Tensor> combine_backward(const Tensor& d, const Tensor& y, const Tensor& source, const Tensor& places,
-                                           const Tensor& offsets, const Tensor& weights) {
+// Undefined where it is not wanted.
+std::pair<Tensor, Tensor> combine_backward(const Tensor& d, const Tensor& y, const Tensor& source, const Tensor& places, const Tensor& offsets,
+                                           const Tensor& weights, bool want_y, bool want_weights) {
   const int dtype = type_of("combine_rows: the rows", y.scalar_type());
   no_backward_here(d);
   no_backward_here(y);
@@ -427,14 +434,15 @@ std::pair<Tensor, Tensor> combine_backward(const Tensor& d, const Tensor& y, con
   const int type = weights_type("combine_rows", weights, places);
   const c10::cuda::CUDAGuard guard(y.device());
   const Tensor w = weights.contiguous();
-  const Tensor d_y = at::empty({order.rows, a.cols}, at::TensorOptions().dtype(y.scalar_type()).device(y.device()));
-  const Tensor d_weights = at::empty(places.sizes(), at::TensorOptions().dtype(at::kFloat).device(y.device()));
-  if (order.rows == 0) return {d_y, d_weights};
+  Tensor d_y, d_weights;
+  if (want_y) d_y = at::empty({order.rows, a.cols}, at::TensorOptions().dtype(y.scalar_type()).device(y.device()));
+  if (want_weights) d_weights = at::empty(places.sizes(), at::TensorOptions().dtype(at::kFloat).device(y.device()));
+  if (order.rows == 0 || (!want_y && !want_weights)) return {d_y, d_weights};
   std::string err;
   TORCH_CHECK(experts_combine_backward_sm100(dtype, int(order.tokens), int(order.choices), a.cols, current_stream(), g.data, g.bytes, g.ld,
                                              a.data, a.bytes, a.ld, w.data_ptr(), w.nbytes(), type, source.data_ptr(), source.nbytes(),
-                                             order.count, d_y.data_ptr(), d_y.nbytes(), a.cols, d_weights.data_ptr(), d_weights.nbytes(),
-                                             &err) == 0,
+                                             order.count, want_y ? d_y.data_ptr() : nullptr, want_y ? d_y.nbytes() : 0, a.cols,
+                                             want_weights ? d_weights.data_ptr() : nullptr, want_weights ? d_weights.nbytes() : 0, &err) == 0,
               err);
   return {d_y, d_weights};
 }
@@ -452,6 +460,70 @@ void check_captured_leaf(const Tensor& x) {
               "make it on this stream");
 }
 
+// ---- their backward passes ----
+// Gradients that have none of their own: the error is the one of a second differentiation, not of the first with a graph.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (const Tensor& g : grads)
+    if (g.defined()) defined.push_back(g.detach().set_requires_grad(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "gather_rows and combine_rows cannot be differentiated twice", int64_t(defined.size()));
+  const variable_list out = (*error)(std::move(defined));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
+struct GatherRows : torch::autograd::Function<GatherRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& source, const Tensor& places, const Tensor& offsets) {
+    ctx->save_for_backward({source, places, offsets});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return gather(x, source, places, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list grads(4);
+    {
+      const at::AutoGradMode off(false);
+      grads[0] = combine(d[0], saved[0], saved[1], saved[2], nullptr).view(ctx->saved_data["shape"].toIntVector());
+    }
+    return once(std::move(grads));
+  }
+};
+
+struct CombineRows : torch::autograd::Function<CombineRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor& source, const Tensor& places,
+                        const Tensor& offsets) {
+    ctx->save_for_backward({y, weights, source, places, offsets});
+    return combine(y, source, places, offsets, &weights);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list grads(5);
+    {
+      const at::AutoGradMode off(false);
+      std::tie(grads[0], grads[1]) = combine_backward(d[0], saved[0], saved[2], saved[3], saved[4], saved[1], ctx->needs_input_grad(0),
+                                                      ctx->needs_input_grad(1));
+      if (grads[1].defined()) grads[1] = grads[1].to(saved[1].scalar_type());
+    }
+    return once(std::move(grads));
+  }
+};
+
+Tensor gather_with_backward(const Tensor& x, const Tensor& source, const Tensor& places, const Tensor& offsets) {
+  if (!x.requires_grad() || !at::GradMode::is_enabled()) return gather(x, source, places, offsets);
+  check_captured_leaf(x);
+  return GatherRows::apply(x, source, places, offsets);
+}
+Tensor combine_with_backward(const Tensor& y, const Tensor& source, const Tensor& places, const Tensor& offsets, const Tensor& weights) {
+  if (!(y.requires_grad() || weights.requires_grad()) || !at::GradMode::is_enabled()) return combine(y, source, places, offsets, &weights);
+  check_captured_leaf(y);
+  check_captured_leaf(weights);
+  return CombineRows::apply(y, weights, source, places, offsets);
+}
+
 // ---- the calls' arguments, by position ----
 // Fp8Rows, Fp8Weight and ExpertOrder, named tuples of the Python modules: made here, since their own constructors are Python functions.
 PyTypeObject* g_types[3] = {};
@@ -461,7 +533,7 @@ PyObject* wrap(int type, std::initializer_list<const Tensor*> tensors) {
   if (!plain) throw python_error();
   Py_ssize_t i = 0;
   for (const Tensor* t : tensors) PyTuple_SET_ITEM(plain, i++, THPVariable_Wrap(*t));
-  if (type < 0 || !g_types[type]) return plain;
+  if (!g_types[type]) return plain;
   PyObject* args = PyTuple_Pack(1, plain);
   Py_DECREF(plain);
   if (!args) throw python_error();
@@ -552,7 +624,7 @@ PyObject* py_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   count_args(nargs, 4, "experts_gather(x, source, places, offsets)");
   constexpr const char* call = "gather_rows";
-  return THPVariable_Wrap(gather(tensor(args[0], call), tensor(args[1], call), tensor(args[2], call), tensor(args[3], call)));
+  return THPVariable_Wrap(gather_with_backward(tensor(args[0], call), tensor(args[1], call), tensor(args[2], call), tensor(args[3], call)));
   END_HANDLE_TH_ERRORS
 }
 
@@ -560,30 +632,12 @@ PyObject* py_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   count_args(nargs, 5, "experts_combine(y, source, places, offsets, weights)");
   constexpr const char* call = "combine_rows";
-  return THPVariable_Wrap(combine(tensor(args[0], call), tensor(args[1], call), tensor(args[2], call), tensor(args[3], call),
-                                  tensor_or_none(args[4], call)));
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_combine_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  HANDLE_TH_ERRORS
-  count_args(nargs, 6, "experts_combine_backward(d, y, source, places, offsets, weights)");
-  constexpr const char* call = "combine_rows";
-  const auto both = combine_backward(tensor(args[0], call), tensor(args[1], call), tensor(args[2], call), tensor(args[3], call),
-                                     tensor(args[4], call), tensor(args[5], call));
-  return wrap(-1, {&both.first, &both.second});
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_check_captured_leaves(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  HANDLE_TH_ERRORS
-  for (Py_ssize_t i = 0; i < nargs; ++i) check_captured_leaf(tensor(args[i], "experts_check_captured_leaves"));
-  Py_RETURN_NONE;
+  return THPVariable_Wrap(combine_with_backward(tensor(args[0], call), tensor(args[1], call), tensor(args[2], call), tensor(args[3], call),
+                                                tensor(args[4], call)));
   END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef g_methods[] = {
-    {"experts_check_captured_leaves", fast<py_check_captured_leaves>(), METH_FASTCALL, "Refuses leaves whose backward pass a capture would not outlive"},
     {"fp8_types", fast<py_types>(), METH_FASTCALL, "The tuple's subclasses that rows, weights and orders are returned as"},
     {"fp8_quantize", fast<py_quantize>(), METH_FASTCALL, "The rows of x in e4m3, in the order of their experts where one is given"},
     {"fp8_quantize_weight", fast<py_quantize_weight>(), METH_FASTCALL, "Weights in e4m3, a scale for each 128 x 128"},
@@ -594,7 +648,6 @@ PyMethodDef g_methods[] = {
     {"experts_sort", fast<py_sort>(), METH_FASTCALL, "The order of the choices by expert"},
     {"experts_gather", fast<py_gather>(), METH_FASTCALL, "Tokens in the order of their experts"},
     {"experts_combine", fast<py_combine>(), METH_FASTCALL, "The weighted sum of each token's rows"},
-    {"experts_combine_backward", fast<py_combine_backward>(), METH_FASTCALL, "Its gradient"},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

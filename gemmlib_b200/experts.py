@@ -19,7 +19,6 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import ms_blkq4linear_ext
 from .fp8_linear import BLOCK, Fp8Rows, Fp8Weight, KeepsScales, own_weight, quantize_fp8, quantize_fp8_weight, silu_mul_fp8
@@ -27,9 +26,7 @@ from .fp8_linear import BLOCK, Fp8Rows, Fp8Weight, KeepsScales, own_weight, quan
 _sort = ms_blkq4linear_ext.experts_sort
 _gather = ms_blkq4linear_ext.experts_gather
 _combine = ms_blkq4linear_ext.experts_combine
-_combine_backward = ms_blkq4linear_ext.experts_combine_backward
 _expert_linear = ms_blkq4linear_ext.fp8_expert_linear
-_check_captured_leaves = ms_blkq4linear_ext.experts_check_captured_leaves
 
 
 class ExpertOrder(NamedTuple):
@@ -53,48 +50,15 @@ def sort_by_expert(experts: torch.Tensor, n_experts: int) -> ExpertOrder:
     return _sort(experts, n_experts)
 
 
-class _Gather(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, source, places, offsets):
-        ctx.save_for_backward(source, places, offsets)
-        ctx.shape = x.shape
-        return _gather(x, source, places, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d):
-        return _combine(d, *ctx.saved_tensors, None).view(ctx.shape), None, None, None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, source, places, offsets):
-        ctx.save_for_backward(y, weights, source, places, offsets)
-        return _combine(y, source, places, offsets, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d):
-        y, weights, source, places, offsets = ctx.saved_tensors
-        d_y, d_weights = _combine_backward(d, y, source, places, offsets, weights)
-        return d_y if ctx.needs_input_grad[0] else None, d_weights.to(weights.dtype) if ctx.needs_input_grad[1] else None, None, None, None
-
-
 def gather_rows(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The row of ``x`` [..., features] (float16 or bfloat16) of every choice, in the order's places: [n, features]; zeros behind
     ``order.offsets[-1]``.  A token's gradient is the sum of its rows'."""
-    if x.requires_grad and torch.is_grad_enabled():
-        _check_captured_leaves(x)
-        return _Gather.apply(x, *order)
     return _gather(x, *order)
 
 
 def combine_rows(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor) -> torch.Tensor:
     """The sum of each token's rows of ``y`` [n, features], with ``weights`` (float32, float16 or bfloat16) of the shape of ``order.places``:
     [..., features], in the type of ``y``.  What stands behind ``order.offsets[-1]`` is not read."""
-    if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
-        _check_captured_leaves(y, weights)
-        return _Combine.apply(y, weights, *order)
     return _combine(y, *order, weights)
 
 

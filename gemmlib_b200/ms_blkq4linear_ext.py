@@ -59,5 +59,3 @@ fp8_expert_linear = _mod.fp8_expert_linear
 experts_sort = _mod.experts_sort
 experts_gather = _mod.experts_gather
 experts_combine = _mod.experts_combine
-experts_combine_backward = _mod.experts_combine_backward
-experts_check_captured_leaves = _mod.experts_check_captured_leaves

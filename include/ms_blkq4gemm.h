@@ -545,7 +545,7 @@ int experts_combine_sm100(
   void* error_message);
 
 /** The gradient of experts_combine_sm100: d_y[p] = weights[source[p]] * d[token of p] (zeros behind *count), d_weights[source[p]] = sum of y[p] * d[token
- *  of p] in fp32 (0 for choices of no expert). */
+ *  of p] in fp32 (0 for choices of no expert).  Either may be null: it is not computed then, and what it alone needs is not read. */
 int experts_combine_backward_sm100(
   int dtype, int tokens, int choices, int cols, void* stream,
   void const* d, size_t d_size, int64_t ldd,

@@ -568,3 +568,52 @@ def test_more_than_2_to_the_31_elements():
     rounded_close(out[t], x[t].double() * used, x[t].double().abs() * used, 3)
     q = quantize_fp8(x[:n // 2], order)
     assert torch.equal(q.values[at].float(), quantize_fp8(rows[at]).values.float()) and (q.scales[kept:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,choices,n_experts,k", [(1, 8, 8, 4096), (7, 3, 5, 1237), (300, 2, 7, 24)])
+def test_a_gradient_by_itself(tokens, choices, n_experts, k, dtype):
+    """Of the rows or of the weights alone: bit for bit as together."""
+    from gemmlib_b200.experts import combine_rows
+
+    p = problem(tokens, choices, n_experts, k, dtype, 4)
+    y, weights = p["y"].clone().requires_grad_(), p["weights"].clone().requires_grad_()
+    want = torch.autograd.grad(combine_rows(y, p["order"], weights), (y, weights), p["d_out"])
+    assert torch.equal(torch.autograd.grad(combine_rows(y, p["order"], p["weights"]), y, p["d_out"])[0], want[0])
+    out = combine_rows(p["y"], p["order"], weights)
+    assert torch.equal(torch.autograd.grad(out, weights, p["d_out"])[0], want[1])
+    out = combine_rows(y, p["order"], weights)  # both have one, one is asked for
+    assert torch.equal(torch.autograd.grad(out, weights, p["d_out"], retain_graph=True)[0], want[1])
+    assert torch.equal(torch.autograd.grad(out, y, p["d_out"])[0], want[0])
+
+
+def test_the_abi_computes_either_gradient():
+    from gemmlib_b200 import capi
+
+    p = problem(9, 3, 5, 40, torch.float16, 6)
+    source, count = p["order"].source, p["order"].offsets.data_ptr() + 4 * 5
+    new = lambda: (torch.full((27, 40), 7.0, dtype=torch.float16, device="cuda"), torch.full((9, 3), 7.0, device="cuda"))  # noqa: E731
+    run = lambda d_y, d_weights: capi.experts_combine_backward(  # noqa: E731
+        0, 9, 3, 40, (p["d_out"], 40), (p["y"], 40), p["weights"], 2, source, count, d_y, d_weights, stream=torch.cuda.current_stream().cuda_stream)
+    both, alone = new(), new()
+    run((both[0], 40), both[1])
+    run((alone[0], 40), None)
+    run(None, alone[1])
+    assert all(torch.equal(a, b) for a, b in zip(both, alone)) and not (both[0] == 7).all()
+    with pytest.raises(capi.BlkQ4Error, match="Null tensor pointer: d_weights"):
+        run(None, None)
+
+
+def test_a_second_differentiation_is_refused():
+    """A first one with a graph is not."""
+    from gemmlib_b200.experts import combine_rows, gather_rows
+
+    p = problem(9, 3, 5, 40, torch.float16, 6)
+    for leaf, call in ((p["x"], lambda t: gather_rows(t, p["order"])), (p["weights"], lambda t: combine_rows(p["y"], p["order"], t))):
+        leaf = leaf.clone().requires_grad_()
+        out = call(leaf)
+        plain, = torch.autograd.grad(out, leaf, torch.ones_like(out), retain_graph=True)
+        grad, = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)
+        assert torch.equal(grad, plain) and grad.requires_grad
+        with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+            grad.float().sum().backward()

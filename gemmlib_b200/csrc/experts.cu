@@ -260,22 +260,31 @@ __global__ void __launch_bounds__(kThreads) weigh_kernel(const MoveParams p) {
   const T* from = reinterpret_cast<const T*>(p.from) + (int64_t)(choice >= 0 ? choice / p.choices : 0) * p.ldf;
   const T* y = reinterpret_cast<const T*>(p.y) + row * p.ldy;
   T* to = reinterpret_cast<T*>(p.to) + row * p.ldt;
-  const int chunks = (p.cols + 7) / 8;
+  const int chunks = (p.cols + 7) / 8, cols = choice >= 0 ? p.cols : 0;  // (of a place without an expert nothing is read)
   float dot = 0.0f;
   constexpr int kAhead = 4;
   for (int c0 = lane; c0 < chunks; c0 += 32 * kAhead) {
-    uint32_t a[kAhead][4] = {}, b[kAhead][4] = {};
+    uint32_t a[kAhead][4] = {}, b[kAhead][4] = {}, wa[VEC ? 1 : kAhead][5], wb[VEC ? 1 : kAhead][5];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int c = c0 + 32 * u;
-      if (choice >= 0 && c < chunks) {
-        load8<T, VEC>(from, c, p.cols, a[u]);
-        if (p.dots) load8<T, VEC>(y, c, p.cols, b[u]);
+      if constexpr (VEC) {
+        if (choice >= 0 && c < chunks) {
+          load8<T, VEC>(from, c, p.cols, a[u]);
+          if (p.dots) load8<T, VEC>(y, c, p.cols, b[u]);
+        }
+      } else {
+        load_words(from, off_word(from), c, cols, wa[u]);
+        load_words(y, off_word(y), c, p.dots ? cols : 0, wb[u]);
       }
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int c = c0 + 32 * u;
+      if constexpr (!VEC) {
+        take_words(from, off_word(from), c, cols, wa[u], a[u]);
+        take_words(y, off_word(y), c, p.dots ? cols : 0, wb[u], b[u]);
+      }
       if (c >= chunks) continue;
       float d[8], v[8];
       unpack8<T>(a[u], d);

@@ -165,18 +165,30 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
   const int places = SCATTER ? p.rows * p.choices : 0;
   int first_zero = places;
   if constexpr (SCATTER) first_zero = max(0, *p.count);
+  const T *row_a = reinterpret_cast<const T*>(p.a) + at.row * p.lda, *row_b = reinterpret_cast<const T*>(p.b) + (OP == kSiluMul ? at.row * p.ldb : 0);
   uint32_t a[U][4] = {}, b[U][4] = {};
+  uint32_t wa[VEC ? 1 : U][5], wb[VEC ? 1 : U][5];
+  const int off_a = off_word(row_a), off_b = off_word(row_b), cols = in ? p.cols : 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int chunk = (at.block + u) * 16 + lane;
-    if (in && chunk * 8 < p.cols) {
-      load8<T, VEC, OP == kSiluMul || ONCE ? kOnce : kKept>(reinterpret_cast<const T*>(p.a) + at.row * p.lda, chunk, p.cols, a[u]);
-      if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.b) + at.row * p.ldb, chunk, p.cols, b[u]);
+    if constexpr (VEC) {
+      if (chunk * 8 < cols) {
+        load8<T, VEC, OP == kSiluMul || ONCE ? kOnce : kKept>(row_a, chunk, p.cols, a[u]);
+        if constexpr (OP == kSiluMul) load8<T, VEC, kOnce>(row_b, chunk, p.cols, b[u]);
+      }
+    } else {
+      load_words(row_a, off_a, chunk, cols, wa[u]);
+      if constexpr (OP == kSiluMul) load_words(row_b, off_b, chunk, cols, wb[u]);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int chunk = (at.block + u) * 16 + lane;
+    if constexpr (!VEC) {
+      take_words(row_a, off_a, chunk, cols, wa[u], a[u]);
+      if constexpr (OP == kSiluMul) take_words(row_b, off_b, chunk, cols, wb[u], b[u]);
+    }
     float v[8];
     uint32_t top;
     if constexpr (OP == kSiluMul) {
@@ -230,10 +242,19 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const RowsParam
   const bool in_cols = chunk * 8 < p.cols;
   const int64_t row0 = expert * p.expert_rows + n0;
   uint32_t a[8][4] = {};
+  const T* first = reinterpret_cast<const T*>(p.a) + row0 * p.lda;
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (in_cols && n0 + 16 * i < p.expert_rows)
-      load8<T, VEC, kOnce>(reinterpret_cast<const T*>(p.a) + (row0 + 16 * i) * p.lda, chunk, p.cols, a[i]);
+    for (int i = 0; i < 8; ++i)
+      if (in_cols && n0 + 16 * i < p.expert_rows) load8<T, VEC, kOnce>(first + 16 * i * p.lda, chunk, p.cols, a[i]);
+  } else {
+    uint32_t w[8][5];
+    const int off = off_word(first);  // (of all eight: sixteen rows are a multiple of 32 bytes)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load_words(first + 16 * i * p.lda, off, chunk, n0 + 16 * i < p.expert_rows ? p.cols : 0, w[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) take_words(first + 16 * i * p.lda, off, chunk, n0 + 16 * i < p.expert_rows ? p.cols : 0, w[i], a[i]);
+  }
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, top_of<T>(a[i]));

@@ -237,3 +237,24 @@ def test_refusals_on_the_gpu():
         quantize_fp8_weight(x[0])
     with pytest.raises(RuntimeError, match="at least one element"):
         quantize_fp8(x[:, :0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_that_begin_anywhere(dtype):
+    """Bit for bit as rows that begin on 16 bytes, for every width around a piece and a block, and every beginning within 16 bytes; what stands
+    beside the rows is NaN."""
+    from gemmlib_b200.fp8_linear import quantize_fp8, quantize_fp8_weight, silu_mul_fp8
+
+    def same(a, b, case):
+        assert torch.equal(a.values.view(torch.uint8), b.values.view(torch.uint8)) and torch.equal(a.scales, b.scales), case
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for k in [*range(1, 35), 127, 128, 129, 255, 257, 500, 1237]:
+        for before in range(9):
+            for behind in (0, 1, 4):
+                wide = torch.full((2, 19, before + k + behind), float("nan"), dtype=dtype, device="cuda")
+                gate, up = wide[:, :, before:before + k].copy_(torch.randn(2, 19, k, generator=g, device="cuda").to(dtype))
+                held = torch.zeros(2, 19, -(-k // 8) * 8, dtype=dtype, device="cuda")[:, :, :k].copy_(wide[:, :, before:before + k])
+                same(quantize_fp8(gate), quantize_fp8(held[0]), (k, before, behind))
+                same(quantize_fp8_weight(gate), quantize_fp8_weight(held[0]), (k, before, behind))
+                same(silu_mul_fp8(gate, up), silu_mul_fp8(*held), (k, before, behind))

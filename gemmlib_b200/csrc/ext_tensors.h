@@ -69,11 +69,14 @@ inline int type_of(const char* name, torch::ScalarType t) {
   return t == torch::kFloat16 ? INT8_FP16 : INT8_BF16;
 }
 
+inline void no_tangent(const Tensor& x, const char* kind) {
+  TORCH_CHECK(!x._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+              "The ", kind, " operators have no forward derivatives: take the primal of the dual tensor");
+}
 inline void no_backward(const Tensor& x, const char* kind) {
   TORCH_CHECK(!x.requires_grad() || !at::GradMode::is_enabled(),
               "The ", kind, " operators have no backward pass: call them under torch.no_grad(), or detach the tensor");
-  TORCH_CHECK(!x._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
-              "The ", kind, " operators have no forward derivatives: take the primal of the dual tensor");
+  no_tangent(x, kind);
 }
 
 // A caller's tensor is about to be written: what autograd has saved of it, or of a view, is not what it was.  (Tensors made under

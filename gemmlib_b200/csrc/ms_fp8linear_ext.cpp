@@ -514,13 +514,16 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
 
 Tensor gather_with_backward(const Tensor& x, const Tensor& source, const Tensor& places, const Tensor& offsets) {
   if (!x.requires_grad() || !at::GradMode::is_enabled()) return gather(x, source, places, offsets);
+  no_tangent(x, "experts'");
   check_captured_leaf(x);
   return GatherRows::apply(x, source, places, offsets);
 }
 Tensor combine_with_backward(const Tensor& y, const Tensor& source, const Tensor& places, const Tensor& offsets, const Tensor& weights) {
   if (!(y.requires_grad() || weights.requires_grad()) || !at::GradMode::is_enabled()) return combine(y, source, places, offsets, &weights);
-  check_captured_leaf(y);
-  check_captured_leaf(weights);
+  for (const Tensor* t : {&y, &weights}) {
+    no_tangent(*t, "experts'");
+    check_captured_leaf(*t);
+  }
   return CombineRows::apply(y, weights, source, places, offsets);
 }
 

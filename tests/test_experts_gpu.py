@@ -617,3 +617,60 @@ def test_a_second_differentiation_is_refused():
         assert torch.equal(grad, plain) and grad.requires_grad
         with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
             grad.float().sum().backward()
+
+
+def test_what_was_saved_for_a_gradient_must_not_change():
+    from gemmlib_b200.experts import combine_rows
+
+    p = problem(9, 3, 5, 40, torch.float16, 6)
+    y, weights = p["y"].clone(), p["weights"].clone().requires_grad_()
+    out = combine_rows(y, p["order"], weights)
+    y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+    out = combine_rows(y, p["order"], weights).float().sum()
+    out.backward()
+    with pytest.raises(RuntimeError, match="backward through the graph a second time"):
+        out.backward()
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwAD
+
+    from gemmlib_b200.experts import combine_rows, gather_rows
+
+    p = problem(9, 3, 5, 40, torch.float16, 6)
+    for wanted in (False, True):
+        with fwAD.dual_level():
+            x = fwAD.make_dual(p["x"].clone().requires_grad_(wanted), torch.ones_like(p["x"]))
+            weights = fwAD.make_dual(p["weights"].clone().requires_grad_(wanted), torch.ones_like(p["weights"]))
+            with pytest.raises(RuntimeError, match="no forward derivatives"):
+                gather_rows(x, p["order"])
+            with pytest.raises(RuntimeError, match="no forward derivatives"):
+                combine_rows(p["y"], p["order"], weights)
+    assert torch.equal(gather_rows(p["x"], p["order"]), gather_rows(p["x"].clone().requires_grad_(), p["order"]))
+
+
+def test_hooks_shared_leaves_and_sums_of_gradients():
+    """The same rows and weights in two sums, and a leaf's gradient that is added to."""
+    from gemmlib_b200.experts import combine_rows, gather_rows
+
+    p = problem(31, 2, 4, 72, torch.float16, 9)
+    order = p["order"]
+    x, weights = p["x"].clone().requires_grad_(), p["weights"].clone().requires_grad_()
+    seen = []
+    x.register_hook(lambda g: seen.append(g.clone()))
+    rows = gather_rows(x, order)
+    out = combine_rows(rows, order, weights) + combine_rows(rows * 2, order, weights)
+    for i in (1, 2):
+        out.backward(p["d_out"], retain_graph=True)
+        assert len(seen) == i
+    one = torch.autograd.grad(combine_rows(gather_rows(x, order), order, weights), weights, p["d_out"])[0]
+    # each gradient of the weights is a sum of 72 products in fp32, three times as large as one together; twice added up
+    size = 6 * (p["x"].double().abs() * p["d_out"].double().abs()).sum(1, keepdim=True)
+    assert ((weights.grad.double() - 6 * one.double()).abs() <= (72 / 32 + 10) * 2.0 ** -23 * size + 1e-30).all()
+    kept = (order.places >= 0).double() * p["weights"].double()
+    want = 2 * 3 * kept.sum(1, keepdim=True) * p["d_out"].double()
+    # rounded to fp16: each d_y (two of them, the one of the doubled rows again), their sum, the sum over a token's rows, the two backward passes' sum
+    bound = 2.0 ** -11 * 8 * 2 * 3 * kept.sum(1, keepdim=True) * p["d_out"].double().abs() + 2.0 ** -23
+    assert ((x.grad.double() - want).abs() <= bound).all()

@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "rows_io.cuh"
@@ -119,21 +120,6 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
   for (int s = 8; s > 0; s >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, s));
   return v;
 }
-template <class T>
-__device__ __forceinline__ void gated(uint32_t (&a)[4], uint32_t (&b)[4], float (&v)[8]) {
-  float u[8];
-  unpack8<T>(a, v);
-  unpack8<T>(b, u);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    // g / (1 + 2^(-g log2 e)); 1 + an infinity has the reciprocal 0
-    float p, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(v[e] * -1.44269504f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + p));
-    v[e] = v[e] * r * u[e];
-  }
-}
-
 // The part of a row that a half-warp takes: U blocks from `block` on.
 struct Part {
   int64_t row;
@@ -182,38 +168,46 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
       if constexpr (OP == kSiluMul) load_words(row_b, off_b, chunk, cols, wb[u]);
     }
   }
+  if constexpr (!VEC) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int chunk = (at.block + u) * 16 + lane;
-    if constexpr (!VEC) {
+    for (int u = 0; u < U; ++u) {
+      const int chunk = (at.block + u) * 16 + lane;
       take_words(row_a, off_a, chunk, cols, wa[u], a[u]);
       if constexpr (OP == kSiluMul) take_words(row_b, off_b, chunk, cols, wb[u], b[u]);
     }
-    float v[8];
-    uint32_t top;
-    if constexpr (OP == kSiluMul) {
-      gated<T>(a[u], b[u], v);
-      top = top_of(v);
-    } else {
-      top = top_of<T>(a[u]);
-      unpack8<T>(a[u], v);
-    }
-    top = half_warp_max(top);
-    if (!in || chunk * 8 >= p.cols) continue;
-    const uint2 q = convert8<OP == kQuant>(scale_of<OP == kQuant>(top), v);
-    const float scale = scale_value(top);
-    if constexpr (SCATTER) {
-      for (int j = 0; j < p.choices; ++j) {
-        const int place = p.places[at.row * p.choices + j];
-        if (place < 0 || place >= places) continue;  // of no expert (or of an order that is none)
-        store_q8(p.q + place * p.ldq, q_vec, chunk, p.cols, q);
-        if (lane == 0) p.scales[place * p.lds + at.block + u] = scale;
-      }
-    } else {
-      store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, q);
-      if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale;
-    }
   }
+  auto write = [&](auto far) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int chunk = (at.block + u) * 16 + lane;
+      float v[8];
+      uint32_t top;
+      if constexpr (OP == kSiluMul) {
+        silu_mul8<T, decltype(far)::value>(a[u], b[u], v);
+        top = top_of(v);
+      } else {
+        top = top_of<T>(a[u]);
+        unpack8<T>(a[u], v);
+      }
+      top = half_warp_max(top);
+      if (!in || chunk * 8 >= p.cols) continue;
+      const uint2 q = convert8<OP == kQuant>(scale_of<OP == kQuant>(top), v);
+      const float scale = scale_value(top);
+      if constexpr (SCATTER) {
+        for (int j = 0; j < p.choices; ++j) {
+          const int place = p.places[at.row * p.choices + j];
+          if (place < 0 || place >= places) continue;  // of no expert (or of an order that is none)
+          store_q8(p.q + place * p.ldq, q_vec, chunk, p.cols, q);
+          if (lane == 0) p.scales[place * p.lds + at.block + u] = scale;
+        }
+      } else {
+        store_q8(p.q + at.row * p.ldq, q_vec, chunk, p.cols, q);
+        if (lane == 0) p.scales[at.row * p.lds + at.block + u] = scale;
+      }
+    }
+  };
+  if (OP == kSiluMul && __any_sync(0xffffffffu, far_gates<T>(a))) write(std::true_type());
+  else write(std::false_type());
   if constexpr (SCATTER) {
     const int64_t halves = (int64_t)gridDim.x * (kThreads / 16), blocks = (p.cols + kBlock - 1) / kBlock;
     const int64_t end = ((int64_t)places - first_zero) * blocks;

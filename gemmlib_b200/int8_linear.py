@@ -60,7 +60,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
 
 
 def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor) -> Int8Rows:
-    """``gate / (1 + exp(-gate)) * up``, quantized by row; gate and up may be halves of one tensor."""
+    """``gate / (1 + exp(-gate)) * up``, quantized by row; gate and up may be halves of one tensor.  A gate below -87.3, whose sigmoid is no
+    normal float32, counts as 0."""
     return _silu_mul(gate, up)
 
 

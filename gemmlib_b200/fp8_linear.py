@@ -18,6 +18,7 @@ import torch
 from torch import nn
 
 from . import ms_blkq4linear_ext
+from .layers import KeepsBias
 
 BLOCK = 128
 
@@ -123,7 +124,7 @@ class KeepsScales(nn.Module):
         return super()._load_from_state_dict(*args, **kwargs)
 
 
-class Fp8Linear(KeepsScales):
+class Fp8Linear(KeepsBias, KeepsScales):
     """Linear layer with e4m3 weights: ``weights`` [out_features, in_features] (float16 or bfloat16, on the GPU) are quantized in the constructor.
     ``forward`` takes a float16 or bfloat16 tensor, and answers in its type, or ``Fp8Rows``, and answers in ``out``'s type or the weights'.
     From the second call on the weights' first tiles are fetched while the kernel ahead still runs (``early_weight_fetch = False`` on a layer
@@ -149,13 +150,13 @@ class Fp8Linear(KeepsScales):
         values, scales = own_weight(weight, copy)
         self.register_buffer("q_weights", values)
         self.register_buffer("q_scales", scales)
-        self.bias = bias_tensor
+        self._keep_bias(bias_tensor, copy)
         self.early_weight_fetch = True
         self._settled = False  # the first forward is a plain launch
 
     @classmethod
     def from_weight(cls, weight: Fp8Weight, bias_tensor: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16):
-        """A layer of weights that are e4m3 with their scales already, as a checkpoint has them, of any layout: it keeps a copy."""
+        """A layer of weights that are e4m3 with their scales already, as a checkpoint has them, of any layout: it keeps a copy of them and the bias."""
         self = cls.__new__(cls)
         nn.Module.__init__(self)
         self._set(Fp8Weight(*weight), bias_tensor, dtype, copy=True)

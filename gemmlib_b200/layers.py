@@ -1,0 +1,22 @@
+"""What the 8-bit linear layers share as modules."""
+from torch import nn
+
+
+class KeepsBias(nn.Module):
+    """Layers whose bias goes with their weights: into their state and out of it, to other devices and types."""
+
+    _version = 2  # states of version 1 have no bias: a layer that loads one keeps its own
+
+    def _keep_bias(self, bias, copy):
+        if bias is not None and copy:
+            bias = bias.detach().clone()
+        if isinstance(bias, nn.Parameter):
+            self.bias = bias
+        else:
+            self.register_buffer("bias", bias)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, *args, **kwargs):
+        version = local_metadata.get("version")
+        if (version is None or version < 2) and self.bias is not None:
+            state_dict.setdefault(prefix + "bias", self.bias)
+        return super()._load_from_state_dict(state_dict, prefix, local_metadata, *args, **kwargs)

@@ -1,0 +1,88 @@
+"""The bias of the 8-bit layers is part of them: of their state, of a move, of a copy."""
+import copy
+import io
+
+import pytest
+
+torch = pytest.importorskip("torch")
+E4M3 = torch.float8_e4m3fn
+
+
+def fp8(bias, n=130, k=64, device="cpu"):
+    from gemmlib_b200.fp8_linear import Fp8Linear, Fp8Weight
+
+    w = torch.full((n, k), 2.0, device=device).to(E4M3)
+    return Fp8Linear.from_weight(Fp8Weight(w, torch.ones(-(-n // 128), 1, device=device)), bias, torch.float16)
+
+
+LAYERS = {"fp8": fp8}
+
+
+def ramp(n=130, device="cpu"):
+    return torch.linspace(-3, 3, n, device=device).half()
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+def test_the_state_has_the_bias(kind):
+    make = LAYERS[kind]
+    layer, other = make(ramp()), make(torch.zeros(130, dtype=torch.float16))
+    held = io.BytesIO()
+    torch.save(layer.state_dict(), held)
+    held.seek(0)
+    other.load_state_dict(torch.load(held))
+    assert torch.equal(other.bias, ramp()) and "bias" not in make(None).state_dict() and make(None).bias is None
+    with pytest.raises(RuntimeError, match="bias"):  # neither dropped nor made up
+        make(None).load_state_dict(layer.state_dict())
+    with pytest.raises(RuntimeError, match="bias"):
+        layer.load_state_dict(make(None).state_dict())
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+def test_states_that_were_saved_without_it_are_loaded(kind):
+    make = LAYERS[kind]
+    layer, old = torch.nn.Sequential(make(ramp()), make(None)), torch.nn.Sequential(make(None), make(None)).state_dict()
+    for m in old._metadata.values():
+        m["version"] = 1
+    for state in (old, dict(old)):
+        layer.load_state_dict(state)
+        assert torch.equal(layer[0].bias, ramp()) and "0.bias" not in state
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+def test_the_bias_moves_and_is_copied(kind):
+    make = LAYERS[kind]
+    given = ramp()
+    layer = make(given)
+    given.zero_()  # the layer of given weights has a copy of it
+    assert torch.equal(layer.bias, ramp()) and torch.equal(copy.deepcopy(layer).bias, ramp())
+    assert torch.equal(copy.deepcopy(layer).bfloat16().bias, ramp().bfloat16())
+    assert layer.to("meta").bias.device.type == "meta"
+    parameter = make(torch.nn.Parameter(ramp()))
+    assert torch.equal(parameter.bias, ramp()) and not parameter.bias.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", LAYERS)
+def test_restored_and_moved_layers_on_the_gpu(kind):
+    make = LAYERS[kind]
+    layer = make(ramp(device="cuda"), device="cuda")
+    x = torch.randn(5, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    want = layer(x)
+    assert not torch.equal(want, make(None, device="cuda")(x))
+    other = make(torch.zeros(130, dtype=torch.float16, device="cuda"), device="cuda")
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), want)
+    for moved in (make(ramp()).cuda(), copy.deepcopy(layer).cpu().cuda()):  # the first one was made without a GPU
+        assert torch.equal(moved(x), want) and moved.bias.is_cuda
+
+
+@pytest.mark.gpu
+def test_layers_that_quantize_keep_a_parameter_as_one():
+    from gemmlib_b200.fp8_linear import Fp8Linear
+
+    plain = torch.nn.Linear(64, 130, device="cuda", dtype=torch.float16)
+    for cls in (Fp8Linear,):
+        layer = cls(plain.weight, plain.bias)
+        assert layer.bias is plain.bias and "bias" in layer.state_dict()
+        layer = cls(plain.weight, plain.bias.detach())
+        assert "bias" in dict(layer.named_buffers()) and layer.double().bias.dtype == torch.float64

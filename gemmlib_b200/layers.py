@@ -3,7 +3,8 @@ from torch import nn
 
 
 class KeepsBias(nn.Module):
-    """Layers whose bias goes with their weights: into their state and out of it, to other devices and types."""
+    """Layers whose bias goes with their weights: into their state and out of it, and to other devices.  Its type stays what it is when the
+    model is converted, as the scales' does: it is rounded once, to the output's."""
 
     _version = 2  # states of version 1 have no bias: a layer that loads one keeps its own
 
@@ -14,6 +15,13 @@ class KeepsBias(nn.Module):
             self.bias = bias
         else:
             self.register_buffer("bias", bias)
+
+    def _apply(self, fn, recurse=True):
+        held = self._buffers.get("bias")
+        super()._apply(fn, recurse)
+        if held is not None and self.bias.dtype != held.dtype:
+            self.bias = held.to(self.bias.device)
+        return self
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, *args, **kwargs):
         version = local_metadata.get("version")

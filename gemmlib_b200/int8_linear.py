@@ -19,6 +19,7 @@ import torch
 from torch import nn
 
 from . import ms_blkq4linear_ext
+from .layers import KeepsBias
 
 _EARLY = ms_blkq4linear_ext.EARLY_WEIGHT_FETCH
 _quantize = ms_blkq4linear_ext.int8_quantize
@@ -87,7 +88,7 @@ class RMSNormInt8(nn.Module):
         return f"{self.weight.numel()}, eps={self.eps}"
 
 
-class Int8Linear(nn.Module):
+class Int8Linear(KeepsBias):
     """Linear layer with int8 weights, one scale an output channel: ``weights`` [out_features, in_features] (float16 or
     bfloat16, on the GPU) are quantized in the constructor.  ``forward`` takes a float16 or bfloat16 tensor, and answers in its
     type, or ``Int8Rows``, and answers in ``out``'s type or the weights'.  From the second call on the weights' first tiles are
@@ -112,13 +113,14 @@ class Int8Linear(nn.Module):
             values = values.clone(memory_format=torch.contiguous_format)
         self.register_buffer("q_weights", values)
         self.register_buffer("q_scales", rows.scales.detach().clone())  # (the operators' rows and scales share their memory)
-        self.bias = bias_tensor
+        self._keep_bias(bias_tensor, copy)
         self.early_weight_fetch = True
         self._settled = False  # the first forward is a plain launch
 
     @classmethod
     def from_rows(cls, weight: Int8Rows, bias_tensor: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16):
-        """A layer of weights that are int8 rows already, [out_features, in_features], of any layout: it keeps a copy."""
+        """A layer of weights that are int8 rows already, [out_features, in_features], of any layout: it keeps a copy of them and the
+        bias."""
         self = cls.__new__(cls)
         nn.Module.__init__(self)
         self._set(Int8Rows(*weight), bias_tensor, dtype, copy=True)

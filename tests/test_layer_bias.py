@@ -15,7 +15,13 @@ def fp8(bias, n=130, k=64, device="cpu"):
     return Fp8Linear.from_weight(Fp8Weight(w, torch.ones(-(-n // 128), 1, device=device)), bias, torch.float16)
 
 
-LAYERS = {"fp8": fp8}
+def int8(bias, n=130, k=64, device="cpu"):
+    from gemmlib_b200.int8_linear import Int8Linear, Int8Rows
+
+    return Int8Linear.from_rows(Int8Rows(torch.full((n, k), 2, dtype=torch.int8, device=device), torch.ones(n, device=device)), bias)
+
+
+LAYERS = {"fp8": fp8, "int8": int8}
 
 
 def ramp(n=130, device="cpu"):
@@ -80,9 +86,10 @@ def test_restored_and_moved_layers_on_the_gpu(kind):
 @pytest.mark.gpu
 def test_layers_that_quantize_keep_a_parameter_as_one():
     from gemmlib_b200.fp8_linear import Fp8Linear
+    from gemmlib_b200.int8_linear import Int8Linear
 
     plain = torch.nn.Linear(64, 130, device="cuda", dtype=torch.float16)
-    for cls in (Fp8Linear,):
+    for cls in (Fp8Linear, Int8Linear):
         layer = cls(plain.weight, plain.bias)
         assert layer.bias is plain.bias and "bias" in layer.state_dict()
         layer = cls(plain.weight, plain.bias.detach())

@@ -1,6 +1,6 @@
 // Product of one or two e4m3 rows: weight rows streamed once through registers.
 //
-// Bound by the weights' bytes.  A warp takes R weight rows at a time, 512 consecutive bytes of each per load: a lane's 16 lie within a block of
+// Bound by the weights' bytes.  A warp takes R weight rows, 512 consecutive bytes of each per load: a lane's 16 lie within a block of
 // 128, so its products, exact in fp32, are added up and the sum is scaled once.  e4m3 is exact in fp16, and the multiply-add of two fp16 numbers
 // into fp32 takes them as they are converted: 24 instructions for 16 products.  No shared memory, no barrier: at a token's sizes a call is mostly
 // latency.  The loads of the next piece are issued before the products of the present one.  One order of additions for a row, whatever
@@ -62,15 +62,15 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
 template <class T, int MR, int R, int U, int CTAS>
 __global__ void __launch_bounds__(32 * kWarps, CTAS) fp8_gemv_kernel(const GemvParams p) {
   const int lane = threadIdx.x & 31;
-  const int groups = (p.N + R - 1) / R, step = (int)gridDim.x * kWarps;
-  // neighbouring groups go to different CTAs, so that every SM has the same number of them (give or take one)
-  int g = (int)(threadIdx.x >> 5) * (int)gridDim.x + (int)blockIdx.x;
+  const int groups = (p.N + R - 1) / R;
+  // one for each warp at most; neighbouring groups go to different CTAs, so that every SM has the same number of them (give or take one)
+  const int g = (int)(threadIdx.x >> 5) * (int)gridDim.x + (int)blockIdx.x;
   const int whole = p.K & ~15;  // the last K % 16 k are taken one by one
   uint4 w[R][U];
-  auto load = [&](int group, int k0) {
+  auto load = [&](int k0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint8_t* row = p.w + (int64_t)min(group * R + r, p.N - 1) * p.ldw;
+      const uint8_t* row = p.w + (int64_t)min(g * R + r, p.N - 1) * p.ldw;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int k = k0 + u * 512 + lane * 16;
@@ -79,19 +79,15 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) fp8_gemv_kernel(const GemvP
     }
   };
   if (p.early) {
-    if (g < groups) load(g, 0);
-  } else if (lane < R && whole > 0) {  // on their way into L2, where a write that is still to come would find them
-    for (int i = 0; i < 2; ++i)
-      if ((int64_t)g + (int64_t)i * step < groups)
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.w + (int64_t)min((g + i * step) * R + lane, p.N - 1) * p.ldw),
-                     "r"(whole)
-                     : "memory");
+    if (g < groups) load(0);
+  } else if (lane < R && whole > 0 && g < groups) {  // on their way into L2, where a write that is still to come would find them
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.w + (int64_t)min(g * R + lane, p.N - 1) * p.ldw), "r"(whole) : "memory");
   }
   griddep_wait();
   griddep_launch_dependents();
-  if (!p.early && g < groups) load(g, 0);
+  if (!p.early && g < groups) load(0);
 
-  for (; g < groups; g += step) {
+  if (g < groups) {
     float acc[R][MR] = {};
     const int n_l = g * R + lane % R, m_l = lane / R;
     const bool mine = lane < R * MR && n_l < p.N && m_l < p.M;
@@ -116,8 +112,7 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) fp8_gemv_kernel(const GemvP
       const int at = k0;
       k0 += 512 * U;
       const bool last = k0 >= whole;
-      if (!last) load(g, k0);
-      else if (g + step < groups) load(g + step, 0);
+      if (!last) load(k0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int k = at + u * 512 + lane * 16;
@@ -174,9 +169,10 @@ __global__ void __launch_bounds__(32 * kWarps, CTAS) fp8_gemv_kernel(const GemvP
 
 template <class T, int MR, int R, int U, int CTAS>
 std::string launch_instance(const GemvParams& p, cudaStream_t stream) {
-  const int groups = (p.N + R - 1) / R;
+  const int groups = (p.N + R - 1) / R, ctas = std::min(CTAS * std::max(1, sm_count()), groups);
+  if (groups > ctas * kWarps) return "more weight rows than warps";  // (gemv_takes leaves those to the other kernels)
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(CTAS * std::max(1, sm_count()), groups));
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(32 * kWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -191,17 +187,25 @@ std::string launch_instance(const GemvParams& p, cudaStream_t stream) {
 
 template <class T>
 std::string launch_typed(const GemvParams& p, cudaStream_t stream) {
-  // Two rows: two weight rows at a time, which share the conversion of the activations.  One / two weight rows a warp, us: M = 1, 2048 x 2816
+  // Two rows: two weight rows at a time, which share the conversion of the activations.  (gemv_takes goes by these.)  One / two weight rows a warp, us: M = 1, 2048 x 2816
   // 3.1 / 3.2; M = 2 4.3 / 3.6.
   return p.M == 1 ? launch_instance<T, 1, 1, 4, 3>(p, stream) : launch_instance<T, 2, 2, 4, 2>(p, stream);
 }
 
 }  // namespace
 
-// Small problems: this kernel has no set-up, no tensor memory and no exchange of parts, but takes its products' instructions, which the tensor
-// cores do not (4096 x 11008 15.1 us, the tensor cores 11.1).  Measured, this one / tensor cores, us: 1024 x 1024 2.2 / 3.2, 1408 x 2048 2.6 / 3.6, 2048 x
-// 2816 3.1 / 3.8, 4096 x 4096 5.6 / 6.0 (two rows 6.9 / 5.9), 8192 x 1024 6.3 / 5.5, 512 x 20000 8.7 / 4.5.
-bool gemv_takes(int M, int N, int K) { return M <= 2 && (int64_t)N * K <= (6 << 20); }
+// This kernel has no set-up, no tensor memory and no exchange of parts, but takes its products' instructions, which the tensor cores do not, and a warp
+// has a whole weight row (of two rows' calls: two) to itself.  So it is for weights that have one for each warp on the GPU at most, and whose rows are no long
+// chains of loads.  Measured, this one / tensor cores, us, K x N: one row, 1024 x 1024 1.8 / 3.0, 1408 x 2048 2.4 / 3.4, 2048 x 2816 2.9 / 4.2, 4096 x 3552 4.8 /
+// 6.5; two, 2048 x 2816 3.6 / 4.2, 2560 x 512 3.4 / 3.9, 512 x 4700 2.6 / 3.2.  With a loop over more rows than warps, or beyond the limits of K: one row, 1024 x
+// 4096 3.7 / 3.8, 512 x 5504 3.7 / 3.3, 200 x 28672 17.1 / 4.4, 5504 x 512 4.7 / 4.4, 8192 x 512 6.0 / 4.9, 28672 x 200 17.9 / 10.5; two, 512 x 5504 3.8 / 3.2, 4096 x
+// 512 4.2 / 3.7, 2560 x 3500 5.6 / 4.6.  Of 484 such problems (with the loop) the choices are 0.3 % slower than the better kernel on average; as the product N * K alone
+// would have it, 17 %.
+bool gemv_takes(int M, int N, int K) {
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  if (M == 1) return K <= 4096 && N <= sms * 3 * kWarps;
+  return M == 2 && K <= 2816 && N <= sms * 2 * kWarps * 2 && (int64_t)N * K <= (6 << 20);
+}
 
 std::string launch_gemv(Dtype dtype, const GemmArgs& g, unsigned flags, cudaStream_t stream) {
   const GemvParams p{g.M, g.N, g.K, (flags & BLKQ4_GEMM_EARLY_WEIGHT_FETCH) != 0, g.x, g.ldx, g.x_scales, g.ldxs, g.w, g.ldw,

@@ -71,7 +71,8 @@ def fp8_expert_linear(x: Fp8Rows, weight: Fp8Weight, offsets: torch.Tensor, dtyp
 
 class Fp8Experts(KeepsScales):
     """A layer of gated feed-forward experts with e4m3 weights: ``gate_up`` [experts, 2 * ffn, features] (gate first) and ``down`` [experts,
-    features, ffn], 16-bit tensors that are quantized in the constructor, one expert at a time.
+    features, ffn], 16-bit tensors that are quantized in the constructor, each in one call (with a second copy of the e4m3 values for as long as it
+    lasts where rows are no whole 32 bytes).
 
     ``forward(x, experts, weights)``: the weighted sum of the experts' ``down(silu(gate) * up)`` for ``x`` [..., features], choices ``experts`` [...,
     choices] and their ``weights``.  The weights' gradient is computed (a router can be trained); there is none for ``x``."""

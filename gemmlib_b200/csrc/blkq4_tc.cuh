@@ -143,26 +143,6 @@ __device__ __forceinline__ void st_async_v4(uint32_t dst, uint32_t bar, uint32_t
                "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
-__device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
-}
-// Arrives, once every earlier MMA of the pair has retired, on the barrier at this offset in both CTAs.
-__device__ __forceinline__ void commit_both(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
-      : "memory");
-}
-// Copy into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar_cluster) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar_cluster)
-      : "memory");
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
-}
 
 // Shared-memory matrix descriptor of a K-major operand tile stored as rows of 128 bytes
 // (64 fp16) with the 128-byte swizzle, rows contiguous, tile base 1024-byte aligned:

@@ -36,7 +36,6 @@ __device__ int g_fp8_error = 0;  // 0 ok; otherwise (role << 8) | stage of the w
 namespace {
 
 using namespace blkq4::int8;
-using tc::prefetch_l2_2d;
 using tc::st_async_v4;
 using tc::try_wait_cluster;
 
@@ -85,25 +84,22 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int umma_m, int umma_n) {
   return (1u << 4) | ((uint32_t)(umma_n >> 3) << 17) | ((uint32_t)(umma_m >> 4) << 24);
 }
 // The four MMAs of a step: 32 k each, both operands two descriptor units (32 bytes) further on.  The first one starts the sum.
-#define FP8_UMMA_X4(NAME, GROUP)                                                                                                   \
-  __device__ __forceinline__ void NAME(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {           \
-    asm volatile(                                                                                                                  \
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t"              \
-        "setp.ne.b32 p, 0, 0;\n\t"                                                                                                 \
-        "setp.eq.b32 q, 0, 0;\n\t"                                                                                                 \
-        "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\t"                                                       \
-        "add.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"                                                       \
-        "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"                     \
-        "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"                     \
-        "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a0, b0, %4, p;\n\t"                                                   \
-        "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a1, b1, %4, q;\n\t"                                                   \
-        "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a2, b2, %4, q;\n\t"                                                   \
-        "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], a3, b3, %4, q;\n\t}" ::"r"(d_tmem),                                   \
-        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc)                                                                             \
-        : "memory");                                                                                                               \
-  }
-FP8_UMMA_X4(umma_e4m3_x4, "1")
-#undef FP8_UMMA_X4
+__device__ __forceinline__ void umma_e4m3_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t"
+      "setp.ne.b32 p, 0, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\t"
+      "add.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+      "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+      "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a0, b0, %4, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %4, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %4, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %4, q;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc)
+      : "memory");
+}
 
 // Groups of eight columns, 16 columns apart, there when it returns: loads and wait are one statement, so that no use of the registers can
 // come between them.

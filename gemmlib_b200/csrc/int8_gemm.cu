@@ -31,11 +31,7 @@ __device__ int g_int8_error = 0;  // 0 ok; otherwise (role << 8) | stage of the 
 
 namespace {
 
-using tc::arrive_cluster;
-using tc::commit_both;
-using tc::prefetch_l2_2d;
 using tc::st_async_v4;
-using tc::tma_load_pair;
 using tc::try_wait_cluster;
 
 constexpr int kStepK = 128;                 // k of a pipeline step: one 128-byte swizzle row
@@ -97,6 +93,9 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+__device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 // How two neighbouring outputs of a row may be stored at once: not; from every even n; in rows of even m from every even n, in the others
 // from every odd one (contiguous rows of an odd length).
@@ -390,6 +389,23 @@ __device__ __forceinline__ void umma_i8_x4_pair(uint32_t d_tmem, uint32_t a_lo, 
       "tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %4, q;\n\t}"
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// Arrives, once every earlier MMA of the pair has retired, on the barrier at this offset in both CTAs.
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Copy into this CTA's shared memory whose bytes complete on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar_cluster)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 // The tiles of a pair: every num_pairs-th.  Tiles run in bands of group_m m tiles, m fastest, so that those under way at a time
 // share the rows of both operands in L2.

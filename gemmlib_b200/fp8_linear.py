@@ -18,7 +18,7 @@ import torch
 from torch import nn
 
 from . import ms_blkq4linear_ext
-from .layers import KeepsBias
+from .layers import KeepsBias, SettlesAnew
 
 BLOCK = 128
 
@@ -98,7 +98,7 @@ def own_weight(weight: Fp8Weight, copy: bool) -> Fp8Weight:
 
 
 class KeepsScales(nn.Module):
-    """Layers whose float32 scales stay what they are when the model is converted, and whose weights settle anew whenever they are written."""
+    """Layers whose float32 scales and e4m3 weights stay what they are when the model is converted."""
 
     _scale_names = ()
 
@@ -112,19 +112,10 @@ class KeepsScales(nn.Module):
         for name, v in values.items():
             if self._buffers[name].dtype != torch.float8_e4m3fn:
                 self._buffers[name] = v.to(self._buffers[name].device)
-        self._settled = False
         return self
 
-    def __setstate__(self, state):
-        super().__setstate__(state)
-        self._settled = False  # a copy's buffers are written on some stream too
 
-    def _load_from_state_dict(self, *args, **kwargs):
-        self._settled = False  # the buffers are about to be overwritten by a copy on some stream
-        return super()._load_from_state_dict(*args, **kwargs)
-
-
-class Fp8Linear(KeepsBias, KeepsScales):
+class Fp8Linear(KeepsBias, SettlesAnew, KeepsScales):
     """Linear layer with e4m3 weights: ``weights`` [out_features, in_features] (float16 or bfloat16, on the GPU) are quantized in the constructor.
     ``forward`` takes a float16 or bfloat16 tensor, and answers in its type, or ``Fp8Rows``, and answers in ``out``'s type or the weights'.
     From the second call on the weights' first tiles are fetched while the kernel ahead still runs (``early_weight_fetch = False`` on a layer

@@ -19,7 +19,7 @@ import torch
 from torch import nn
 
 from . import ms_blkq4linear_ext
-from .layers import KeepsBias
+from .layers import KeepsBias, SettlesAnew
 
 _EARLY = ms_blkq4linear_ext.EARLY_WEIGHT_FETCH
 _quantize = ms_blkq4linear_ext.int8_quantize
@@ -88,7 +88,7 @@ class RMSNormInt8(nn.Module):
         return f"{self.weight.numel()}, eps={self.eps}"
 
 
-class Int8Linear(KeepsBias):
+class Int8Linear(KeepsBias, SettlesAnew):
     """Linear layer with int8 weights, one scale an output channel: ``weights`` [out_features, in_features] (float16 or
     bfloat16, on the GPU) are quantized in the constructor.  ``forward`` takes a float16 or bfloat16 tensor, and answers in its
     type, or ``Int8Rows``, and answers in ``out``'s type or the weights'.  From the second call on the weights' first tiles are
@@ -131,16 +131,7 @@ class Int8Linear(KeepsBias):
         super()._apply(fn, recurse)
         if self.q_scales.dtype != torch.float32:  # .half() and the like are for the model's 16-bit tensors
             self.q_scales = scales.to(self.q_scales.device)
-        self._settled = False
         return self
-
-    def __setstate__(self, state):
-        super().__setstate__(state)
-        self._settled = False  # a copy's buffers are written on some stream too
-
-    def _load_from_state_dict(self, *args, **kwargs):
-        self._settled = False  # the buffers are about to be overwritten by a copy on some stream
-        return super()._load_from_state_dict(*args, **kwargs)
 
     def weight_bytes(self) -> int:
         return self.out_features * self.in_features + 4 * self.out_features

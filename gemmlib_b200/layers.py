@@ -28,3 +28,22 @@ class KeepsBias(nn.Module):
         if (version is None or version < 2) and self.bias is not None:
             state_dict.setdefault(prefix + "bias", self.bias)
         return super()._load_from_state_dict(state_dict, prefix, local_metadata, *args, **kwargs)
+
+
+class SettlesAnew(nn.Module):
+    """Layers that fetch their weights early only from the second call on (``_settled``), counted from when the weights were last written."""
+
+    _settled = False
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._settled = False
+        return self
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._settled = False  # a copy's buffers are written on some stream too
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._settled = False  # the buffers are about to be overwritten by a copy on some stream
+        return super()._load_from_state_dict(*args, **kwargs)

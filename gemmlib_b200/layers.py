@@ -9,12 +9,11 @@ class KeepsBias(nn.Module):
     _version = 2  # states of version 1 have no bias: a layer that loads one keeps its own
 
     def _keep_bias(self, bias, copy):
-        if bias is not None and copy:
-            bias = bias.detach().clone()
+        """A copy, so that a state that is loaded does not reach the caller's tensor; of a parameter only where `copy` is wanted."""
         if isinstance(bias, nn.Parameter):
-            self.bias = bias
+            self.bias = nn.Parameter(bias.detach().clone(), bias.requires_grad) if copy else bias
         else:
-            self.register_buffer("bias", bias)
+            self.register_buffer("bias", None if bias is None else bias.detach().clone().requires_grad_(bias.requires_grad))
 
     def _apply(self, fn, recurse=True):
         held = self._buffers.get("bias")

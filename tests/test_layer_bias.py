@@ -64,8 +64,19 @@ def test_the_bias_moves_and_is_copied(kind):
     converted = copy.deepcopy(layer).bfloat16().bias
     assert converted.dtype == torch.float16 and torch.equal(converted, ramp())
     assert layer.to("meta").bias.device.type == "meta"
-    parameter = make(torch.nn.Parameter(ramp()))
-    assert torch.equal(parameter.bias, ramp()) and not parameter.bias.requires_grad
+    given = torch.nn.Parameter(ramp())
+    kept = make(given).bias
+    assert isinstance(kept, torch.nn.Parameter) and kept is not given and kept.requires_grad and torch.equal(kept, ramp())
+    assert make(ramp().requires_grad_()).bias.requires_grad  # which a call refuses while gradients are enabled
+
+
+@pytest.mark.parametrize("kind", LAYERS)
+def test_a_state_is_not_loaded_into_what_was_given(kind):
+    make = LAYERS[kind]
+    given = torch.zeros(130, dtype=torch.float16)
+    layer, other = make(given), make(given)
+    layer.load_state_dict(make(ramp()).state_dict())
+    assert torch.equal(layer.bias, ramp()) and not given.any() and not other.bias.any()
 
 
 @pytest.mark.gpu
@@ -92,5 +103,9 @@ def test_layers_that_quantize_keep_a_parameter_as_one():
     for cls in (Fp8Linear, Int8Linear):
         layer = cls(plain.weight, plain.bias)
         assert layer.bias is plain.bias and "bias" in layer.state_dict()
-        layer = cls(plain.weight, plain.bias.detach())
-        assert "bias" in dict(layer.named_buffers()) and layer.double().bias.dtype == torch.float16
+        given = plain.bias.detach()
+        layer = cls(plain.weight, given)
+        assert "bias" in dict(layer.named_buffers()) and layer.bias.data_ptr() != given.data_ptr() and torch.equal(layer.bias, given)
+        with torch.no_grad():
+            assert torch.equal(layer(torch.zeros(2, 64, device="cuda").half())[1], given)
+        assert layer.double().bias.dtype == torch.float16

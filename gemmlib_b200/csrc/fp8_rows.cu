@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const RowsParams p, int 
       if constexpr (OP == kSiluMul) load_words(row_b, off_b, chunk, cols, wb[u]);
     }
   }
-  if constexpr (!VEC) {
+  if constexpr (!VEC) {  // all of them ahead of the first use: 16000 x 2747 quantized 32.6 -> 31.4 us
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int chunk = (at.block + u) * 16 + lane;

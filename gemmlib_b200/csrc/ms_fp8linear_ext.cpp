@@ -5,8 +5,10 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <tuple>
+#include <unordered_set>
 
 namespace {
 
@@ -460,6 +462,37 @@ void check_captured_leaf(const Tensor& x) {
               "make it on this stream");
 }
 
+// The same of a leaf that stands behind other operators, or of an input that was computed before the capture: asked in the backward pass, when it is known which
+// nodes it will come to.  Those of the legacy default stream are the ones that nothing captured can be waited for on.
+void check_captured_backward(const Tensor& d) {
+  if (!d.is_cuda()) return;
+  const c10::cuda::CUDAGuard guard(d.device());
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();  // empty: all of them
+  const auto here = torch::autograd::get_current_node();
+  if (!here) return;
+  std::vector<torch::autograd::Node*> left{here.get()};
+  std::unordered_set<torch::autograd::Node*> seen{here.get()};
+  while (!left.empty()) {
+    torch::autograd::Node* node = left.back();
+    left.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      torch::autograd::Node* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (wanted && !wanted->empty()) {
+        const auto it = wanted->find(next);
+        if (it == wanted->end() || !it->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      TORCH_CHECK(!stream || stream->device_type() != c10::DeviceType::CUDA || c10::cuda::CUDAStream(c10::cuda::CUDAStream::UNCHECKED, *stream).stream() != nullptr,
+                  "A backward pass that is captured comes to a node of the default stream (", next->name(),
+                  "), which lives on another stream than the one that is captured: compute the input inside the capture, and delete eager graphs of the same leaves (their "
+                  "outputs) first, or make them on this stream");
+      left.push_back(next);
+    }
+  }
+}
+
 // ---- their backward passes ----
 // Gradients that have none of their own: the error is the one of a second differentiation, not of the first with a graph.
 variable_list once(variable_list grads) {
@@ -483,6 +516,7 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
     return gather(x, source, places, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
+    check_captured_backward(d[0]);
     const auto saved = ctx->get_saved_variables();
     variable_list grads(4);
     {
@@ -500,6 +534,7 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
     return combine(y, source, places, offsets, &weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
+    check_captured_backward(d[0]);
     const auto saved = ctx->get_saved_variables();
     variable_list grads(5);
     {

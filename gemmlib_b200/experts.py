@@ -11,7 +11,7 @@ expert that is none of 0 .. n_experts - 1 (-1 for padding, or another GPU's expe
 ``gather_rows`` and ``combine_rows`` have a backward pass (of one order).  All sums are float32, taken in the order of a token's choices, and
 rounded once; nothing depends on the order of atomics.  Offsets stay on the device: no call waits for the GPU, and all of them can be captured, with
 their backward pass (not while an eager graph of the same leaves lives on another stream: autograd would make the capture wait for it; such a
-call is refused).
+call is refused, or its backward pass where the leaf stands behind other operators).
 """
 from __future__ import annotations
 

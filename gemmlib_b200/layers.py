@@ -15,6 +15,11 @@ class KeepsBias(nn.Module):
         else:
             self.register_buffer("bias", None if bias is None else bias.detach().clone().requires_grad_(bias.requires_grad))
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "bias" in self.__dict__:  # of a layer that was pickled when its bias was a plain attribute
+            self._keep_bias(self.__dict__.pop("bias"), copy=False)
+
     def _apply(self, fn, recurse=True):
         held = self._buffers.get("bias")
         super()._apply(fn, recurse)

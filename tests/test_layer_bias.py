@@ -79,6 +79,19 @@ def test_a_state_is_not_loaded_into_what_was_given(kind):
     assert torch.equal(layer.bias, ramp()) and not given.any() and not other.bias.any()
 
 
+@pytest.mark.parametrize("kind", LAYERS)
+def test_layers_that_were_pickled_with_a_plain_attribute(kind):
+    for bias in (ramp(), None):
+        old = LAYERS[kind](bias)
+        old.__dict__["bias"] = old._buffers.pop("bias")
+        held = io.BytesIO()
+        torch.save(old, held)
+        held.seek(0)
+        layer = torch.load(held, weights_only=False)
+        assert "bias" not in layer.__dict__ and "bias" in layer._buffers and (layer.bias is None if bias is None else torch.equal(layer.bias, bias))
+        assert ("bias" in layer.state_dict()) == (bias is not None) and layer.to("meta") is layer
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", LAYERS)
 def test_restored_and_moved_layers_on_the_gpu(kind):
